@@ -1,4 +1,5 @@
-"""ctypes binding of ``libcresso_b200.so`` (C ABI in ``include/cresso_b200.h``).
+"""ctypes binding of ``libcresso_b200.so`` (C ABI in ``include/cresso_b200.h`` and,
+for the training operators, ``include/cresso_b200_train.h``).
 
 The library is built ahead of time (``python -m cresso_b200.build``).  There is
 no JIT and no fallback: if the shared library is missing or cannot be loaded,
@@ -67,6 +68,13 @@ EXPORTS = (
     "cresso_spectral64_run", "cresso_spectral_run_status", "cresso_status_copy", "cresso_copy_segments",
 )
 
+# entry points of include/cresso_b200_train.h
+TRAIN_EXPORTS = (
+    "cresso_embedding_gather", "cresso_embedding_grad_scratch_bytes", "cresso_embedding_grad", "cresso_block_norm",
+    "cresso_block_norm_grad_scratch_bytes", "cresso_block_norm_grad", "cresso_distill",
+)
+TRAIN_MAX_TOP = 1024  # CRESSO_TRAIN_MAX_TOP
+
 _lock = threading.Lock()
 _lib = None
 _load_error: Exception | None = None
@@ -109,6 +117,16 @@ def _declare(lib) -> None:
         "cresso_shape_workspace64_init": (ctypes.c_int, [_i64, _pi64, _i64, _pi64, _p, _p]),
         "cresso_spectral64_scratch_bytes": (ctypes.c_int, [_p, _i64, _p, _pi64]),
         "cresso_spectral64_run": (ctypes.c_int, [_p, _i64, _p, _p, _i64, _p]),
+        "cresso_embedding_gather": (ctypes.c_int, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _dbl, _p, _i64,
+                                                   _p]),
+        "cresso_embedding_grad_scratch_bytes": (ctypes.c_int, [_i64, _i64, _i64, _pi64]),
+        "cresso_embedding_grad": (ctypes.c_int, [_p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _dbl,
+                                                 _p, _i64, _i64, _p, _i64, _p]),
+        "cresso_block_norm": (ctypes.c_int, [_p] * 5 + [_i64] * 7 + [_dbl, _dbl, _p, _p, _p]),
+        "cresso_block_norm_grad_scratch_bytes": (ctypes.c_int, [_i64, _i64, _i64, _pi64]),
+        "cresso_block_norm_grad": (ctypes.c_int, [_p] * 7 + [_i64] * 7 + [_dbl, _dbl] + [_p] * 6 + [_i64, _p]),
+        "cresso_distill": (ctypes.c_int, [_p, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _dbl, _p, _p,
+                                          _p]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

@@ -2,7 +2,7 @@
 
 Compiles every ``csrc/*.cu`` for sm_100a with nvcc (no JIT, no torch
 extension machinery) and links one shared library with a plain C ABI
-(``include/cresso_b200.h``).  Run ``python -m cresso_b200.build``.
+(``include/cresso_b200.h``, ``include/cresso_b200_train.h``).  Run ``python -m cresso_b200.build``.
 """
 
 from __future__ import annotations
@@ -37,7 +37,7 @@ def sources() -> list[Path]:
 def _stale(obj: Path, src: Path) -> bool:
     if not obj.exists():
         return True
-    deps = [src] + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + [PKG.parent / "include" / "cresso_b200.h"]
+    deps = [src] + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list((PKG.parent / "include").glob("*.h"))
     return any(d.stat().st_mtime > obj.stat().st_mtime for d in deps)
 
 

@@ -1,0 +1,94 @@
+// Shared device helpers of the training operators (embedding, block norm, distillation).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/cresso_b200_train.h"
+#include "cresso_common.cuh"
+#include "cresso_status.h"
+
+namespace cresso {
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Element i of an array whose type is only known at run time (weights, gates,
+// teacher logits: small next to the rows they go with, so the branch is uniform
+// and its loads hit in cache).
+__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
+    if (dtype == CRESSO_DTYPE_F32) return static_cast<const float*>(p)[i];
+    if (dtype == CRESSO_DTYPE_F16) return to_float(static_cast<const __half*>(p)[i]);
+    return to_float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v) {
+    if (dtype == CRESSO_DTYPE_F32)
+        static_cast<float*>(p)[i] = v;
+    else if (dtype == CRESSO_DTYPE_F16)
+        static_cast<__half*>(p)[i] = from_float<__half>(v);
+    else
+        static_cast<__nv_bfloat16*>(p)[i] = from_float<__nv_bfloat16>(v);
+}
+
+__device__ __forceinline__ int64_t load_id(const void* p, int bytes, int64_t i) {
+    return bytes == 8 ? static_cast<const int64_t*>(p)[i] : (int64_t) static_cast<const int32_t*>(p)[i];
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// Sum over the block, the same in every thread and in a fixed order; `sh` holds
+// one float per warp.  Ends with a barrier, so that `sh` can be used again.
+__device__ __forceinline__ float block_sum(float v, float* sh) {
+    const int warps = blockDim.x >> 5;
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float s = (threadIdx.x & 31) < warps ? sh[threadIdx.x & 31] : 0.0f;
+    s = warp_sum(s);
+    __syncthreads();
+    return s;
+}
+__device__ __forceinline__ float block_max(float v, float* sh) {
+    const int warps = blockDim.x >> 5;
+    v = warp_max(v);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float s = (threadIdx.x & 31) < warps ? sh[threadIdx.x & 31] : -INFINITY;
+    s = warp_max(s);
+    __syncthreads();
+    return s;
+}
+
+inline bool train_dtype_ok(int64_t d) { return d == CRESSO_DTYPE_F32 || d == CRESSO_DTYPE_F16 || d == CRESSO_DTYPE_BF16; }
+inline int64_t dtype_bytes(int64_t d) { return d == CRESSO_DTYPE_F32 ? 4 : 2; }
+
+// f(T()) with the element type of a dtype code.
+template <typename F>
+int with_dtype(int64_t d, F f) {
+    if (d == CRESSO_DTYPE_F32) return f(float());
+    if (d == CRESSO_DTYPE_F16) return f(__half());
+    return f(__nv_bfloat16());
+}
+
+}  // namespace cresso
