@@ -10,6 +10,8 @@
 //   d_pre = sum_t d_y n,       d_post = sum_t dp q,  d_gate = scale sum e p.
 #include "train_common.cuh"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 namespace cresso {
@@ -60,98 +62,324 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(NormArgs a, const TR* __
         y[t * d + c] = from_float<TX>(value(c) * rh * load_any(a.pre_w, a.w_dtype, c));
 }
 
-struct RowStats {
-    float rx, rh, mean_dn_n, mean_dq_q;
+// ---------------------------------------------------------------- backward ---
+//
+// One pass over the rows.  A thread owns fixed columns, so the factors of a column
+// (pre = w_pre, A = scale gate w_post) and its sums over rows stay in registers.
+// Per row: six sums over the row in one reduction (the second mean is expanded,
+//   sum A x e = sum A x dh + Rh (sum A x dn - Rh m1 sum A x h),  m1 = mean(dn n)),
+// then e, d_x and the column sums B = sum e q and sum d_y n.  Both remaining
+// gradients follow from B, since the gate is constant over the rows of a unit:
+//   d_gate = scale w_post B,  d_post = scale gate B
+// (a gate with a row of its own for each row: d_gate per row, B over e q gate).
+// Rows come through `stages` stages of shared memory that cp.async fills ahead; each
+// thread copies and reads the same columns.  A row of more than 8192 columns is cut
+// over a cluster of 2 to 8 blocks, which add their six sums through distributed shared
+// memory.
+constexpr int kNormElems = 16;                         // columns of a thread
+constexpr int kNormBlockWidth = 512 * kNormElems;      // columns of a block
+constexpr int kNormMaxWidth = CRESSO_TRAIN_MAX_NORM_WIDTH;  // columns of a cluster of 8
+
+struct NormGrad {
+    NormArgs a;
+    const void *h, *x, *dh, *dy;
+    void *dres, *dx, *dgate;  // dgate: only with a gate row for each row
+    float *part_b, *part_pre;
+    int64_t units, units_per_gate;
+    int stages, cluster, block_width;
 };
 
-// Row-wise gradients; leaves the row's statistics for the column sums.
-template <typename TR, typename TX>
-__global__ void __launch_bounds__(kThreads) norm_grad_kernel(NormArgs a, const TR* __restrict__ h,
-                                                             const TX* __restrict__ x, const TR* __restrict__ dh,
-                                                             const TX* __restrict__ dy, TR* __restrict__ dres,
-                                                             TX* __restrict__ dx, RowStats* __restrict__ stats) {
-    __shared__ float sh[32];
-    const int64_t t = blockIdx.x, d = a.width;
-    const int64_t g0 = a.gate != nullptr ? t / a.rows_per_gate * d : 0;
-    const float inv_d = 1.0f / (float)d;
-    float sh2 = 0.0f, sx2 = 0.0f, sdn = 0.0f;
-    for (int64_t c = threadIdx.x; c < d; c += kThreads) {
-        const float hv = to_float(h[t * d + c]);
-        sh2 += hv * hv;
-        if (x != nullptr) {
-            const float xv = to_float(x[t * d + c]);
-            sx2 += xv * xv;
-        }
-        if (dy != nullptr) sdn += to_float(dy[t * d + c]) * load_any(a.pre_w, a.w_dtype, c) * hv;
+// Sums of 8 values over the block; every thread gets all of them, in the same order.
+// One barrier; `red` [warps][8] is used again two calls later at the earliest.
+__device__ __forceinline__ void sum8(float (&v)[8], float* red, int warps) {
+    const int lane = threadIdx.x & 31;
+    // a lane keeps half of its values in each of three exchanges, then sums the last one over 4 lanes
+    float w4[4], w2[2], w1;
+    const bool b4 = lane & 16, b3 = lane & 8, b2 = lane & 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w4[i] = (b4 ? v[4 + i] : v[i]) + __shfl_xor_sync(0xffffffffu, b4 ? v[i] : v[4 + i], 16);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        w2[i] = (b3 ? w4[2 + i] : w4[i]) + __shfl_xor_sync(0xffffffffu, b3 ? w4[i] : w4[2 + i], 8);
+    w1 = (b2 ? w2[1] : w2[0]) + __shfl_xor_sync(0xffffffffu, b2 ? w2[0] : w2[1], 4);
+    w1 += __shfl_xor_sync(0xffffffffu, w1, 2);
+    w1 += __shfl_xor_sync(0xffffffffu, w1, 1);
+    // lanes 4 i .. 4 i + 3 hold value i = 4 (lane bit 4) + 2 (lane bit 3) + (lane bit 2)
+    if (warps == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __shfl_sync(0xffffffffu, w1, 4 * i);
+        __syncwarp();
+        return;
     }
-    RowStats r;
-    r.rh = rsqrtf(block_sum(sh2, sh) * inv_d + a.eps);
-    r.rx = a.post_w != nullptr ? rsqrtf(block_sum(sx2, sh) * inv_d + a.eps) : 1.0f;
-    r.mean_dn_n = block_sum(sdn, sh) * inv_d * r.rh;
-    auto grad_h = [&](int64_t c) {
-        float e = dh != nullptr ? to_float(dh[t * d + c]) : 0.0f;
-        if (dy != nullptr) {
-            const float dn = to_float(dy[t * d + c]) * load_any(a.pre_w, a.w_dtype, c);
-            e += r.rh * (dn - to_float(h[t * d + c]) * r.rh * r.mean_dn_n);
-        }
-        return e;
-    };
-    auto grad_q = [&](int64_t c, float e) {
-        float v = a.scale * e;
-        if (a.gate != nullptr) v *= load_any(a.gate, a.gate_dtype, g0 + c);
-        if (a.post_w != nullptr) v *= load_any(a.post_w, a.w_dtype, c);
-        return v;
-    };
-    float sdq = 0.0f;
-    for (int64_t c = threadIdx.x; c < d; c += kThreads) {
-        const float e = grad_h(c);
-        if (x != nullptr && a.post_w != nullptr) sdq += grad_q(c, e) * to_float(x[t * d + c]);
+    if ((lane & 3) == 0) red[(threadIdx.x >> 5) * 8 + (lane >> 2)] = w1;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    for (int w = 0; w < warps; ++w) {
+        const float4 lo = reinterpret_cast<const float4*>(red)[2 * w], hi = reinterpret_cast<const float4*>(red)[2 * w + 1];
+        v[0] += lo.x;
+        v[1] += lo.y;
+        v[2] += lo.z;
+        v[3] += lo.w;
+        v[4] += hi.x;
+        v[5] += hi.y;
+        v[6] += hi.z;
+        v[7] += hi.w;
     }
-    r.mean_dq_q = block_sum(sdq, sh) * inv_d * r.rx;
-    for (int64_t c = threadIdx.x; c < d; c += kThreads) {
-        const float e = grad_h(c);
-        dres[t * d + c] = from_float<TR>(e);
-        if (x != nullptr) {
-            const float dq = grad_q(c, e);
-            dx[t * d + c] = from_float<TX>(
-                a.post_w != nullptr ? r.rx * (dq - to_float(x[t * d + c]) * r.rx * r.mean_dq_q) : dq);
-        }
-    }
-    if (threadIdx.x == 0) stats[t] = r;
 }
 
-// Column sums of the weight gradients and the gate gradient over the rows
-// [blockIdx.y * span, + span); one thread a column.  which: 0 post, 1 pre, 2 gate.
-template <typename TR, typename TX>
-__global__ void __launch_bounds__(kThreads) norm_columns_kernel(NormArgs a, int which, int64_t span,
-                                                                const TR* __restrict__ h, const TX* __restrict__ x,
-                                                                const TR* __restrict__ dh, const TX* __restrict__ dy,
-                                                                const RowStats* __restrict__ stats, void* out,
-                                                                int out_dtype) {
-    const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x, d = a.width;
-    if (c >= d) return;
-    const float pre = dy != nullptr ? load_any(a.pre_w, a.w_dtype, c) : 0.0f;
-    const float post = a.post_w != nullptr ? load_any(a.post_w, a.w_dtype, c) : 1.0f;
-    for (int64_t b = blockIdx.y; b * span < a.n; b += gridDim.y) {
-        float sum = 0.0f;
-        for (int64_t t = b * span; t < min(a.n, (b + 1) * span); ++t) {
-            const RowStats r = stats[t];
-            const float n = to_float(h[t * d + c]) * r.rh;
-            const float dyv = dy != nullptr ? to_float(dy[t * d + c]) : 0.0f;
-            if (which == 1) {
-                sum += dyv * n;
-                continue;
-            }
-            const float e = (dh != nullptr ? to_float(dh[t * d + c]) : 0.0f) + r.rh * (dyv * pre - n * r.mean_dn_n);
-            const float q = to_float(x[t * d + c]) * r.rx;
-            if (which == 2)
-                sum += a.scale * e * q * post;
-            else
-                sum += a.scale * e * q *
-                       (a.gate != nullptr ? load_any(a.gate, a.gate_dtype, t / a.rows_per_gate * d + c) : 1.0f);
+template <typename TR, typename TX, int VEC, bool OWN_GATE>
+__global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
+    constexpr int NV = kNormElems / VEC;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ __align__(16) float red[2][16 * 8];
+    const NormArgs& a = k.a;
+    const int tid = threadIdx.x, T = blockDim.x, warps = T >> 5;
+    __shared__ __align__(16) float peer_sums[2][8];
+    const int64_t width = a.width;
+    const int rank = k.cluster > 1 ? (int)(blockIdx.x % k.cluster) : 0;
+    const int64_t col0 = (int64_t)rank * k.block_width, worker = blockIdx.x / k.cluster, workers = gridDim.x / k.cluster;
+    const int d = (int)min((int64_t)k.block_width, width - col0);  // columns of this block
+    const int slots = (d + 7) / 8 * 8;
+    const float inv_d = 1.0f / (float)width;
+    // columns are counted from the block's first one: rows of `width` from here on
+    const TR *h = static_cast<const TR*>(k.h) + col0, *dh = k.dh != nullptr ? static_cast<const TR*>(k.dh) + col0 : nullptr;
+    const TX *x = k.x != nullptr ? static_cast<const TX*>(k.x) + col0 : nullptr;
+    const TX *dy = k.dy != nullptr ? static_cast<const TX*>(k.dy) + col0 : nullptr;
+    TR* dres = static_cast<TR*>(k.dres) + col0;
+    TX* dx = x != nullptr ? static_cast<TX*>(k.dx) + col0 : nullptr;
+    const int64_t pitch = align_up(width, 4);
+    const int stage_bytes = slots * 2 * (int)(sizeof(TR) + sizeof(TX));
+    auto stage_h = [&](int s) { return reinterpret_cast<TR*>(smem + s * stage_bytes); };
+    auto stage_dh = [&](int s) { return stage_h(s) + slots; };
+    auto stage_x = [&](int s) { return reinterpret_cast<TX*>(stage_h(s) + 2 * slots); };
+    auto stage_dy = [&](int s) { return stage_x(s) + slots; };
+    auto fetch = [&](int s, int64_t r) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = (v * T + tid) * VEC;
+            if (c >= d) break;
+            copy_vec<TR, VEC>(stage_h(s) + c, h + r * width + c);
+            if (x != nullptr) copy_vec<TX, VEC>(stage_x(s) + c, x + r * width + c);
+            if (dh != nullptr) copy_vec<TR, VEC>(stage_dh(s) + c, dh + r * width + c);
+            if (dy != nullptr) copy_vec<TX, VEC>(stage_dy(s) + c, dy + r * width + c);
         }
-        store_any(out, out_dtype, b * d + c, sum);
+    };
+    float pre[NV][VEC], post[NV][VEC], sum_b[NV][VEC], sum_pre[NV][VEC];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const int c = (v * T + tid) * VEC + j;
+            pre[v][j] = dy != nullptr && c < d ? load_any(a.pre_w, a.w_dtype, col0 + c) : 0.0f;
+            sum_pre[v][j] = 0.0f;
+        }
+    int parity = 0;
+    for (int64_t u = worker; u < k.units; u += workers) {
+        const int64_t g = u / k.units_per_gate, part = u % k.units_per_gate;
+        const int64_t r0 = g * a.rows_per_gate + part * a.rows_per_gate / k.units_per_gate;
+        const int64_t r1 = g * a.rows_per_gate + (part + 1) * a.rows_per_gate / k.units_per_gate;
+        for (int i = 0; i < k.stages - 1; ++i) {
+            if (r0 + i < r1) fetch(i, r0 + i);
+            copy_commit();
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const int c = (v * T + tid) * VEC + j;
+                float f = x != nullptr && c < d ? a.scale : 0.0f;
+                if (c < d && a.post_w != nullptr) f *= load_any(a.post_w, a.w_dtype, col0 + c);
+                if (c < d && a.gate != nullptr && !OWN_GATE) f *= load_any(a.gate, a.gate_dtype, g * width + col0 + c);
+                post[v][j] = f;  // A of above; with OWN_GATE without the gate
+                sum_b[v][j] = 0.0f;
+            }
+        int s = 0;
+        for (int64_t r = r0; r < r1; ++r) {
+            if (k.stages == 1) {
+                fetch(0, r);
+                copy_commit();
+            }
+            if (k.stages >= 4)
+                copy_wait<2>();
+            else if (k.stages == 3)
+                copy_wait<1>();
+            else
+                copy_wait<0>();
+            float t[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int c = (v * T + tid) * VEC;
+                if (c >= d) break;
+                float hv[VEC], xv[VEC] = {}, dhv[VEC] = {}, dyv[VEC] = {};
+                load_vec<TR, VEC>(stage_h(s) + c, hv);
+                if (x != nullptr) load_vec<TX, VEC>(stage_x(s) + c, xv);
+                if (dh != nullptr) load_vec<TR, VEC>(stage_dh(s) + c, dhv);
+                if (dy != nullptr) load_vec<TX, VEC>(stage_dy(s) + c, dyv);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float dn = dyv[j] * pre[v][j];
+                    float ax = post[v][j] * xv[j];
+                    if (OWN_GATE) ax *= load_any(a.gate, a.gate_dtype, r * width + col0 + c + j);
+                    t[0] += hv[j] * hv[j];
+                    t[1] += xv[j] * xv[j];
+                    t[2] += dn * hv[j];
+                    t[3] += ax * dhv[j];
+                    t[4] += ax * dn;
+                    t[5] += ax * hv[j];
+                }
+            }
+            sum8(t, red[parity], warps);
+            if (k.cluster > 1) {
+                namespace cg = cooperative_groups;
+                cg::cluster_group cluster = cg::this_cluster();
+                if (tid == 0)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) peer_sums[parity][i] = t[i];
+                cluster.sync();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[i] = 0.0f;
+                for (int q = 0; q < k.cluster; ++q) {
+                    const float* peer = cluster.map_shared_rank(peer_sums[parity], q);
+#pragma unroll
+                    for (int i = 0; i < 6; ++i) t[i] += peer[i];
+                }
+            }
+            parity ^= 1;
+            // every thread has left the previous row: its stage takes the row stages - 1 ahead
+            const int free_stage = s == 0 ? k.stages - 1 : s - 1;
+            if (k.stages > 1) {
+                if (r + k.stages - 1 < r1) fetch(free_stage, r + k.stages - 1);
+                copy_commit();
+            }
+            const float rh = rsqrtf(t[0] * inv_d + a.eps);
+            const float m1 = t[2] * rh * inv_d;
+            float rx = 1.0f, m2 = 0.0f;
+            if (a.post_w != nullptr) {
+                rx = rsqrtf(t[1] * inv_d + a.eps);
+                m2 = rx * inv_d * (t[3] + rh * (t[4] - rh * m1 * t[5]));
+            }
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int c = (v * T + tid) * VEC;
+                if (c >= d) break;
+                float hv[VEC], xv[VEC] = {}, ev[VEC] = {}, dyv[VEC] = {};
+                load_vec<TR, VEC>(stage_h(s) + c, hv);
+                if (x != nullptr) load_vec<TX, VEC>(stage_x(s) + c, xv);
+                if (dh != nullptr) load_vec<TR, VEC>(stage_dh(s) + c, ev);
+                if (dy != nullptr) load_vec<TX, VEC>(stage_dy(s) + c, dyv);
+                float dxv[VEC], dgv[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float n = hv[j] * rh, q = xv[j] * rx;
+                    ev[j] += rh * (dyv[j] * pre[v][j] - n * m1);
+                    float gate = 1.0f;
+                    if (OWN_GATE) gate = load_any(a.gate, a.gate_dtype, r * width + col0 + c + j);
+                    const float dq = post[v][j] * gate * ev[j];
+                    dxv[j] = rx * (dq - q * m2);
+                    dgv[j] = post[v][j] * ev[j] * q;
+                    sum_b[v][j] += ev[j] * gate * q;
+                    sum_pre[v][j] += dyv[j] * n;
+                }
+                store_vec<TR, VEC>(dres + r * width + c, ev);
+                if (x != nullptr) store_vec<TX, VEC>(dx + r * width + c, dxv);
+                if (OWN_GATE)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) store_any(k.dgate, a.gate_dtype, r * width + col0 + c + j, dgv[j]);
+            }
+            s = s == k.stages - 1 ? 0 : s + 1;
+        }
+        copy_wait<0>();
+        if (warps > 1) __syncthreads();  // the next unit fills the stages again
+        if (x != nullptr)
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int c = (v * T + tid) * VEC;
+                if (c < d) store_vec<float, VEC>(k.part_b + u * pitch + col0 + c, sum_b[v]);
+            }
     }
+    if (dy != nullptr)
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = (v * T + tid) * VEC;
+            if (c < d) store_vec<float, VEC>(k.part_pre + worker * pitch + col0 + c, sum_pre[v]);
+        }
+    if (k.cluster > 1) cooperative_groups::this_cluster().sync();  // a peer may still read this block's sums
+}
+
+// Sums of `count` consecutive rows of `part` (width columns, rows align_up(width, 4)
+// apart) for each group y: a block takes 32 columns, its 8 warps every eighth row.
+//   sum B of the group:  d_gate[y] = scale post B,  and scale gate[y] B into `out` or,
+//                        with more than one group, into row y of `post_rows`
+//   plain sums:          into `out` (which = 1: pre weight, 2: post weight over groups)
+struct NormColumns {
+    const float* part;
+    int64_t count, groups;
+    int which;  // 0: sum B
+    void *out, *dgate;
+    float* post_rows;
+};
+
+__global__ void __launch_bounds__(kThreads) norm_columns_kernel(NormArgs a, NormColumns k) {
+    __shared__ float sh[kWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane, d = a.width, pitch = align_up(d, 4);
+    for (int64_t g = blockIdx.y; g < k.groups; g += gridDim.y) {
+        float s = 0.0f;
+        if (c < d)
+            for (int64_t i = warp; i < k.count; i += kWarps) s += k.part[(g * k.count + i) * pitch + c];
+        sh[warp][lane] = s;
+        __syncthreads();
+        if (warp == 0 && c < d) {
+            s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) s += sh[w][lane];
+            if (k.which != 0) {
+                store_any(k.out, a.w_dtype, c, s);
+            } else {
+                s *= a.scale;
+                if (k.dgate != nullptr)
+                    store_any(k.dgate, a.gate_dtype, g * d + c,
+                              a.post_w != nullptr ? s * load_any(a.post_w, a.w_dtype, c) : s);
+                if (a.post_w != nullptr) {
+                    if (k.dgate != nullptr) s *= load_any(a.gate, a.gate_dtype, g * d + c);
+                    if (k.groups > 1)
+                        k.post_rows[g * pitch + c] = s;
+                    else
+                        store_any(k.out, a.w_dtype, c, s);
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Threads of a block, resident blocks to fill and the units of a backward pass, from
+// the sizes alone.
+struct NormGradPlan {
+    int threads, cluster, block_width;
+    int64_t workers, units, units_per_gate;  // workers: blocks or clusters
+    int64_t off_b, off_pre, off_post, bytes;
+};
+static NormGradPlan norm_grad_plan(int64_t n, int64_t width, int64_t gate_rows) {
+    NormGradPlan p{};
+    p.cluster = pow2_ceil(ceil_div(width, kNormBlockWidth));
+    p.block_width = (int)(p.cluster > 1 ? align_up(ceil_div(width, p.cluster), 8) : width);
+    p.threads = std::max(32, pow2_ceil(ceil_div(p.block_width, kNormElems)));
+    const int64_t want = 148 * std::max(1, 512 / p.threads) / p.cluster;
+    const bool own = gate_rows == n && n > 1;
+    const int64_t groups = own || gate_rows < 1 ? 1 : gate_rows;
+    const int64_t rows = n / groups;
+    p.units_per_gate = std::min(rows, std::max<int64_t>(1, want / groups));
+    p.units = groups * p.units_per_gate;
+    p.workers = std::min(p.units, want);
+    const int64_t pitch = 4 * align_up(width, 4);
+    p.off_b = 0;
+    p.off_pre = align_up(p.off_b + p.units * pitch, 256);
+    p.off_post = align_up(p.off_pre + p.workers * pitch, 256);
+    p.bytes = align_up(p.off_post + (groups > 1 ? groups : 0) * pitch, 256);
+    return p;
 }
 
 static int norm_check(const char* who, int64_t n, int64_t width, int64_t gate_rows, bool has_gate, int64_t res_dtype,
@@ -211,7 +439,8 @@ int cresso_block_norm(const void* residual, const void* x, const void* post_weig
 int cresso_block_norm_grad_scratch_bytes(int64_t n, int64_t width, int64_t gate_rows, int64_t* bytes) {
     CRESSO_REQUIRE(bytes != nullptr, CRESSO_EINVAL, "block_norm_grad_scratch_bytes: NULL result");
     CRESSO_REQUIRE(n >= 0 && width >= 0 && gate_rows >= 0, CRESSO_EINVAL, "block_norm_grad: negative size");
-    *bytes = align_up(n * (int64_t)sizeof(RowStats), 256);
+    CRESSO_REQUIRE(width <= kNormMaxWidth, CRESSO_EUNSUPPORTED, "block_norm_grad: width above %d", kNormMaxWidth);
+    *bytes = n == 0 || width == 0 ? 0 : norm_grad_plan(n, width, gate_rows).bytes;
     return CRESSO_OK;
 }
 
@@ -235,6 +464,7 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
             CRESSO_CUDA(cudaMemsetAsync(d_gate, 0, (size_t)(gate_rows * width * dtype_bytes(gate_dtype)), s));
         return CRESSO_OK;
     }
+    CRESSO_REQUIRE(width <= kNormMaxWidth, CRESSO_EUNSUPPORTED, "block_norm_grad: width above %d", kNormMaxWidth);
     CRESSO_REQUIRE(x != nullptr || (post_weight == nullptr && gate == nullptr), CRESSO_EINVAL,
                    "block_norm_grad: a post weight or a gate needs x");
     CRESSO_REQUIRE(h != nullptr && d_residual != nullptr && (d_h != nullptr || d_y != nullptr) &&
@@ -243,34 +473,89 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
     CRESSO_REQUIRE((x != nullptr) == (d_x != nullptr) && (post_weight != nullptr) == (d_post_weight != nullptr) &&
                        (d_y != nullptr) == (d_pre_weight != nullptr) && (gate != nullptr) == (d_gate != nullptr),
                    CRESSO_EINVAL, "block_norm_grad: an input without its gradient, or a gradient without its input");
-    int64_t need = 0;
-    const int sb = cresso_block_norm_grad_scratch_bytes(n, width, gate_rows, &need);
-    if (sb != CRESSO_OK) return sb;
-    CRESSO_REQUIRE(scratch != nullptr && scratch_bytes >= need, CRESSO_ESCRATCH,
-                   "block_norm_grad: scratch has %lld bytes, %lld are needed", (long long)scratch_bytes, (long long)need);
+    const NormGradPlan p = norm_grad_plan(n, width, gate != nullptr ? gate_rows : 0);
+    CRESSO_REQUIRE(scratch != nullptr && scratch_bytes >= p.bytes, CRESSO_ESCRATCH,
+                   "block_norm_grad: scratch has %lld bytes, %lld are needed", (long long)scratch_bytes,
+                   (long long)p.bytes);
+    CRESSO_REQUIRE(aligned_to(scratch, 16), CRESSO_EINVAL, "block_norm_grad: scratch is not 16-byte aligned");
     NvtxRange range("block_norm_grad n=%lld", (long long)n);
-    const NormArgs a{post_weight, pre_weight, gate, n, width, gate != nullptr ? n / gate_rows : n,
-                     (int)weight_dtype, (int)gate_dtype, (float)scale, (float)eps};
-    RowStats* stats = static_cast<RowStats*>(scratch);
-    return with_norm_types(res_dtype, act_dtype, [&](auto tr, auto tx) {
+    const bool own = gate != nullptr && gate_rows == n && n > 1;
+    const int64_t groups = gate == nullptr || own ? 1 : gate_rows;
+    NormGrad k{};
+    k.a = NormArgs{post_weight, pre_weight, gate, n, width, n / groups, (int)weight_dtype, (int)gate_dtype,
+                   (float)scale, (float)eps};
+    k.h = h;
+    k.x = x;
+    k.dh = d_h;
+    k.dy = d_y;
+    k.dres = d_residual;
+    k.dx = d_x;
+    k.dgate = own ? d_gate : nullptr;
+    unsigned char* base = static_cast<unsigned char*>(scratch);
+    k.part_b = reinterpret_cast<float*>(base + p.off_b);
+    k.part_pre = reinterpret_cast<float*>(base + p.off_pre);
+    k.units = p.units;
+    k.units_per_gate = p.units_per_gate;
+    k.cluster = p.cluster;
+    k.block_width = p.block_width;
+    const int64_t rb = dtype_bytes(res_dtype), xb = dtype_bytes(act_dtype);
+    const int stage = (int)(align_up(p.block_width, 8) * 2 * (rb + xb));
+    // as many blocks an SM as the registers admit where each of them has two stages, else
+    // as many stages as fit for one block
+    const int share = 220 * 1024 / std::max(1, 512 / p.threads) - 2048;
+    k.stages = 2 * stage <= share ? std::min(4, share / stage) : std::min(4, 220 * 1024 / stage);
+    const int smem = k.stages * stage;
+    // the widest accesses that the width and the addresses allow
+    auto fits = [&](int vec) {
+        if (width % vec != 0) return false;
+        const int64_t ar = std::min<int64_t>(16, vec * rb), ax = std::min<int64_t>(16, vec * xb);
+        return aligned_to(h, ar) && aligned_to(d_h, ar) && aligned_to(d_residual, ar) && aligned_to(x, ax) &&
+               aligned_to(d_y, ax) && aligned_to(d_x, ax);
+    };
+    const int rc = with_norm_types(res_dtype, act_dtype, [&](auto tr, auto tx) {
         using TR = decltype(tr);
         using TX = decltype(tx);
-        const TR *ph = static_cast<const TR*>(h), *pdh = static_cast<const TR*>(d_h);
-        const TX *px = static_cast<const TX*>(x), *pdy = static_cast<const TX*>(d_y);
-        norm_grad_kernel<TR, TX><<<(unsigned)n, kThreads, 0, s>>>(a, ph, px, pdh, pdy, static_cast<TR*>(d_residual),
-                                                                 static_cast<TX*>(d_x), stats);
-        CRESSO_LAUNCHED("norm_grad_kernel");
-        for (int which = 0; which < 3; ++which) {
-            void* out = which == 0 ? d_post_weight : which == 1 ? d_pre_weight : d_gate;
-            if (out == nullptr) continue;
-            const int64_t span = which == 2 ? a.rows_per_gate : n;
-            const dim3 grid((unsigned)ceil_div(width, kThreads), (unsigned)std::min<int64_t>(65535, n / span));
-            norm_columns_kernel<TR, TX><<<grid, kThreads, 0, s>>>(a, which, span, ph, px, pdh, pdy, stats, out,
-                                                                 (int)(which == 2 ? gate_dtype : weight_dtype));
-            CRESSO_LAUNCHED("norm_columns_kernel");
-        }
-        return (int)CRESSO_OK;
+        auto launch = [&](auto kernel) {
+            CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3((unsigned)(p.workers * p.cluster));
+            cfg.blockDim = dim3((unsigned)p.threads);
+            cfg.dynamicSmemBytes = (size_t)smem;
+            cfg.stream = s;
+            cudaLaunchAttribute attr{};
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = (unsigned)p.cluster;
+            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr;
+            cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+            CRESSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, k));
+            CRESSO_LAUNCHED("norm_grad_kernel");
+            return (int)CRESSO_OK;
+        };
+        if (fits(8)) return own ? launch(norm_grad_kernel<TR, TX, 8, true>) : launch(norm_grad_kernel<TR, TX, 8, false>);
+        if (fits(2)) return own ? launch(norm_grad_kernel<TR, TX, 2, true>) : launch(norm_grad_kernel<TR, TX, 2, false>);
+        return own ? launch(norm_grad_kernel<TR, TX, 1, true>) : launch(norm_grad_kernel<TR, TX, 1, false>);
     });
+    if (rc != CRESSO_OK) return rc;
+    auto columns = [&](const float* part, int64_t count, int64_t grp, int which, void* out, void* dgate) {
+        NormColumns c{part, count, grp, which, out, dgate, reinterpret_cast<float*>(base + p.off_post)};
+        NormArgs args = k.a;
+        if (own) args.gate = nullptr;
+        const dim3 grid((unsigned)ceil_div(width, 32), (unsigned)std::min<int64_t>(65535, grp));
+        norm_columns_kernel<<<grid, kThreads, 0, s>>>(args, c);
+        CRESSO_LAUNCHED("norm_columns_kernel");
+        return (int)CRESSO_OK;
+    };
+    if (post_weight != nullptr || (gate != nullptr && !own)) {
+        const int r1 = columns(k.part_b, p.units_per_gate, groups, 0, d_post_weight, own ? nullptr : d_gate);
+        if (r1 != CRESSO_OK) return r1;
+        if (post_weight != nullptr && groups > 1) {
+            const int r2 = columns(reinterpret_cast<float*>(base + p.off_post), groups, 1, 2, d_post_weight, nullptr);
+            if (r2 != CRESSO_OK) return r2;
+        }
+    }
+    if (d_y != nullptr) return columns(k.part_pre, p.workers, 1, 1, d_pre_weight, nullptr);
+    return CRESSO_OK;
 }
 
 }  // extern "C"

@@ -80,6 +80,72 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
     return s;
 }
 
+// VEC elements of T between memory and float registers, as the widest accesses that
+// VEC * sizeof(T) bytes allow; p is aligned to min(16, VEC * sizeof(T)).
+template <int BYTES>
+struct Word;
+template <>
+struct Word<2> { using type = unsigned short; };
+template <>
+struct Word<4> { using type = unsigned int; };
+template <>
+struct Word<8> { using type = uint2; };
+template <>
+struct Word<16> { using type = uint4; };
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float (&f)[VEC]) {
+    constexpr int B = VEC * (int)sizeof(T) < 16 ? VEC * (int)sizeof(T) : 16, N = VEC * (int)sizeof(T) / B;
+    using W = typename Word<B>::type;
+    union {
+        W w[N];
+        T t[VEC];
+    } u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) u.w[i] = reinterpret_cast<const W*>(p)[i];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = to_float(u.t[i]);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
+    constexpr int B = VEC * (int)sizeof(T) < 16 ? VEC * (int)sizeof(T) : 16, N = VEC * (int)sizeof(T) / B;
+    using W = typename Word<B>::type;
+    union {
+        W w[N];
+        T t[VEC];
+    } u;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) u.t[i] = from_float<T>(f[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) reinterpret_cast<W*>(p)[i] = u.w[i];
+}
+
+// Asynchronous copy of VEC elements from global to shared memory in 16-, 8- or 4-byte
+// pieces, counted by copy_commit / copy_wait; 2-byte pieces are copied at once.
+template <typename T, int VEC>
+__device__ __forceinline__ void copy_vec(T* dst, const T* src) {
+    constexpr int B = VEC * (int)sizeof(T) < 16 ? VEC * (int)sizeof(T) : 16, N = VEC * (int)sizeof(T) / B;
+    if constexpr (B == 2) {
+        *reinterpret_cast<unsigned short*>(dst) = *reinterpret_cast<const unsigned short*>(src);
+    } else {
+        const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+        const char* s = reinterpret_cast<const char*>(src);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (B == 16)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + 16 * i), "l"(s + 16 * i) : "memory");
+            else
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d + B * i), "l"(s + B * i), "n"(B)
+                             : "memory");
+        }
+    }
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
+inline bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
+
 inline bool train_dtype_ok(int64_t d) { return d == CRESSO_DTYPE_F32 || d == CRESSO_DTYPE_F16 || d == CRESSO_DTYPE_BF16; }
 inline int64_t dtype_bytes(int64_t d) { return d == CRESSO_DTYPE_F32 ? 4 : 2; }
 

@@ -7,8 +7,8 @@
  * counterpart in the reference, whose package holds the optimizer only.
  *
  * The conventions are those of cresso_b200.h: raw device pointers, an int status
- * (the message is read with cresso_last_error), caller-owned scratch whose size
- * is queried first, work ordered on the given stream of the current device,
+ * (the message is read with cresso_last_error), caller-owned scratch (16-byte
+ * aligned) whose size is queried first, work ordered on the given stream of the current device,
  * no allocation and no synchronisation.  Element types are CRESSO_DTYPE_F32,
  * _F16 and _BF16; sums, statistics and norms are float32 and every output is
  * rounded once.  The same inputs give the same bits in every run.
@@ -25,6 +25,7 @@ extern "C" {
 /* Bounds of the operators below; larger calls get CRESSO_EUNSUPPORTED. */
 enum { CRESSO_TRAIN_MAX_TOP = 1024 };          /* teacher entries of a row            */
 enum { CRESSO_TRAIN_MAX_ROWS = 2147483392 };   /* rows of a table, tokens, logit rows */
+enum { CRESSO_TRAIN_MAX_NORM_WIDTH = 65536 };  /* columns of a block norm             */
 
 /* ------------------------------------------------------------ embedding --- */
 
