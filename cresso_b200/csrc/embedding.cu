@@ -8,21 +8,63 @@
 #include "train_common.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cresso {
 
+// A row of `width` columns is taken by `tpr` threads (a power of two up to the block),
+// VEC columns an access, COLS / VEC accesses of a thread in flight.
+constexpr int kRowCols = 16;
+template <int VEC>
+constexpr int row_cols() { return VEC == 1 ? 8 : kRowCols; }
+static int threads_per_row(int64_t width, int vec) {
+    return (int)std::min<int64_t>(kThreads, pow2_ceil(ceil_div(width, vec)));
+}
+
+// f(std::integral_constant<int, VEC>) for the widest of 8, 4, 2 and 1 columns an access that
+// the sizes and the addresses allow.
+template <typename F>
+int with_vec(int64_t width, int64_t stride, const void* p, int64_t p_bytes, const void* q, int64_t q_bytes, F f) {
+    auto fits = [&](int vec) {
+        return width % vec == 0 && stride % vec == 0 && aligned_to(p, std::min<int64_t>(16, vec * p_bytes)) &&
+               aligned_to(q, std::min<int64_t>(16, vec * q_bytes));
+    };
+    if (fits(8)) return f(std::integral_constant<int, 8>());
+    if (fits(4)) return f(std::integral_constant<int, 4>());
+    if (fits(2)) return f(std::integral_constant<int, 2>());
+    return f(std::integral_constant<int, 1>());
+}
+
 // ------------------------------------------------------------------ lookup ---
 
-template <typename TW, typename TO>
+template <typename TW, typename TO, int VEC>
 __global__ void __launch_bounds__(kThreads) gather_kernel(const TW* __restrict__ w, int64_t rows, int64_t width,
                                                           int64_t stride, const void* __restrict__ tokens,
-                                                          int token_bytes, int64_t row0, float scale,
-                                                          TO* __restrict__ out) {
-    const int64_t t = blockIdx.x;
+                                                          int token_bytes, int64_t n, int64_t row0, float scale,
+                                                          TO* __restrict__ out, int tpr) {
+    constexpr int U = row_cols<VEC>() / VEC;
+    const int64_t t = (int64_t)blockIdx.x * (kThreads / tpr) + threadIdx.x / tpr;
+    if (t >= n) return;
     const uint64_t r = (uint64_t)load_id(tokens, token_bytes, t) - (uint64_t)row0;
     const bool inside = r < (uint64_t)rows;
-    for (int64_t c = threadIdx.x; c < width; c += kThreads)
-        out[t * width + c] = inside ? from_float<TO>(scale * to_float(w[(int64_t)r * stride + c])) : from_float<TO>(0.0f);
+    const TW* src = w + (inside ? (int64_t)r * stride : 0);
+    TO* dst = out + t * width;
+    for (int64_t c0 = (int64_t)(threadIdx.x & (tpr - 1)) * VEC; c0 < width; c0 += (int64_t)tpr * VEC * U) {
+        float f[U][VEC] = {};
+        if (inside)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t c = c0 + (int64_t)u * tpr * VEC;
+                if (c < width) load_vec<TW, VEC>(src + c, f[u]);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t c = c0 + (int64_t)u * tpr * VEC;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[u][j] = inside ? f[u][j] * scale : 0.0f;
+            if (c < width) store_vec<TO, VEC>(dst + c, f[u]);
+        }
+    }
 }
 
 // ---------------------------------------------------------------- the sort ---
@@ -36,6 +78,7 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const TW* __restrict__
 // of one row ranked by a warp match, which keeps the positions ascending.
 constexpr int kSortWarps = 32;
 constexpr int kSortThreads = kSortWarps * 32;
+constexpr int kSortBatch = 8;      // tokens of a thread in flight
 constexpr int kSortMaxRows = 1536;  // rows of a block: kSortWarps counters each, 192 KB of shared memory
 
 struct TokenWindow {
@@ -67,10 +110,15 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(TokenWindow win, int
     const int64_t i0 = warp * seg, i1 = min(win.n, i0 + seg);
     int* mine = cnt + warp * rb;
     int below = 0;
-    for (int64_t i = i0 + lane; i < i1; i += 32) {
-        const int r = window_row(win, i) - r0;
-        if (r >= 0 && r < nr) atomicAdd(&mine[r], 1);
-        below += (r < 0 && r >= -r0) ? 1 : 0;  // r = -1 - r0: no part
+    for (int64_t i = i0 + lane; i < i1; i += 32 * kSortBatch) {
+        int r[kSortBatch];
+#pragma unroll
+        for (int b = 0; b < kSortBatch; ++b) r[b] = window_row(win, i + 32 * b < i1 ? i + 32 * b : win.n) - r0;
+#pragma unroll
+        for (int b = 0; b < kSortBatch; ++b) {
+            if (r[b] >= 0 && r[b] < nr) atomicAdd(&mine[r[b]], 1);
+            below += (r[b] < 0 && r[b] >= -r0) ? 1 : 0;  // r = -1 - r0: no part
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) below += __shfl_xor_sync(0xffffffffu, below, o);
@@ -110,38 +158,158 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(TokenWindow win, int
         __syncthreads();
     }
     if (r0 + nr == win.rows && threadIdx.x == 0) row_start[win.rows] = carry;
-    for (int64_t i = i0; i < i1; i += 32) {
-        const int r = window_row(win, i + lane < i1 ? i + lane : win.n) - r0;
-        const bool in = r >= 0 && r < nr;
-        const unsigned any = __ballot_sync(0xffffffffu, in);
-        if (any == 0) continue;
-        if (in) {
-            const unsigned same = __match_any_sync(any, r);
-            const int rank = __popc(same & ((1u << lane) - 1u));
-            const int at = mine[r];
-            order[at + rank] = (int)(i + lane);
-            __syncwarp(any);
-            if (rank == 0) mine[r] = at + __popc(same);
+    for (int64_t i = i0; i < i1; i += 32 * kSortBatch) {
+        int rows[kSortBatch];
+#pragma unroll
+        for (int b = 0; b < kSortBatch; ++b)
+            rows[b] = window_row(win, i + 32 * b + lane < i1 ? i + 32 * b + lane : win.n) - r0;
+#pragma unroll
+        for (int b = 0; b < kSortBatch; ++b) {
+            const int r = rows[b];
+            const bool in = r >= 0 && r < nr;
+            const unsigned any = __ballot_sync(0xffffffffu, in);
+            if (any == 0) continue;
+            if (in) {
+                const unsigned same = __match_any_sync(any, r);
+                const int rank = __popc(same & ((1u << lane) - 1u));
+                const int at = mine[r];
+                order[at + rank] = (int)(i + 32 * b + lane);
+                __syncwarp(any);
+                if (rank == 0) mine[r] = at + __popc(same);
+            }
+            __syncwarp();
         }
-        __syncwarp();
     }
 }
 
-// One block sums one row.
-template <typename TG, typename TO>
-__global__ void __launch_bounds__(kThreads) grad_kernel(const TG* __restrict__ g, int64_t width, int64_t stride,
-                                                        const int* __restrict__ row_start,
-                                                        const int* __restrict__ order, float scale,
-                                                        TO* __restrict__ out, int accumulate) {
-    const int64_t r = blockIdx.x;
-    const int s = row_start[r], e = row_start[r + 1];
-    if (accumulate && s == e) return;
-    for (int64_t c = threadIdx.x; c < width; c += kThreads) {
-        float acc = 0.0f;
-        for (int j = s; j < e; ++j) acc += to_float(g[(int64_t)order[j] * stride + c]);
-        acc *= scale;
-        if (accumulate) acc += to_float(out[r * width + c]);
-        out[r * width + c] = from_float<TO>(acc);
+// ----------------------------------------------------------------- the sums ---
+//
+// A row with up to kTile positions is summed by one group of tpr threads and written,
+// zeros where it has none.  The order is also cut into tiles of kTile positions, and a
+// longer row is summed tile by tile into partial rows, which a second kernel adds in
+// their order: a row that holds a tenth of the tokens is spread over the GPU.  A tile
+// meets at most two such rows, one that reaches it from the left (partial 2 tile) and one
+// that begins inside and leaves it to the right (partial 2 tile + 1).
+constexpr int kTile = 32;
+constexpr int kSumCols = 8;  // columns of a thread
+
+// acc += rows order[s .. e) of g, columns c0 + u tpr VEC + j, in order.
+template <typename TG, int VEC, int U>
+__device__ __forceinline__ void add_rows(const TG* __restrict__ g, int64_t width, int64_t stride,
+                                         const int* __restrict__ order, int s, int e, int64_t c0, int tpr,
+                                         float (&acc)[U][VEC]) {
+    constexpr int P = VEC <= 2 ? 2 : 4;  // rows in flight: more of them would spill
+    for (int j = s; j < e; j += P) {
+        Raw<TG, VEC> f[P][U];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            if (j + p >= e) break;
+            const TG* row = g + (int64_t)order[j + p] * stride;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t c = c0 + (int64_t)u * tpr * VEC;
+                if (c < width) f[p][u].load_once(row + c);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            if (j + p >= e) break;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (c0 + (int64_t)u * tpr * VEC < width)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) acc[u][i] += f[p][u].get(i);
+        }
+    }
+}
+
+// out row = scale * acc (+ out row)
+template <typename TO, int VEC, int U>
+__device__ __forceinline__ void write_row(TO* __restrict__ out, int64_t width, int64_t c0, int tpr, float scale,
+                                          int accumulate, float (&acc)[U][VEC]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t c = c0 + (int64_t)u * tpr * VEC;
+        if (c >= width) continue;
+        float old[VEC] = {};
+        if (accumulate) load_vec<TO, VEC>(out + c, old);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[u][i] = acc[u][i] * scale + old[i];
+        store_vec<TO, VEC>(out + c, acc[u]);
+    }
+}
+
+struct GradSums {
+    const int *row_start, *order;
+    float* partial;  // [2 tiles][pitch]
+    int64_t rows, width, stride, tiles, pitch;
+    float scale;
+    int accumulate, tpr;
+};
+
+// Work items: the tiles first (the longest ones), then the rows.
+template <typename TG, typename TO, int VEC>
+__global__ void __launch_bounds__(kThreads, 4) grad_kernel(GradSums k, TokenWindow win, const TG* __restrict__ g,
+                                                        TO* __restrict__ out) {
+    constexpr int U = kSumCols / VEC;
+    const int tpr = k.tpr;
+    const int64_t item = (int64_t)blockIdx.x * (kThreads / tpr) + threadIdx.x / tpr;
+    const int64_t c0 = (int64_t)blockIdx.y * tpr * kSumCols + (int64_t)(threadIdx.x & (tpr - 1)) * VEC;
+    const int64_t r = item - k.tiles;
+    if (r >= k.rows) return;
+    // the range of the order to add, and a second one of a tile that meets two long rows
+    int s, e, s2 = 0, e2 = 0;
+    float* partial = nullptr;
+    if (r < 0) {
+        const int total = k.row_start[k.rows];
+        const int a = (int)item * kTile, b = min(a + kTile, total);
+        if (a >= total) return;
+        const int left = window_row(win, k.order[a]), right = window_row(win, k.order[b - 1]);
+        const int left_end = k.row_start[left + 1], right_start = k.row_start[right];
+        const bool left_long = left_end - k.row_start[left] > kTile;
+        const bool right_long = right != left && k.row_start[right + 1] - right_start > kTile;
+        if (!left_long && !right_long) return;
+        partial = k.partial + 2 * item * k.pitch;
+        s = a;
+        e = left_long ? min(left_end, b) : a;
+        s2 = right_start;
+        e2 = right_long ? b : right_start;
+    } else {
+        s = k.row_start[r];
+        e = k.row_start[r + 1];
+        if (e - s > kTile || (k.accumulate && s == e)) return;
+    }
+    for (int side = 0; side < 2; ++side) {
+        float acc[U][VEC] = {};
+        add_rows<TG, VEC, U>(g, k.width, k.stride, k.order, s, e, c0, tpr, acc);
+        if (partial == nullptr) {
+            write_row<TO, VEC, U>(out + r * k.width, k.width, c0, tpr, k.scale, k.accumulate, acc);
+            return;
+        }
+        if (s < e) write_row<float, VEC, U>(partial + side * k.pitch, k.width, c0, tpr, 1.0f, 0, acc);
+        s = s2;
+        e = e2;
+    }
+}
+
+// Adds the partial rows of the long row that begins in tile blockIdx.x; a thread has a column.
+template <typename TO>
+__global__ void __launch_bounds__(kThreads) grad_join_kernel(GradSums k, TokenWindow win, TO* __restrict__ out) {
+    const int total = k.row_start[k.rows];
+    const int64_t tile = blockIdx.x;
+    const int a = (int)tile * kTile, b = min(a + kTile, total);
+    if (a >= total) return;
+    const int64_t r = window_row(win, k.order[b - 1]);
+    const int s = k.row_start[r], e = k.row_start[r + 1];
+    if (e - s <= kTile || s < a) return;
+    const int64_t last = (e - 1) / kTile;
+    for (int64_t c = (int64_t)blockIdx.y * kThreads + threadIdx.x; c < k.width; c += (int64_t)gridDim.y * kThreads) {
+        float acc = k.partial[(2 * tile + (s > a ? 1 : 0)) * k.pitch + c];
+#pragma unroll 8
+        for (int64_t i = tile + 1; i <= last; ++i) acc += k.partial[2 * i * k.pitch + c];
+        acc *= k.scale;
+        if (k.accumulate) acc += to_float(out[r * k.width + c]);
+        out[r * k.width + c] = from_float<TO>(acc);
     }
 }
 
@@ -169,22 +337,27 @@ int cresso_embedding_gather(const void* weight, int64_t weight_dtype, int64_t ro
         return with_dtype(out_dtype, [&](auto to) {
             using TW = decltype(tw);
             using TO = decltype(to);
-            gather_kernel<TW, TO><<<(unsigned)n, kThreads, 0, (cudaStream_t)stream>>>(
-                static_cast<const TW*>(weight), rows, width, weight_stride, tokens, (int)token_bytes, row0,
-                (float)scale, static_cast<TO*>(out));
-            CRESSO_LAUNCHED("gather_kernel");
-            return (int)CRESSO_OK;
+            return with_vec(width, weight_stride, weight, sizeof(TW), out, sizeof(TO), [&](auto vec) {
+                constexpr int VEC = decltype(vec)::value;
+                const int tpr = threads_per_row(width, VEC);
+                gather_kernel<TW, TO, VEC><<<(unsigned)ceil_div(n, kThreads / tpr), kThreads, 0, (cudaStream_t)stream>>>(
+                    static_cast<const TW*>(weight), rows, width, weight_stride, tokens, (int)token_bytes, n, row0,
+                    (float)scale, static_cast<TO*>(out), tpr);
+                CRESSO_LAUNCHED("gather_kernel");
+                return (int)CRESSO_OK;
+            });
         });
     });
 }
 
-// scratch: row_start [rows + 1], order [n]
+// scratch: row_start [rows + 1], order [n], partial rows [2 ceil(n / kTile)][align_up(width, 4)]
+static int64_t grad_partials(int64_t n) { return n > kTile ? 2 * ceil_div(n, kTile) : 0; }
 int cresso_embedding_grad_scratch_bytes(int64_t n, int64_t rows, int64_t width, int64_t* bytes) {
     CRESSO_REQUIRE(bytes != nullptr, CRESSO_EINVAL, "embedding_grad_scratch_bytes: NULL result");
     CRESSO_REQUIRE(n >= 0 && rows >= 0 && width >= 0, CRESSO_EINVAL, "embedding_grad: negative size");
     CRESSO_REQUIRE(n <= CRESSO_TRAIN_MAX_ROWS && rows <= CRESSO_TRAIN_MAX_ROWS, CRESSO_EUNSUPPORTED,
                    "embedding_grad: more than 2^31 - 256 tokens or rows");
-    *bytes = align_up(4 * (rows + 1), 256) + align_up(4 * n, 256);
+    *bytes = align_up(4 * (rows + 1), 256) + align_up(4 * n, 256) + grad_partials(n) * align_up(width, 4) * 4;
     return CRESSO_OK;
 }
 
@@ -196,6 +369,8 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
                    "embedding_grad: element types are float32, float16 and bfloat16");
     CRESSO_REQUIRE(token_bytes == 4 || token_bytes == 8, CRESSO_EINVAL, "embedding_grad: tokens are int32 or int64");
     CRESSO_REQUIRE(grad_stride >= width, CRESSO_EINVAL, "embedding_grad: row stride below the width");
+    CRESSO_REQUIRE(width <= CRESSO_TRAIN_MAX_EMBEDDING_WIDTH, CRESSO_EUNSUPPORTED, "embedding_grad: width above %d",
+                   (int)CRESSO_TRAIN_MAX_EMBEDDING_WIDTH);
     int64_t need = 0;
     const int st = cresso_embedding_grad_scratch_bytes(n, rows, width, &need);
     if (st != CRESSO_OK) return st;
@@ -209,6 +384,7 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
     CRESSO_REQUIRE(grad != nullptr && tokens != nullptr, CRESSO_EINVAL, "embedding_grad: NULL pointer");
     CRESSO_REQUIRE(scratch != nullptr && scratch_bytes >= need, CRESSO_ESCRATCH,
                    "embedding_grad: scratch has %lld bytes, %lld are needed", (long long)scratch_bytes, (long long)need);
+    CRESSO_REQUIRE(aligned_to(scratch, 16), CRESSO_EINVAL, "embedding_grad: scratch is not 16-byte aligned");
     NvtxRange range("embedding_grad n=%lld rows=%lld", (long long)n, (long long)rows);
     int* row_start = static_cast<int*>(scratch);
     int* order = reinterpret_cast<int*>(static_cast<unsigned char*>(scratch) + align_up(4 * (rows + 1), 256));
@@ -220,14 +396,26 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
                                          kSortWarps * kSortMaxRows * 4));
     sort_kernel<<<(unsigned)ceil_div(rows, rb), kSortThreads, smem, s>>>(win, rb, row_start, order);
     CRESSO_LAUNCHED("sort_kernel");
+    GradSums k{row_start, order, reinterpret_cast<float*>(order + align_up(4 * n, 256) / 4), rows, width, grad_stride,
+               grad_partials(n) / 2, align_up(width, 4), (float)scale, accumulate != 0, 0};
     return with_dtype(grad_dtype, [&](auto tg) {
         return with_dtype(out_dtype, [&](auto to) {
             using TG = decltype(tg);
             using TO = decltype(to);
-            grad_kernel<TG, TO><<<(unsigned)rows, kThreads, 0, s>>>(static_cast<const TG*>(grad), width, grad_stride,
-                                                                   row_start, order, (float)scale,
-                                                                   static_cast<TO*>(out), accumulate != 0);
-            CRESSO_LAUNCHED("grad_kernel");
+            const int rc = with_vec(width, grad_stride, grad, sizeof(TG), out, sizeof(TO), [&](auto vec) {
+                constexpr int VEC = decltype(vec)::value;
+                k.tpr = threads_per_row(width, kSumCols);
+                const dim3 grid((unsigned)ceil_div(k.tiles + rows, kThreads / k.tpr),
+                                (unsigned)ceil_div(width, k.tpr * kSumCols));
+                grad_kernel<TG, TO, VEC><<<grid, kThreads, 0, s>>>(
+                    k, win, static_cast<const TG*>(grad), static_cast<TO*>(out));
+                CRESSO_LAUNCHED("grad_kernel");
+                return (int)CRESSO_OK;
+            });
+            if (rc != CRESSO_OK || k.tiles == 0) return rc;
+            const dim3 grid((unsigned)k.tiles, (unsigned)std::min<int64_t>(64, ceil_div(width, kThreads)));
+            grad_join_kernel<TO><<<grid, kThreads, 0, s>>>(k, win, static_cast<TO*>(out));
+            CRESSO_LAUNCHED("grad_join_kernel");
             return (int)CRESSO_OK;
         });
     });

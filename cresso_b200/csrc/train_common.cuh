@@ -93,18 +93,34 @@ struct Word<8> { using type = uint2; };
 template <>
 struct Word<16> { using type = uint4; };
 
+// VEC elements as they lie in memory.
+template <typename T, int VEC>
+struct Raw {
+    static constexpr int kBytes = VEC * (int)sizeof(T) < 16 ? VEC * (int)sizeof(T) : 16;
+    static constexpr int kWords = VEC * (int)sizeof(T) / kBytes;
+    using W = typename Word<kBytes>::type;
+    union {
+        W w[kWords];
+        T t[VEC];
+    };
+    __device__ __forceinline__ Raw() {}
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const W*>(p)[i];
+    }
+    __device__ __forceinline__ void load_once(const T* p) {  // read-only data
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const W*>(p) + i);
+    }
+    __device__ __forceinline__ float get(int i) const { return to_float(t[i]); }
+};
+
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T* p, float (&f)[VEC]) {
-    constexpr int B = VEC * (int)sizeof(T) < 16 ? VEC * (int)sizeof(T) : 16, N = VEC * (int)sizeof(T) / B;
-    using W = typename Word<B>::type;
-    union {
-        W w[N];
-        T t[VEC];
-    } u;
+    Raw<T, VEC> u;
+    u.load(p);
 #pragma unroll
-    for (int i = 0; i < N; ++i) u.w[i] = reinterpret_cast<const W*>(p)[i];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = to_float(u.t[i]);
+    for (int i = 0; i < VEC; ++i) f[i] = u.get(i);
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
