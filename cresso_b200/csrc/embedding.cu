@@ -83,21 +83,29 @@ constexpr int kSortMaxRows = 1536;  // rows of a block: kSortWarps counters each
 
 struct TokenWindow {
     const void* tokens;
-    int token_bytes;
     int has_padding;
     int64_t n, rows, row0, padding;
 };
 
-// Row of position i in the window, -1 when the token takes no part.
-__device__ __forceinline__ int window_row(const TokenWindow& w, int64_t i) {
-    if (i >= w.n) return -1;
-    const int64_t tok = load_id(w.tokens, w.token_bytes, i);
-    const uint64_t r = (uint64_t)tok - (uint64_t)w.row0;
-    return (r >= (uint64_t)w.rows || (w.has_padding && tok == w.padding)) ? -1 : (int)r;
+// Rows in the window of the positions i, i + 32, ... below end; -1 where there is no position
+// or the token takes no part.  All loads are issued before the first is used.
+template <typename ID>
+__device__ __forceinline__ void window_rows(const TokenWindow& w, int64_t i, int64_t end, int (&row)[kSortBatch]) {
+    ID id[kSortBatch];
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b) id[b] = static_cast<const ID*>(w.tokens)[min(i + 32 * b, w.n - 1)];
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b) {
+        const int64_t tok = (int64_t)id[b];
+        const uint64_t r = (uint64_t)tok - (uint64_t)w.row0;
+        const bool part = i + 32 * b < end && r < (uint64_t)w.rows && !(w.has_padding && tok == w.padding);
+        row[b] = part ? (int)r : -1;
+    }
 }
 
+template <typename ID>
 __global__ void __launch_bounds__(kSortThreads) sort_kernel(TokenWindow win, int rb, int* __restrict__ row_start,
-                                                            int* __restrict__ order) {
+                                                            int2* __restrict__ order) {
     extern __shared__ int cnt[];  // [kSortWarps][rb]
     __shared__ int warp_tot[kSortWarps], base_sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -111,13 +119,12 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(TokenWindow win, int
     int* mine = cnt + warp * rb;
     int below = 0;
     for (int64_t i = i0 + lane; i < i1; i += 32 * kSortBatch) {
-        int r[kSortBatch];
-#pragma unroll
-        for (int b = 0; b < kSortBatch; ++b) r[b] = window_row(win, i + 32 * b < i1 ? i + 32 * b : win.n) - r0;
+        int row[kSortBatch];
+        window_rows<ID>(win, i, i1, row);
 #pragma unroll
         for (int b = 0; b < kSortBatch; ++b) {
-            if (r[b] >= 0 && r[b] < nr) atomicAdd(&mine[r[b]], 1);
-            below += (r[b] < 0 && r[b] >= -r0) ? 1 : 0;  // r = -1 - r0: no part
+            if (row[b] >= r0 && row[b] - r0 < nr) atomicAdd(&mine[row[b] - r0], 1);
+            below += row[b] >= 0 && row[b] < r0 ? 1 : 0;
         }
     }
 #pragma unroll
@@ -159,13 +166,11 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(TokenWindow win, int
     }
     if (r0 + nr == win.rows && threadIdx.x == 0) row_start[win.rows] = carry;
     for (int64_t i = i0; i < i1; i += 32 * kSortBatch) {
-        int rows[kSortBatch];
-#pragma unroll
-        for (int b = 0; b < kSortBatch; ++b)
-            rows[b] = window_row(win, i + 32 * b + lane < i1 ? i + 32 * b + lane : win.n) - r0;
+        int row[kSortBatch];
+        window_rows<ID>(win, i + lane, i1, row);
 #pragma unroll
         for (int b = 0; b < kSortBatch; ++b) {
-            const int r = rows[b];
+            const int r = row[b] - r0;
             const bool in = r >= 0 && r < nr;
             const unsigned any = __ballot_sync(0xffffffffu, in);
             if (any == 0) continue;
@@ -173,7 +178,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(TokenWindow win, int
                 const unsigned same = __match_any_sync(any, r);
                 const int rank = __popc(same & ((1u << lane) - 1u));
                 const int at = mine[r];
-                order[at + rank] = (int)(i + 32 * b + lane);
+                order[at + rank] = make_int2((int)(i + 32 * b + lane), row[b]);
                 __syncwarp(any);
                 if (rank == 0) mine[r] = at + __popc(same);
             }
@@ -184,44 +189,17 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(TokenWindow win, int
 
 // ----------------------------------------------------------------- the sums ---
 //
-// A row with up to kTile positions is summed by one group of tpr threads and written,
-// zeros where it has none.  The order is also cut into tiles of kTile positions, and a
-// longer row is summed tile by tile into partial rows, which a second kernel adds in
-// their order: a row that holds a tenth of the tokens is spread over the GPU.  A tile
-// meets at most two such rows, one that reaches it from the left (partial 2 tile) and one
-// that begins inside and leaves it to the right (partial 2 tile + 1).
+// The order is cut into tiles of kTile positions, one work item each, so that the work is
+// even however the tokens fall.  A tile reads its positions kFlight at a time whatever rows
+// they belong to, and writes a row's sum where the row ends.  A row of up to kTile
+// positions belongs to the tile it begins in.  A longer one is summed tile by tile into
+// partial rows, which a second kernel adds in their order; a tile meets at most two such
+// rows, one that reaches it from the left (partial 2 tile) and one that begins inside and
+// leaves it to the right (partial 2 tile + 1).  Further items write the rows without a
+// token, kEmptyRows rows each.
 constexpr int kTile = 32;
+constexpr int kEmptyRows = 8;
 constexpr int kSumCols = 8;  // columns of a thread
-
-// acc += rows order[s .. e) of g, columns c0 + u tpr VEC + j, in order.
-template <typename TG, int VEC, int U>
-__device__ __forceinline__ void add_rows(const TG* __restrict__ g, int64_t width, int64_t stride,
-                                         const int* __restrict__ order, int s, int e, int64_t c0, int tpr,
-                                         float (&acc)[U][VEC]) {
-    constexpr int P = VEC <= 2 ? 2 : 4;  // rows in flight: more of them would spill
-    for (int j = s; j < e; j += P) {
-        Raw<TG, VEC> f[P][U];
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-            if (j + p >= e) break;
-            const TG* row = g + (int64_t)order[j + p] * stride;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t c = c0 + (int64_t)u * tpr * VEC;
-                if (c < width) f[p][u].load_once(row + c);
-            }
-        }
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-            if (j + p >= e) break;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (c0 + (int64_t)u * tpr * VEC < width)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) acc[u][i] += f[p][u].get(i);
-        }
-    }
-}
 
 // out row = scale * acc (+ out row)
 template <typename TO, int VEC, int U>
@@ -240,66 +218,95 @@ __device__ __forceinline__ void write_row(TO* __restrict__ out, int64_t width, i
 }
 
 struct GradSums {
-    const int *row_start, *order;
-    float* partial;  // [2 tiles][pitch]
+    const int* row_start;
+    const int2* order;  // (position, row)
+    float* partial;     // [2 tiles][pitch]
     int64_t rows, width, stride, tiles, pitch;
     float scale;
     int accumulate, tpr;
 };
 
-// Work items: the tiles first (the longest ones), then the rows.
 template <typename TG, typename TO, int VEC>
-__global__ void __launch_bounds__(kThreads, 4) grad_kernel(GradSums k, TokenWindow win, const TG* __restrict__ g,
-                                                        TO* __restrict__ out) {
+__global__ void __launch_bounds__(kThreads, VEC == 1 ? 3 : 4) grad_kernel(GradSums k, const TG* __restrict__ g,
+                                                           TO* __restrict__ out) {
     constexpr int U = kSumCols / VEC;
+    constexpr int kFlight = VEC <= 2 || sizeof(TG) == 4 ? 2 : 4;  // more of them would spill
     const int tpr = k.tpr;
     const int64_t item = (int64_t)blockIdx.x * (kThreads / tpr) + threadIdx.x / tpr;
     const int64_t c0 = (int64_t)blockIdx.y * tpr * kSumCols + (int64_t)(threadIdx.x & (tpr - 1)) * VEC;
-    const int64_t r = item - k.tiles;
-    if (r >= k.rows) return;
-    // the range of the order to add, and a second one of a tile that meets two long rows
-    int s, e, s2 = 0, e2 = 0;
-    float* partial = nullptr;
-    if (r < 0) {
-        const int total = k.row_start[k.rows];
-        const int a = (int)item * kTile, b = min(a + kTile, total);
-        if (a >= total) return;
-        const int left = window_row(win, k.order[a]), right = window_row(win, k.order[b - 1]);
-        const int left_end = k.row_start[left + 1], right_start = k.row_start[right];
-        const bool left_long = left_end - k.row_start[left] > kTile;
-        const bool right_long = right != left && k.row_start[right + 1] - right_start > kTile;
-        if (!left_long && !right_long) return;
-        partial = k.partial + 2 * item * k.pitch;
-        s = a;
-        e = left_long ? min(left_end, b) : a;
-        s2 = right_start;
-        e2 = right_long ? b : right_start;
-    } else {
-        s = k.row_start[r];
-        e = k.row_start[r + 1];
-        if (e - s > kTile || (k.accumulate && s == e)) return;
+    float acc[U][VEC] = {};
+    if (item >= k.tiles) {
+        if (k.accumulate) return;  // a block's last groups
+        const int64_t r0 = (item - k.tiles) * kEmptyRows;
+        int start[kEmptyRows + 1];
+#pragma unroll
+        for (int i = 0; i <= kEmptyRows; ++i) start[i] = k.row_start[min(r0 + i, k.rows)];
+#pragma unroll
+        for (int i = 0; i < kEmptyRows; ++i)
+            if (r0 + i < k.rows && start[i] == start[i + 1])
+                write_row<TO, VEC, U>(out + (r0 + i) * k.width, k.width, c0, tpr, 1.0f, 0, acc);
+        return;
     }
-    for (int side = 0; side < 2; ++side) {
-        float acc[U][VEC] = {};
-        add_rows<TG, VEC, U>(g, k.width, k.stride, k.order, s, e, c0, tpr, acc);
-        if (partial == nullptr) {
-            write_row<TO, VEC, U>(out + r * k.width, k.width, c0, tpr, k.scale, k.accumulate, acc);
-            return;
+    const int total = k.row_start[k.rows];
+    const int a = (int)item * kTile, b = min(a + kTile, total);
+    if (a >= total) return;
+    const int first = k.order[a].y, last = k.order[b - 1].y;
+    const int first_start = k.row_start[first], first_end = k.row_start[first + 1];
+    const int last_start = k.row_start[last], last_end = k.row_start[last + 1];
+    // [from, to): the positions this item adds
+    const int from = first_end - first_start > kTile || first_start == a ? a : min(first_end, b);
+    const int to = last_end - last_start > kTile ? b : last_start >= a ? last_end : from;
+    int row = -1, row_end = 0;
+    for (int j = from; j < to; j += kFlight) {
+        Raw<TG, VEC> f[kFlight][U];
+        int rows[kFlight];
+#pragma unroll
+        for (int p = 0; p < kFlight; ++p) {
+            const int2 o = k.order[min(j + p, to - 1)];
+            rows[p] = o.y;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t c = c0 + (int64_t)u * tpr * VEC;
+                if (c < k.width) f[p][u].load_once(g + (int64_t)o.x * k.stride + c);
+            }
         }
-        if (s < e) write_row<float, VEC, U>(partial + side * k.pitch, k.width, c0, tpr, 1.0f, 0, acc);
-        s = s2;
-        e = e2;
+#pragma unroll
+        for (int p = 0; p < kFlight; ++p) {
+            if (j + p >= to) break;
+            if (rows[p] != row) {
+                row = rows[p];
+                row_end = k.row_start[row + 1];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) acc[u][i] = 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (c0 + (int64_t)u * tpr * VEC < k.width)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) acc[u][i] += f[p][u].get(i);
+            if (j + p + 1 != row_end && j + p + 1 != to) continue;
+            // the row ends here, or the item does: a long row leaves a partial row
+            const int begin = row == first ? first_start : row == last ? last_start : 0;
+            const bool is_long = (row == first || row == last) && row_end - begin > kTile;
+            if (is_long)
+                write_row<float, VEC, U>(k.partial + (2 * item + (begin > a ? 1 : 0)) * k.pitch, k.width, c0, tpr, 1.0f,
+                                         0, acc);
+            else
+                write_row<TO, VEC, U>(out + (int64_t)row * k.width, k.width, c0, tpr, k.scale, k.accumulate, acc);
+        }
     }
 }
 
 // Adds the partial rows of the long row that begins in tile blockIdx.x; a thread has a column.
 template <typename TO>
-__global__ void __launch_bounds__(kThreads) grad_join_kernel(GradSums k, TokenWindow win, TO* __restrict__ out) {
+__global__ void __launch_bounds__(kThreads) grad_join_kernel(GradSums k, TO* __restrict__ out) {
     const int total = k.row_start[k.rows];
     const int64_t tile = blockIdx.x;
     const int a = (int)tile * kTile, b = min(a + kTile, total);
     if (a >= total) return;
-    const int64_t r = window_row(win, k.order[b - 1]);
+    const int64_t r = k.order[b - 1].y;
     const int s = k.row_start[r], e = k.row_start[r + 1];
     if (e - s <= kTile || s < a) return;
     const int64_t last = (e - 1) / kTile;
@@ -357,7 +364,7 @@ int cresso_embedding_grad_scratch_bytes(int64_t n, int64_t rows, int64_t width, 
     CRESSO_REQUIRE(n >= 0 && rows >= 0 && width >= 0, CRESSO_EINVAL, "embedding_grad: negative size");
     CRESSO_REQUIRE(n <= CRESSO_TRAIN_MAX_ROWS && rows <= CRESSO_TRAIN_MAX_ROWS, CRESSO_EUNSUPPORTED,
                    "embedding_grad: more than 2^31 - 256 tokens or rows");
-    *bytes = align_up(4 * (rows + 1), 256) + align_up(4 * n, 256) + grad_partials(n) * align_up(width, 4) * 4;
+    *bytes = align_up(4 * (rows + 1), 256) + align_up(8 * n, 256) + grad_partials(n) * align_up(width, 4) * 4;
     return CRESSO_OK;
 }
 
@@ -387,17 +394,24 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
     CRESSO_REQUIRE(aligned_to(scratch, 16), CRESSO_EINVAL, "embedding_grad: scratch is not 16-byte aligned");
     NvtxRange range("embedding_grad n=%lld rows=%lld", (long long)n, (long long)rows);
     int* row_start = static_cast<int*>(scratch);
-    int* order = reinterpret_cast<int*>(static_cast<unsigned char*>(scratch) + align_up(4 * (rows + 1), 256));
-    const TokenWindow win{tokens, (int)token_bytes, has_padding != 0, n, rows, row0, padding};
+    unsigned char* after = static_cast<unsigned char*>(scratch) + align_up(4 * (rows + 1), 256);
+    int2* order = reinterpret_cast<int2*>(after);
+    const TokenWindow win{tokens, has_padding != 0, n, rows, row0, padding};
     const int rb = (int)std::min<int64_t>(kSortMaxRows, std::max<int64_t>(1, ceil_div(rows, 148)));
     const int smem = kSortWarps * rb * 4;
-    if (smem > 48 * 1024)
-        CRESSO_CUDA(cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kSortWarps * kSortMaxRows * 4));
-    sort_kernel<<<(unsigned)ceil_div(rows, rb), kSortThreads, smem, s>>>(win, rb, row_start, order);
-    CRESSO_LAUNCHED("sort_kernel");
-    GradSums k{row_start, order, reinterpret_cast<float*>(order + align_up(4 * n, 256) / 4), rows, width, grad_stride,
-               grad_partials(n) / 2, align_up(width, 4), (float)scale, accumulate != 0, 0};
+    auto sort = [&](auto kernel) {
+        if (smem > 48 * 1024)
+            CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             kSortWarps * kSortMaxRows * 4));
+        kernel<<<(unsigned)ceil_div(rows, rb), kSortThreads, smem, s>>>(win, rb, row_start, order);
+        CRESSO_LAUNCHED("sort_kernel");
+        return (int)CRESSO_OK;
+    };
+    const int rs = token_bytes == 8 ? sort(sort_kernel<int64_t>) : sort(sort_kernel<int32_t>);
+    if (rs != CRESSO_OK) return rs;
+    GradSums k{row_start, order, reinterpret_cast<float*>(after + align_up(8 * n, 256)), rows, width, grad_stride,
+               ceil_div(n, kTile), align_up(width, 4), (float)scale, accumulate != 0, 0};
+    const int64_t items = k.tiles + (accumulate ? 0 : ceil_div(rows, kEmptyRows));
     return with_dtype(grad_dtype, [&](auto tg) {
         return with_dtype(out_dtype, [&](auto to) {
             using TG = decltype(tg);
@@ -405,16 +419,16 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
             const int rc = with_vec(width, grad_stride, grad, sizeof(TG), out, sizeof(TO), [&](auto vec) {
                 constexpr int VEC = decltype(vec)::value;
                 k.tpr = threads_per_row(width, kSumCols);
-                const dim3 grid((unsigned)ceil_div(k.tiles + rows, kThreads / k.tpr),
+                const dim3 grid((unsigned)ceil_div(items, kThreads / k.tpr),
                                 (unsigned)ceil_div(width, k.tpr * kSumCols));
                 grad_kernel<TG, TO, VEC><<<grid, kThreads, 0, s>>>(
-                    k, win, static_cast<const TG*>(grad), static_cast<TO*>(out));
+                    k, static_cast<const TG*>(grad), static_cast<TO*>(out));
                 CRESSO_LAUNCHED("grad_kernel");
                 return (int)CRESSO_OK;
             });
-            if (rc != CRESSO_OK || k.tiles == 0) return rc;
+            if (rc != CRESSO_OK || grad_partials(n) == 0) return rc;
             const dim3 grid((unsigned)k.tiles, (unsigned)std::min<int64_t>(64, ceil_div(width, kThreads)));
-            grad_join_kernel<TO><<<grid, kThreads, 0, s>>>(k, win, static_cast<TO*>(out));
+            grad_join_kernel<TO><<<grid, kThreads, 0, s>>>(k, static_cast<TO*>(out));
             CRESSO_LAUNCHED("grad_join_kernel");
             return (int)CRESSO_OK;
         });
