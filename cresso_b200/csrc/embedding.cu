@@ -26,8 +26,8 @@ static int threads_per_row(int64_t width, int vec) {
 template <typename F>
 int with_vec(int64_t width, int64_t stride, const void* p, int64_t p_bytes, const void* q, int64_t q_bytes, F f) {
     auto fits = [&](int vec) {
-        return width % vec == 0 && stride % vec == 0 && aligned_to(p, std::min<int64_t>(16, vec * p_bytes)) &&
-               aligned_to(q, std::min<int64_t>(16, vec * q_bytes));
+        return width % vec == 0 && stride % vec == 0 && aligned_to(p, std::min<int64_t>(32, vec * p_bytes)) &&
+               aligned_to(q, std::min<int64_t>(32, vec * q_bytes));
     };
     if (fits(8)) return f(std::integral_constant<int, 8>());
     if (fits(4)) return f(std::integral_constant<int, 4>());
@@ -55,89 +55,117 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const TW* __restrict__
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int64_t c = c0 + (int64_t)u * tpr * VEC;
-                if (c < width) load_vec<TW, VEC>(src + c, f[u]);
+                if (c < width) load_global<TW, VEC>(src + c, f[u]);
             }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t c = c0 + (int64_t)u * tpr * VEC;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) f[u][j] = inside ? f[u][j] * scale : 0.0f;
-            if (c < width) store_vec<TO, VEC>(dst + c, f[u]);
+            if (c < width) store_global<TO, VEC>(dst + c, f[u]);
         }
     }
 }
 
 // ---------------------------------------------------------------- the sort ---
 //
-// One launch without any exchange between blocks: block b owns the rows
-// [b * rb, (b + 1) * rb) and reads all tokens (they sit in L2).  Its 32 warps take
-// equal contiguous ranges of positions.  First scan: each warp counts its tokens
-// per row in shared memory, and the tokens below the block's rows, whose number is
-// where the block's part of the order begins.  A scan over (row, warp) turns the
-// counts into first places; the second scan puts each position at its place, lanes
-// of one row ranked by a warp match, which keeps the positions ascending.
-constexpr int kSortWarps = 32;
-constexpr int kSortThreads = kSortWarps * 32;
-constexpr int kSortBatch = 8;      // tokens of a thread in flight
-constexpr int kSortMaxRows = 1536;  // rows of a block: kSortWarps counters each, 192 KB of shared memory
+// One launch without any exchange between blocks: of `blocks` (a power of two) blocks,
+// block b owns the rows r = b modulo blocks, so that frequent rows, which often have
+// neighbouring numbers, fall to different blocks.  The order holds the rows block by
+// block.  Every block reads all tokens (they sit in L2); its warps take equal contiguous
+// ranges of positions.  First scan: each warp counts its tokens per owned row in shared
+// memory, and the tokens of the blocks before, whose number is where the block's part of
+// the order begins.  A scan over (row, warp) turns the counts into first places; the second
+// scan puts each position at its place, lanes of one row ranked by a warp match, which
+// keeps the positions of a row ascending.
+constexpr int kSortMaxWarps = 32;
+constexpr int kSortBatch = 8;         // tokens of a thread in flight
+constexpr int kSortCounters = 49152;  // of a block, row ends among them: 192 KB of shared memory
+constexpr int kSortLogBlocks = 7;     // at least 128 blocks
 
 struct TokenWindow {
     const void* tokens;
-    int has_padding;
-    int64_t n, rows, row0, padding;
+    int64_t n, row0;
+    uint32_t rows, padding_row;  // padding_row: 2^32 - 1 where no token is left out
+    int log_blocks;
 };
 
-// Rows in the window of the positions i, i + 32, ... below end; -1 where there is no position
-// or the token takes no part.  All loads are issued before the first is used.
+constexpr uint32_t kNoRow = 0xffffffffu;
+constexpr uint32_t kLastOfRow = 0x80000000u;  // mark of a row's last position in the order
+
+// Rows in the window of the positions i, i + 32, ... below end; kNoRow where there is no
+// position or the token takes no part.  All loads are issued before the first is used.
 template <typename ID>
-__device__ __forceinline__ void window_rows(const TokenWindow& w, int64_t i, int64_t end, int (&row)[kSortBatch]) {
+__device__ __forceinline__ void window_rows(const TokenWindow& w, int i, int end, uint32_t (&row)[kSortBatch]) {
     ID id[kSortBatch];
+    const ID* tokens = static_cast<const ID*>(w.tokens);
+    const bool whole = i + 32 * (kSortBatch - 1) < end;
+    if (whole) {
 #pragma unroll
-    for (int b = 0; b < kSortBatch; ++b) id[b] = static_cast<const ID*>(w.tokens)[min(i + 32 * b, w.n - 1)];
+        for (int b = 0; b < kSortBatch; ++b) id[b] = tokens[(int64_t)i + 32 * b];
+    } else {
+#pragma unroll
+        for (int b = 0; b < kSortBatch; ++b) id[b] = tokens[(int64_t)i + 32 * b < end ? (int64_t)i + 32 * b : end - 1];
+    }
 #pragma unroll
     for (int b = 0; b < kSortBatch; ++b) {
-        const int64_t tok = (int64_t)id[b];
-        const uint64_t r = (uint64_t)tok - (uint64_t)w.row0;
-        const bool part = i + 32 * b < end && r < (uint64_t)w.rows && !(w.has_padding && tok == w.padding);
-        row[b] = part ? (int)r : -1;
+        const uint64_t d = (uint64_t)(int64_t)id[b] - (uint64_t)w.row0;
+        const uint32_t r = (uint32_t)d;
+        const bool part = (uint32_t)(d >> 32) == 0 && r < w.rows && r != w.padding_row;
+        row[b] = part && (whole || (int64_t)i + 32 * b < end) ? r : kNoRow;
     }
 }
 
 template <typename ID>
-__global__ void __launch_bounds__(kSortThreads) sort_kernel(TokenWindow win, int rb, int* __restrict__ row_start,
-                                                            int2* __restrict__ order) {
-    extern __shared__ int cnt[];  // [kSortWarps][rb]
-    __shared__ int warp_tot[kSortWarps], base_sh;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int r0 = blockIdx.x * rb;
-    const int nr = (int)min((int64_t)rb, win.rows - r0);
-    for (int i = threadIdx.x; i < kSortWarps * rb; i += kSortThreads) cnt[i] = 0;
+__global__ void __launch_bounds__(kSortMaxWarps * 32) sort_kernel(TokenWindow win, int nr_max, int2* __restrict__ range,
+                                                                  int2* __restrict__ order, int* __restrict__ total) {
+    next_kernel_may_start();
+    extern __shared__ int cnt[];  // [warps][nr_max], then the end of each row [nr_max]
+    __shared__ int warp_tot[kSortMaxWarps], base_sh;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, threads = blockDim.x, warps = threads >> 5;
+    const int log_b = win.log_blocks, blocks = 1 << log_b, b0 = blockIdx.x;
+    const int nr = (int)((win.rows + (uint32_t)(blocks - 1 - b0)) >> log_b);
+    for (int i = threadIdx.x; i < warps * nr_max; i += threads) cnt[i] = 0;
     if (threadIdx.x == 0) base_sh = 0;
     __syncthreads();
-    const int64_t seg = ceil_div(ceil_div(win.n, kSortWarps), 32) * 32;
-    const int64_t i0 = warp * seg, i1 = min(win.n, i0 + seg);
-    int* mine = cnt + warp * rb;
+    const int64_t seg = ceil_div(ceil_div(win.n, warps), 32) * 32;
+    const int i0 = (int)min(win.n, warp * seg), i1 = (int)min(win.n, (warp + 1) * seg);
+    int *mine = cnt + warp * nr_max, *row_end = cnt + warps * nr_max;
+    auto owner = [&](uint32_t row) { return row == kNoRow ? blocks : (int)(row & (uint32_t)(blocks - 1)); };
     int below = 0;
-    for (int64_t i = i0 + lane; i < i1; i += 32 * kSortBatch) {
-        int row[kSortBatch];
-        window_rows<ID>(win, i, i1, row);
+    auto count = [&](const uint32_t(&row)[kSortBatch]) {
 #pragma unroll
         for (int b = 0; b < kSortBatch; ++b) {
-            if (row[b] >= r0 && row[b] - r0 < nr) atomicAdd(&mine[row[b] - r0], 1);
-            below += row[b] >= 0 && row[b] < r0 ? 1 : 0;
+            const int o = owner(row[b]);
+            if (o == b0) atomicAdd(&mine[row[b] >> log_b], 1);
+            below += o < b0 ? 1 : 0;
         }
+    };
+    // the rows of two batches stay in registers for the second scan, which is all of a warp's
+    // range up to 16384 tokens
+    constexpr int kStep = 32 * kSortBatch;
+    uint32_t held[2][kSortBatch];
+    if (i0 < i1) window_rows<ID>(win, i0 + lane, i1, held[0]);
+    if (i0 + kStep < i1) window_rows<ID>(win, i0 + kStep + lane, i1, held[1]);
+    if (i0 < i1) count(held[0]);
+    if (i0 + kStep < i1) count(held[1]);
+    for (int64_t i = (int64_t)i0 + 2 * kStep; i < i1; i += kStep) {
+        uint32_t row[kSortBatch];
+        window_rows<ID>(win, (int)i + lane, i1, row);
+        count(row);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) below += __shfl_xor_sync(0xffffffffu, below, o);
     if (lane == 0 && below) atomicAdd(&base_sh, below);
     __syncthreads();
-    // exclusive scan over the rows of the block, kSortThreads rows a turn
+    // exclusive scan over the rows of the block, a row a thread and `threads` rows a turn
     int carry = base_sh;
-    for (int c = 0; c < nr; c += kSortThreads) {
+    for (int c = 0; c < nr; c += threads) {
         const int r = c + threadIdx.x;
         int tot = 0;
         if (r < nr)
-            for (int w = 0; w < kSortWarps; ++w) tot += cnt[w * rb + r];
+#pragma unroll 8
+            for (int w = 0; w < warps; ++w) tot += cnt[w * nr_max + r];
         int incl = tot;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -147,59 +175,68 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(TokenWindow win, int
         if (lane == 31) warp_tot[warp] = incl;
         __syncthreads();
         int before = 0, all = 0;
-        for (int w = 0; w < kSortWarps; ++w) {
+        for (int w = 0; w < warps; ++w) {
             const int v = warp_tot[w];
             before += w < warp ? v : 0;
             all += v;
         }
         int at = carry + before + incl - tot;
         if (r < nr) {
-            row_start[r0 + r] = at;
-            for (int w = 0; w < kSortWarps; ++w) {
-                const int v = cnt[w * rb + r];
-                cnt[w * rb + r] = at;
-                at += v;
-            }
+            range[((int64_t)r << log_b) + b0] = make_int2(at, at + tot);
+            row_end[r] = at + tot;
+            if (tot > 0)
+#pragma unroll 8
+                for (int w = 0; w < warps; ++w) {
+                    const int v = cnt[w * nr_max + r];
+                    cnt[w * nr_max + r] = at;
+                    at += v;
+                }
         }
         carry += all;
         __syncthreads();
     }
-    if (r0 + nr == win.rows && threadIdx.x == 0) row_start[win.rows] = carry;
-    for (int64_t i = i0; i < i1; i += 32 * kSortBatch) {
-        int row[kSortBatch];
-        window_rows<ID>(win, i + lane, i1, row);
+    if (b0 == blocks - 1 && threadIdx.x == 0) *total = carry;
+    auto place = [&](const uint32_t(&row)[kSortBatch], int i) {
 #pragma unroll
         for (int b = 0; b < kSortBatch; ++b) {
-            const int r = row[b] - r0;
-            const bool in = r >= 0 && r < nr;
+            const bool in = owner(row[b]) == b0;
             const unsigned any = __ballot_sync(0xffffffffu, in);
             if (any == 0) continue;
             if (in) {
+                const int r = (int)(row[b] >> log_b);
                 const unsigned same = __match_any_sync(any, r);
                 const int rank = __popc(same & ((1u << lane) - 1u));
                 const int at = mine[r];
-                order[at + rank] = make_int2((int)(i + 32 * b + lane), row[b]);
+                const uint32_t last = at + rank + 1 == row_end[r] ? kLastOfRow : 0;
+                order[at + rank] = make_int2(i + lane + 32 * b, (int)(row[b] | last));
                 __syncwarp(any);
                 if (rank == 0) mine[r] = at + __popc(same);
             }
             __syncwarp();
         }
+    };
+    if (i0 < i1) place(held[0], i0);
+    if (i0 + kStep < i1) place(held[1], i0 + kStep);
+    for (int64_t i = (int64_t)i0 + 2 * kStep; i < i1; i += kStep) {
+        uint32_t row[kSortBatch];
+        window_rows<ID>(win, (int)i + lane, i1, row);
+        place(row, (int)i);
     }
 }
 
 // ----------------------------------------------------------------- the sums ---
 //
-// The order is cut into tiles of kTile positions, one work item each, so that the work is
-// even however the tokens fall.  A tile reads its positions kFlight at a time whatever rows
-// they belong to, and writes a row's sum where the row ends.  A row of up to kTile
+// The order is cut into tiles of `tile` positions, one work item each, so that the work is
+// even however the tokens fall.  A tile fetches its positions ahead whatever rows they
+// belong to, and writes a row's sum where the row ends.  A row of up to `tile`
 // positions belongs to the tile it begins in.  A longer one is summed tile by tile into
 // partial rows, which a second kernel adds in their order; a tile meets at most two such
 // rows, one that reaches it from the left (partial 2 tile) and one that begins inside and
 // leaves it to the right (partial 2 tile + 1).  Further items write the rows without a
 // token, kEmptyRows rows each.
-constexpr int kTile = 32;
 constexpr int kEmptyRows = 8;
-constexpr int kSumCols = 8;  // columns of a thread
+constexpr int kSumCols = 8;    // columns of a thread
+constexpr int kJoinCols = 128;
 
 // out row = scale * acc (+ out row)
 template <typename TO, int VEC, int U>
@@ -213,112 +250,164 @@ __device__ __forceinline__ void write_row(TO* __restrict__ out, int64_t width, i
         if (accumulate) load_vec<TO, VEC>(out + c, old);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[u][i] = acc[u][i] * scale + old[i];
-        store_vec<TO, VEC>(out + c, acc[u]);
+        store_global<TO, VEC>(out + c, acc[u]);
     }
 }
 
 struct GradSums {
-    const int* row_start;
-    const int2* order;  // (position, row)
+    const int2* range;  // (begin, end) of each row in the order
+    const int2* order;  // (position, row | kLastOfRow)
+    const int* total;   // length of the order
     float* partial;     // [2 tiles][pitch]
     int64_t rows, width, stride, tiles, pitch;
     float scale;
-    int accumulate, tpr;
+    int accumulate, tpr, tile;
 };
 
+__device__ __forceinline__ int order_row(int2 entry) { return entry.y & (int)~kLastOfRow; }
+
 template <typename TG, typename TO, int VEC>
-__global__ void __launch_bounds__(kThreads, VEC == 1 ? 3 : 4) grad_kernel(GradSums k, const TG* __restrict__ g,
+__global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG* __restrict__ g,
                                                            TO* __restrict__ out) {
     constexpr int U = kSumCols / VEC;
-    constexpr int kFlight = VEC <= 2 || sizeof(TG) == 4 ? 2 : 4;  // more of them would spill
+    constexpr int kDepth = 16 / sizeof(TG);  // positions in 32 KB of shared memory
+    __shared__ __align__(16) TG ring[kDepth * kThreads * kSumCols];
     const int tpr = k.tpr;
     const int64_t item = (int64_t)blockIdx.x * (kThreads / tpr) + threadIdx.x / tpr;
     const int64_t c0 = (int64_t)blockIdx.y * tpr * kSumCols + (int64_t)(threadIdx.x & (tpr - 1)) * VEC;
     float acc[U][VEC] = {};
+    next_kernel_may_start();
+    previous_kernel_done();
     if (item >= k.tiles) {
         if (k.accumulate) return;  // a block's last groups
         const int64_t r0 = (item - k.tiles) * kEmptyRows;
-        int start[kEmptyRows + 1];
+        bool empty[kEmptyRows];
 #pragma unroll
-        for (int i = 0; i <= kEmptyRows; ++i) start[i] = k.row_start[min(r0 + i, k.rows)];
+        for (int i = 0; i < kEmptyRows; ++i) {
+            const int2 at = k.range[min(r0 + i, k.rows - 1)];
+            empty[i] = r0 + i < k.rows && at.x == at.y;
+        }
 #pragma unroll
         for (int i = 0; i < kEmptyRows; ++i)
-            if (r0 + i < k.rows && start[i] == start[i + 1])
-                write_row<TO, VEC, U>(out + (r0 + i) * k.width, k.width, c0, tpr, 1.0f, 0, acc);
+            if (empty[i]) write_row<TO, VEC, U>(out + (r0 + i) * k.width, k.width, c0, tpr, 1.0f, 0, acc);
         return;
     }
-    const int total = k.row_start[k.rows];
-    const int a = (int)item * kTile, b = min(a + kTile, total);
+    const int total = *k.total;
+    const int a = (int)item * k.tile, b = min(a + k.tile, total);
     if (a >= total) return;
-    const int first = k.order[a].y, last = k.order[b - 1].y;
-    const int first_start = k.row_start[first], first_end = k.row_start[first + 1];
-    const int last_start = k.row_start[last], last_end = k.row_start[last + 1];
+    const int first = order_row(k.order[a]), last = order_row(k.order[b - 1]);
+    const int2 fr = k.range[first], lr = k.range[last];
+    const bool first_long = fr.y - fr.x > k.tile, last_long = lr.y - lr.x > k.tile;
     // [from, to): the positions this item adds
-    const int from = first_end - first_start > kTile || first_start == a ? a : min(first_end, b);
-    const int to = last_end - last_start > kTile ? b : last_start >= a ? last_end : from;
-    int row = -1, row_end = 0;
-    for (int j = from; j < to; j += kFlight) {
-        Raw<TG, VEC> f[kFlight][U];
-        int rows[kFlight];
+    const int from = first_long || fr.x == a ? a : min(fr.y, b);
+    const int to = last_long ? b : lr.x >= a ? lr.y : from;
+    if (from >= to) return;
+    // each thread fetches its columns of the next kDepth - 1 positions ahead
+    TG* mine = ring + threadIdx.x * VEC;
+    auto fetch = [&](int j, int slot) {
+        const TG* src = g + (int64_t)k.order[j].x * k.stride + c0;
 #pragma unroll
-        for (int p = 0; p < kFlight; ++p) {
-            const int2 o = k.order[min(j + p, to - 1)];
-            rows[p] = o.y;
+        for (int u = 0; u < U; ++u)
+            if (c0 + (int64_t)u * tpr * VEC < k.width)
+                copy_vec<TG, VEC>(mine + (slot * U + u) * kThreads * VEC, src + u * tpr * VEC);
+    };
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t c = c0 + (int64_t)u * tpr * VEC;
-                if (c < k.width) f[p][u].load_once(g + (int64_t)o.x * k.stride + c);
+    for (int p = 0; p < kDepth - 1; ++p) {
+        if (from + p < to) fetch(from + p, p);
+        copy_commit();
+    }
+    int slot = 0;
+    for (int j = from; j < to; ++j) {
+        const int mark = k.order[j].y;
+        copy_wait<kDepth - 2>();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c0 + (int64_t)u * tpr * VEC < k.width) {
+                float f[VEC];
+                load_vec<TG, VEC>(mine + (slot * U + u) * kThreads * VEC, f);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) acc[u][i] += f[i];
             }
-        }
+        if (j + kDepth - 1 < to) fetch(j + kDepth - 1, slot == 0 ? kDepth - 1 : slot - 1);
+        copy_commit();
+        slot = slot == kDepth - 1 ? 0 : slot + 1;
+        if (mark >= 0 && j + 1 < to) continue;
+        // the row ends here, or the item does: a long row leaves a partial row
+        const int row = mark & (int)~kLastOfRow;
+        if ((row == first && first_long) || (row == last && last_long))
+            write_row<float, VEC, U>(k.partial + (2 * item + ((row == first ? fr.x : lr.x) > a ? 1 : 0)) * k.pitch,
+                                     k.width, c0, tpr, 1.0f, 0, acc);
+        else
+            write_row<TO, VEC, U>(out + (int64_t)row * k.width, k.width, c0, tpr, k.scale, k.accumulate, acc);
 #pragma unroll
-        for (int p = 0; p < kFlight; ++p) {
-            if (j + p >= to) break;
-            if (rows[p] != row) {
-                row = rows[p];
-                row_end = k.row_start[row + 1];
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) acc[u][i] = 0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (c0 + (int64_t)u * tpr * VEC < k.width)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) acc[u][i] += f[p][u].get(i);
-            if (j + p + 1 != row_end && j + p + 1 != to) continue;
-            // the row ends here, or the item does: a long row leaves a partial row
-            const int begin = row == first ? first_start : row == last ? last_start : 0;
-            const bool is_long = (row == first || row == last) && row_end - begin > kTile;
-            if (is_long)
-                write_row<float, VEC, U>(k.partial + (2 * item + (begin > a ? 1 : 0)) * k.pitch, k.width, c0, tpr, 1.0f,
-                                         0, acc);
-            else
-                write_row<TO, VEC, U>(out + (int64_t)row * k.width, k.width, c0, tpr, k.scale, k.accumulate, acc);
-        }
+            for (int i = 0; i < VEC; ++i) acc[u][i] = 0.0f;
     }
 }
 
-// Adds the partial rows of the long row that begins in tile blockIdx.x; a thread has a column.
+// Adds the partial rows of the long rows that begin in the tiles [256 x, 256 x + 256): a
+// thread looks at a tile each, then the block takes every gridDim.z-th of the rows found, 128
+// columns of it, and its eight warps add every eighth partial row.
 template <typename TO>
 __global__ void __launch_bounds__(kThreads) grad_join_kernel(GradSums k, TO* __restrict__ out) {
-    const int total = k.row_start[k.rows];
-    const int64_t tile = blockIdx.x;
-    const int a = (int)tile * kTile, b = min(a + kTile, total);
-    if (a >= total) return;
-    const int64_t r = k.order[b - 1].y;
-    const int s = k.row_start[r], e = k.row_start[r + 1];
-    if (e - s <= kTile || s < a) return;
-    const int64_t last = (e - 1) / kTile;
-    for (int64_t c = (int64_t)blockIdx.y * kThreads + threadIdx.x; c < k.width; c += (int64_t)gridDim.y * kThreads) {
-        float acc = k.partial[(2 * tile + (s > a ? 1 : 0)) * k.pitch + c];
-#pragma unroll 8
-        for (int64_t i = tile + 1; i <= last; ++i) acc += k.partial[2 * i * k.pitch + c];
-        acc *= k.scale;
-        if (k.accumulate) acc += to_float(out[r * k.width + c]);
-        out[r * k.width + c] = from_float<TO>(acc);
+    __shared__ int found[kThreads], warp_count[kWarps];
+    __shared__ __align__(16) float part[kWarps][kJoinCols];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t tile = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    previous_kernel_done();
+    const int total = *k.total;
+    int row = -1;
+    if (tile < k.tiles && tile * k.tile < total) {
+        const int a = (int)tile * k.tile;
+        const int r = order_row(k.order[min(a + k.tile, total) - 1]);
+        const int2 at = k.range[r];
+        if (at.x >= a && at.y - at.x > k.tile) row = r;
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, row >= 0);
+    if (lane == 0) warp_count[warp] = __popc(here);
+    __syncthreads();
+    int before = 0, count = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        before += w < warp ? warp_count[w] : 0;
+        count += warp_count[w];
+    }
+    if (row >= 0) found[before + __popc(here & ((1u << lane) - 1u))] = row;
+    __syncthreads();
+    const int64_t c = (int64_t)blockIdx.y * kJoinCols + 4 * lane, own = (int64_t)blockIdx.y * kJoinCols + threadIdx.x;
+    for (int i = blockIdx.z; i < count; i += gridDim.z) {
+        const int64_t r = found[i];
+        const int2 at = k.range[r];
+        const int64_t t0 = at.x / k.tile, t1 = (at.y - 1) / k.tile;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (c < k.width) {
+#pragma unroll 4
+            for (int64_t t = t0 + warp; t <= t1; t += kWarps) {
+                const float4 v = *reinterpret_cast<const float4*>(
+                    k.partial + (2 * t + (t == t0 && at.x > t0 * k.tile ? 1 : 0)) * k.pitch + c);
+                acc.x += v.x;
+                acc.y += v.y;
+                acc.z += v.z;
+                acc.w += v.w;
+            }
+        }
+        *reinterpret_cast<float4*>(&part[warp][4 * lane]) = acc;
+        __syncthreads();
+        if (threadIdx.x < kJoinCols && own < k.width) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) v += part[w][threadIdx.x];
+            v *= k.scale;
+            if (k.accumulate) v += to_float(out[r * k.width + own]);
+            out[r * k.width + own] = from_float<TO>(v);
+        }
+        __syncthreads();
     }
 }
+
+// Positions of a tile: few where there are few tokens, so that their latencies overlap.
+static int grad_tile(int64_t n) { return n <= 4096 ? 8 : n <= 32768 ? 32 : 128; }
 
 }  // namespace cresso
 
@@ -357,14 +446,29 @@ int cresso_embedding_gather(const void* weight, int64_t weight_dtype, int64_t ro
     });
 }
 
-// scratch: row_start [rows + 1], order [n], partial rows [2 ceil(n / kTile)][align_up(width, 4)]
-static int64_t grad_partials(int64_t n) { return n > kTile ? 2 * ceil_div(n, kTile) : 0; }
+// scratch: range [rows], order [n], total, partial rows [2 tiles][align_up(width, 4)]
+struct GradScratch {
+    int64_t tile, tiles, order, total, partial, bytes;
+};
+static GradScratch grad_scratch(int64_t n, int64_t rows, int64_t width) {
+    GradScratch p{};
+    p.tile = grad_tile(n);
+    p.tiles = ceil_div(n, p.tile);
+    p.order = align_up(8 * rows, 256);
+    p.total = p.order + align_up(8 * n, 256);
+    p.partial = p.total + 256;
+    p.bytes = p.partial + (p.tiles > 1 ? 2 * p.tiles * align_up(width, 4) * 4 : 0);
+    return p;
+}
+
 int cresso_embedding_grad_scratch_bytes(int64_t n, int64_t rows, int64_t width, int64_t* bytes) {
     CRESSO_REQUIRE(bytes != nullptr, CRESSO_EINVAL, "embedding_grad_scratch_bytes: NULL result");
     CRESSO_REQUIRE(n >= 0 && rows >= 0 && width >= 0, CRESSO_EINVAL, "embedding_grad: negative size");
     CRESSO_REQUIRE(n <= CRESSO_TRAIN_MAX_ROWS && rows <= CRESSO_TRAIN_MAX_ROWS, CRESSO_EUNSUPPORTED,
                    "embedding_grad: more than 2^31 - 256 tokens or rows");
-    *bytes = align_up(4 * (rows + 1), 256) + align_up(8 * n, 256) + grad_partials(n) * align_up(width, 4) * 4;
+    CRESSO_REQUIRE(width <= CRESSO_TRAIN_MAX_EMBEDDING_WIDTH, CRESSO_EUNSUPPORTED, "embedding_grad: width above %d",
+                   (int)CRESSO_TRAIN_MAX_EMBEDDING_WIDTH);
+    *bytes = grad_scratch(n, rows, width).bytes;
     return CRESSO_OK;
 }
 
@@ -376,8 +480,6 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
                    "embedding_grad: element types are float32, float16 and bfloat16");
     CRESSO_REQUIRE(token_bytes == 4 || token_bytes == 8, CRESSO_EINVAL, "embedding_grad: tokens are int32 or int64");
     CRESSO_REQUIRE(grad_stride >= width, CRESSO_EINVAL, "embedding_grad: row stride below the width");
-    CRESSO_REQUIRE(width <= CRESSO_TRAIN_MAX_EMBEDDING_WIDTH, CRESSO_EUNSUPPORTED, "embedding_grad: width above %d",
-                   (int)CRESSO_TRAIN_MAX_EMBEDDING_WIDTH);
     int64_t need = 0;
     const int st = cresso_embedding_grad_scratch_bytes(n, rows, width, &need);
     if (st != CRESSO_OK) return st;
@@ -393,24 +495,30 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
                    "embedding_grad: scratch has %lld bytes, %lld are needed", (long long)scratch_bytes, (long long)need);
     CRESSO_REQUIRE(aligned_to(scratch, 16), CRESSO_EINVAL, "embedding_grad: scratch is not 16-byte aligned");
     NvtxRange range("embedding_grad n=%lld rows=%lld", (long long)n, (long long)rows);
-    int* row_start = static_cast<int*>(scratch);
-    unsigned char* after = static_cast<unsigned char*>(scratch) + align_up(4 * (rows + 1), 256);
-    int2* order = reinterpret_cast<int2*>(after);
-    const TokenWindow win{tokens, has_padding != 0, n, rows, row0, padding};
-    const int rb = (int)std::min<int64_t>(kSortMaxRows, std::max<int64_t>(1, ceil_div(rows, 148)));
-    const int smem = kSortWarps * rb * 4;
+    const GradScratch at = grad_scratch(n, rows, width);
+    unsigned char* base = static_cast<unsigned char*>(scratch);
+    int2 *ranges = reinterpret_cast<int2*>(base), *order = reinterpret_cast<int2*>(base + at.order);
+    int* total = reinterpret_cast<int*>(base + at.total);
+    // warps that have a batch of tokens each (eight scan the rows quickly); blocks whose counters fit shared memory
+    const int warps = std::max(8, std::min(kSortMaxWarps, pow2_ceil(ceil_div(n, 32 * kSortBatch))));
+    int log_blocks = kSortLogBlocks;
+    while ((warps + 1) * ceil_div(rows, (int64_t)1 << log_blocks) > kSortCounters) ++log_blocks;
+    const int nr_max = (int)ceil_div(rows, (int64_t)1 << log_blocks);
+    const uint64_t pad = (uint64_t)padding - (uint64_t)row0;
+    const TokenWindow win{tokens, n, row0, (uint32_t)rows, has_padding != 0 && pad < (uint64_t)rows ? (uint32_t)pad : kNoRow,
+                          log_blocks};
+    const int smem = (warps + 1) * nr_max * 4;
     auto sort = [&](auto kernel) {
         if (smem > 48 * 1024)
-            CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             kSortWarps * kSortMaxRows * 4));
-        kernel<<<(unsigned)ceil_div(rows, rb), kSortThreads, smem, s>>>(win, rb, row_start, order);
+            CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortCounters * 4));
+        kernel<<<1u << log_blocks, warps * 32, smem, s>>>(win, nr_max, ranges, order, total);
         CRESSO_LAUNCHED("sort_kernel");
         return (int)CRESSO_OK;
     };
     const int rs = token_bytes == 8 ? sort(sort_kernel<int64_t>) : sort(sort_kernel<int32_t>);
     if (rs != CRESSO_OK) return rs;
-    GradSums k{row_start, order, reinterpret_cast<float*>(after + align_up(8 * n, 256)), rows, width, grad_stride,
-               ceil_div(n, kTile), align_up(width, 4), (float)scale, accumulate != 0, 0};
+    GradSums k{ranges, order, total, reinterpret_cast<float*>(base + at.partial), rows, width, grad_stride, at.tiles,
+               align_up(width, 4), (float)scale, accumulate != 0, 0, (int)at.tile};
     const int64_t items = k.tiles + (accumulate ? 0 : ceil_div(rows, kEmptyRows));
     return with_dtype(grad_dtype, [&](auto tg) {
         return with_dtype(out_dtype, [&](auto to) {
@@ -421,14 +529,16 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
                 k.tpr = threads_per_row(width, kSumCols);
                 const dim3 grid((unsigned)ceil_div(items, kThreads / k.tpr),
                                 (unsigned)ceil_div(width, k.tpr * kSumCols));
-                grad_kernel<TG, TO, VEC><<<grid, kThreads, 0, s>>>(
-                    k, static_cast<const TG*>(grad), static_cast<TO*>(out));
+                CRESSO_CUDA(launch_overlapped(grad_kernel<TG, TO, VEC>, grid, kThreads, 0, s, k,
+                                              static_cast<const TG*>(grad), static_cast<TO*>(out)));
                 CRESSO_LAUNCHED("grad_kernel");
                 return (int)CRESSO_OK;
             });
-            if (rc != CRESSO_OK || grad_partials(n) == 0) return rc;
-            const dim3 grid((unsigned)k.tiles, (unsigned)std::min<int64_t>(64, ceil_div(width, kThreads)));
-            grad_join_kernel<TO><<<grid, kThreads, 0, s>>>(k, static_cast<TO*>(out));
+            if (rc != CRESSO_OK || k.tiles == 1) return rc;  // one tile holds no long row
+            const int64_t parts = ceil_div(width, kJoinCols);
+            const dim3 grid((unsigned)ceil_div(k.tiles, kThreads), (unsigned)parts,
+                            (unsigned)std::max<int64_t>(1, std::min<int64_t>(32, 512 / parts)));
+            CRESSO_CUDA(launch_overlapped(grad_join_kernel<TO>, grid, kThreads, 0, s, k, static_cast<TO*>(out)));
             CRESSO_LAUNCHED("grad_join_kernel");
             return (int)CRESSO_OK;
         });

@@ -136,6 +136,49 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
     for (int i = 0; i < N; ++i) reinterpret_cast<W*>(p)[i] = u.w[i];
 }
 
+// The same for global memory, with 32-byte accesses (sm_100) where VEC elements have 32
+// bytes: a warp's access then covers whole sectors.  p is aligned to min(32, VEC *
+// sizeof(T)).  load_global reads data that the kernel does not write.
+struct alignas(32) Word32 {
+    uint32_t w[8];
+};
+__device__ __forceinline__ Word32 load_word32(const void* p) {
+    Word32 v;
+    asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+        : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void store_word32(void* p, const Word32& v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v.w[0]), "r"(v.w[1]),
+                 "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
+                 : "memory");
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void load_global(const T* p, float (&f)[VEC]) {
+    if constexpr (VEC * sizeof(T) == 32) {
+        const Word32 v = load_word32(p);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = __uint_as_float(v.w[i]);
+    } else {
+        Raw<T, VEC> u;
+        u.load_once(p);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = u.get(i);
+    }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_global(T* p, const float (&f)[VEC]) {
+    if constexpr (VEC * sizeof(T) == 32) {
+        Word32 v;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v.w[i] = __float_as_uint(f[i]);
+        store_word32(p, v);
+    } else {
+        store_vec<T, VEC>(p, f);
+    }
+}
+
 // Asynchronous copy of VEC elements from global to shared memory in 16-, 8- or 4-byte
 // pieces, counted by copy_commit / copy_wait; 2-byte pieces are copied at once.
 template <typename T, int VEC>
@@ -159,6 +202,25 @@ __device__ __forceinline__ void copy_vec(T* dst, const T* src) {
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
+// Launch of a kernel that begins with previous_kernel_done() and may be set up while the
+// stream's previous kernel still runs.
+__device__ __forceinline__ void previous_kernel_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void next_kernel_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename K, typename... Args>
+cudaError_t launch_overlapped(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 inline bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
 

@@ -25,7 +25,7 @@ extern "C" {
 /* Bounds of the operators below; larger calls get CRESSO_EUNSUPPORTED. */
 enum { CRESSO_TRAIN_MAX_TOP = 1024 };          /* teacher entries of a row            */
 enum { CRESSO_TRAIN_MAX_ROWS = 2147483392 };   /* rows of a table, tokens, logit rows */
-enum { CRESSO_TRAIN_MAX_EMBEDDING_WIDTH = 1 << 24 };
+enum { CRESSO_TRAIN_MAX_EMBEDDING_WIDTH = 4194240 }; /* columns of a table row     */
 enum { CRESSO_TRAIN_MAX_NORM_WIDTH = 65536 };  /* columns of a block norm             */
 
 /* ------------------------------------------------------------ embedding --- */
