@@ -1,16 +1,18 @@
 // Distillation from a teacher's top logits: the loss of each row and the gradient
-// of the student's logits, from one reading of the row where the gradient is wanted.
+// of the student's logits, from one reading of the row.
 //
 // A row has V student logits z, K teacher entries (id, u), a weight w and the
 // temperature tau:
 //   p = softmax(u / tau) over the valid entries,  q = softmax(z / tau) over V,
 //   loss = w tau^2 sum_k p_k (log p_k - log q[id_k]),
 //   dz_v = w tau (q_v - P_v),  P_v = sum of p_k with id_k = v.
-// Exponentials are taken relative to the row's maximum and summed in float32.  A
-// NaN or +inf logit makes its row NaN through the sum; a row of -inf alone has
-// q = 0.  Repeated ids: every entry forms the whole P of its id, so that all of
-// them write the same value.
+// Exponentials are 2^((z - max) log2(e) / tau): the difference first, so that their error
+// stays that of the difference however large the logits are; sums are float32.  A NaN or
+// +inf logit makes its row NaN through the sum; a row of -inf alone has q = 0.  Repeated
+// ids: every entry forms the whole P of its id, so that all of them write the same value.
 #include "train_common.cuh"
+
+#include <cooperative_groups.h>
 
 namespace cresso {
 
@@ -22,95 +24,271 @@ struct DistillArgs {
     float tau;
 };
 
-constexpr int kDistillThreads = 512;
-
 // The teacher's side of a row in shared memory.
 struct TopList {
     int id[CRESSO_TRAIN_MAX_TOP];   // -1: not valid
     float p[CRESSO_TRAIN_MAX_TOP];  // teacher probability
-    float z[CRESSO_TRAIN_MAX_TOP];  // student logit / tau at the id
+    float z[CRESSO_TRAIN_MAX_TOP];  // student logit at the id
+    float entropy;                  // sum of p log p
+    int any;                        // a valid entry exists
 };
 
-// Fills ids and probabilities; returns sum_k p_k log p_k in every thread, and in
-// `any` whether a valid entry exists.
-__device__ __forceinline__ float load_teacher(const DistillArgs& a, int64_t t, TopList& top, float* sh, bool& any) {
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float exp2_fast(float x) {  // relative error 2^-22
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Fills the list with one warp; the block sees it after its next barrier.
+template <typename T>
+__device__ __forceinline__ void load_teacher(const DistillArgs& a, int64_t t, const T* row, TopList& top) {
+    const int lane = threadIdx.x & 31;
     float m = -INFINITY;
-    bool valid_here = false;
-    for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
+    for (int k = lane; k < a.k; k += 32) {
         const int64_t id = load_id(a.ids, a.id_bytes, t * a.k + k);
-        const float u = load_any(a.teacher, a.teacher_dtype, t * a.k + k) / a.tau;
+        const float u = load_any(a.teacher, a.teacher_dtype, t * a.k + k);
         const bool valid = id >= 0 && id < a.vocab && u != -INFINITY;
         top.id[k] = valid ? (int)id : -1;
         top.p[k] = u;
-        if (valid) {
-            m = fmaxf(m, u);
-            valid_here = true;
-        }
+        top.z[k] = valid ? to_float(row[id]) : 0.0f;
+        if (valid) m = fmaxf(m, u);
     }
-    any = __syncthreads_or(valid_here);
-    m = block_max(m, sh);
+    m = warp_max(m);
+    const float inv_tau = 1.0f / a.tau;
     float s = 0.0f;
-    for (int k = threadIdx.x; k < a.k; k += blockDim.x)
-        if (top.id[k] >= 0) s += expf(top.p[k] - m);
-    s = block_sum(s, sh);
+    bool valid_here = false;
+    for (int k = lane; k < a.k; k += 32) {
+        if (top.id[k] < 0) continue;
+        valid_here = true;
+        s += expf((top.p[k] - m) * inv_tau);
+    }
+    const bool any = __any_sync(0xffffffffu, valid_here);
+    s = warp_sum(s);
     const float log_s = logf(s);
-    float ent = 0.0f;
-    for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
-        const float lp = top.p[k] - m - log_s;
+    float entropy = 0.0f;
+    for (int k = lane; k < a.k; k += 32) {
+        const float lp = (top.p[k] - m) * inv_tau - log_s;
         const float p = top.id[k] >= 0 ? expf(lp) : 0.0f;
-        if (top.id[k] >= 0 && p != 0.0f) ent += p * lp;
+        if (p != 0.0f) entropy += p * lp;
         top.p[k] = p;
     }
-    return block_sum(ent, sh);  // ends with a barrier: the list is complete
+    entropy = warp_sum(entropy);
+    if (lane == 0) {
+        top.entropy = entropy;
+        top.any = any;
+    }
+    __syncwarp();
 }
 
+// Joins (maximum, sum of exponentials relative to it) over a warp.
+__device__ __forceinline__ void join_warp(float& m, float& s, float c2) {
+    const float top = warp_max(m);
+    // a part without a finite maximum holds 0 or NaN and keeps it
+    s = warp_sum(s * (m == top ? 1.0f : exp2_fast((m - top) * c2)));
+    m = top;
+}
+
+// Loss of the row from its maximum and sum, and the entries' own gradients; one warp for the
+// loss, `threads` threads for the gradients of the ids in [v0, v1).
+__device__ __forceinline__ float row_loss(const DistillArgs& a, const TopList& top, float w, float m, float s) {
+    const float inv_tau = 1.0f / a.tau, log_s = s == 0.0f ? 0.0f : logf(s);
+    float cross = 0.0f;
+    for (int k = threadIdx.x & 31; k < a.k; k += 32)
+        if (top.p[k] != 0.0f) cross += top.p[k] * ((top.z[k] - m) * inv_tau - log_s);
+    return w * a.tau * a.tau * (top.entropy - warp_sum(cross));
+}
 template <typename T>
-__global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a, const T* z, float* __restrict__ loss,
-                                                                  T* grad) {
+__device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopList& top, T* out, int64_t v0, int64_t v1,
+                                              float c, float c2, float m, float inv_s) {
+    for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
+        const int id = top.id[k];
+        if (id < v0 || id >= v1) continue;
+        float p = 0.0f;
+        for (int j = 0; j < a.k; ++j) p += top.id[j] == id ? top.p[j] : 0.0f;
+        out[id] = from_float<T>(c * (exp2_fast((top.z[k] - m) * c2) * inv_s - p));
+    }
+}
+
+// ------------------------------------------------------- rows in registers ---
+//
+// A row is cut into the 16-byte words of its memory (the first and the last may reach over
+// its ends) and lies in the registers of a block, NV words a thread, or of a cluster of
+// blocks: read once, written once.  Each thread takes the maximum of its logits and the sum
+// relative to it, which are joined over warps, block and cluster in one exchange.
+constexpr int kDistillThreads = 512;
+constexpr int kDistillVecs = 8;
+
+template <typename T>
+struct RowWord {
+    static constexpr int kN = 16 / (int)sizeof(T);
+    union {
+        uint4 w;
+        T t[kN];
+    };
+    __device__ __forceinline__ RowWord() {}
+};
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
+    distill_kernel(DistillArgs a, const T* z, float* __restrict__ loss, T* grad, int cluster) {
+    constexpr int N = RowWord<T>::kN;
+    __shared__ TopList top;
+    __shared__ float2 warp_part[32], block_part;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
+    const int64_t t = blockIdx.x / cluster;
+    const int rank = (int)(blockIdx.x % cluster);
+    const T* row = z + t * a.stride;
+    T* out = grad != nullptr ? grad + t * a.vocab : nullptr;
+    const float w = a.weight != nullptr ? a.weight[t] : 1.0f;
+    // words of the row: word i holds the logits i N - skew ...
+    const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    const int64_t words = (a.vocab + skew + N - 1) / N, share = (words + cluster - 1) / cluster;
+    const int64_t first = rank * share, last = min(words, first + share);
+    const int64_t v0 = max((int64_t)0, first * N - skew), v1 = min(a.vocab, last * N - skew);
+    const bool live = w != 0.0f;
+    RowWord<T> x[NV];
+    if (live) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int64_t i = first + v * threads + tid, at = i * N - skew;
+            if (i >= last) break;
+            if (at >= 0 && at + N <= a.vocab) {
+                x[v].w = *reinterpret_cast<const uint4*>(row + at);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    x[v].t[j] = at + j >= 0 && at + j < a.vocab ? row[at + j] : from_float<T>(-INFINITY);
+            }
+        }
+        if (warp == 0) load_teacher<T>(a, t, row, top);
+    }
+    const float c2 = kLog2E / a.tau;
+    float m = -INFINITY, s = 0.0f;
+    if (live) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if (first + v * threads + tid >= last) break;
+#pragma unroll
+            for (int j = 0; j < N; ++j) m = fmaxf(m, to_float(x[v].t[j]));
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if (first + v * threads + tid >= last) break;
+#pragma unroll
+            for (int j = 0; j < N; ++j) s += exp2_fast((to_float(x[v].t[j]) - base) * c2);
+        }
+        join_warp(m, s, c2);
+    }
+    if (lane == 0) warp_part[warp] = make_float2(m, s);
+    __syncthreads();
+    m = lane < warps ? warp_part[lane].x : -INFINITY;
+    s = lane < warps ? warp_part[lane].y : 0.0f;
+    join_warp(m, s, c2);
+    if (cluster > 1) {
+        namespace cg = cooperative_groups;
+        cg::cluster_group group = cg::this_cluster();
+        if (tid == 0) block_part = make_float2(m, s);
+        group.sync();
+        const float2 part = lane < cluster ? *group.map_shared_rank(&block_part, lane) : make_float2(-INFINITY, 0.0f);
+        m = part.x;
+        s = part.y;
+        join_warp(m, s, c2);
+    }
+    const bool any = live && top.any;
+    if (m == -INFINITY) m = 0.0f;
+    if (rank == 0 && warp == 0) {
+        const float l = any ? row_loss(a, top, w, m, s) : 0.0f;
+        if (lane == 0) loss[t] = l;
+    }
+    if (out != nullptr) {
+        const float inv_s = s == 0.0f ? 0.0f : 1.0f / s, c = any ? w * a.tau : 0.0f, ci = c * inv_s;
+        const bool same_skew = (reinterpret_cast<uintptr_t>(out) & 15) / sizeof(T) == skew;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int64_t i = first + v * threads + tid, at = i * N - skew;
+            if (i >= last) break;
+            RowWord<T> y;
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                y.t[j] = from_float<T>(any ? ci * exp2_fast((to_float(x[v].t[j]) - m) * c2) : 0.0f);
+            if (same_skew && at >= 0 && at + N <= a.vocab) {
+                *reinterpret_cast<uint4*>(out + at) = y.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (at + j >= 0 && at + j < a.vocab) out[at + j] = y.t[j];
+            }
+        }
+        if (any) {
+            __syncthreads();
+            top_gradients<T>(a, top, out, v0, v1, c, c2, m, inv_s);
+        }
+    }
+    if (cluster > 1) cooperative_groups::this_cluster().sync();  // a peer may still read this block's part
+}
+
+// ------------------------------------------------------------- longer rows ---
+//
+// A row beyond the registers of a cluster of eight blocks: one block reads it three times.
+template <typename T>
+__global__ void __launch_bounds__(1024) distill_long_kernel(DistillArgs a, const T* z, float* __restrict__ loss,
+                                                            T* grad) {
     __shared__ TopList top;
     __shared__ float sh[32];
     const int64_t t = blockIdx.x;
     const T* row = z + t * a.stride;
     T* out = grad != nullptr ? grad + t * a.vocab : nullptr;
     const float w = a.weight != nullptr ? a.weight[t] : 1.0f;
-    bool any = false;
-    float ent = 0.0f;
-    if (w != 0.0f) ent = load_teacher(a, t, top, sh, any);
-    if (!any) {
+    if (w != 0.0f && threadIdx.x < 32) load_teacher<T>(a, t, row, top);
+    __syncthreads();
+    if (w == 0.0f || !top.any) {
         if (out != nullptr)
-            for (int64_t v = threadIdx.x; v < a.vocab; v += kDistillThreads) out[v] = from_float<T>(0.0f);
+            for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) out[v] = from_float<T>(0.0f);
         if (threadIdx.x == 0) loss[t] = 0.0f;
         return;
     }
-    const float inv_tau = 1.0f / a.tau;
+    const float c2 = kLog2E / a.tau;
     float m = -INFINITY;
-    for (int64_t v = threadIdx.x; v < a.vocab; v += kDistillThreads) m = fmaxf(m, to_float(row[v]) * inv_tau);
+    for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) m = fmaxf(m, to_float(row[v]));
     m = block_max(m, sh);
     if (m == -INFINITY) m = 0.0f;
     float s = 0.0f;
-    for (int64_t v = threadIdx.x; v < a.vocab; v += kDistillThreads) s += expf(to_float(row[v]) * inv_tau - m);
+    for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) s += exp2_fast((to_float(row[v]) - m) * c2);
     s = block_sum(s, sh);
-    const float log_s = s == 0.0f ? 0.0f : logf(s), inv_s = s == 0.0f ? 0.0f : 1.0f / s;
-    float cross = 0.0f;
-    for (int k = threadIdx.x; k < a.k; k += kDistillThreads) {
-        if (top.id[k] < 0) continue;
-        const float zk = to_float(row[top.id[k]]) * inv_tau;
-        top.z[k] = zk;
-        if (top.p[k] != 0.0f) cross += top.p[k] * (zk - m - log_s);
+    if (threadIdx.x < 32) {
+        const float l = row_loss(a, top, w, m, s);
+        if (threadIdx.x == 0) loss[t] = l;
     }
-    cross = block_sum(cross, sh);  // the barrier also ends the reads of z before grad may overwrite them
-    if (threadIdx.x == 0) loss[t] = w * a.tau * a.tau * (ent - cross);
     if (out == nullptr) return;
-    const float c = w * a.tau;
-    for (int64_t v = threadIdx.x; v < a.vocab; v += kDistillThreads)
-        out[v] = from_float<T>(c * (expf(to_float(row[v]) * inv_tau - m) * inv_s));
+    const float inv_s = s == 0.0f ? 0.0f : 1.0f / s, c = w * a.tau;
+    for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x)
+        out[v] = from_float<T>(c * inv_s * exp2_fast((to_float(row[v]) - m) * c2));
     __syncthreads();
-    for (int k = threadIdx.x; k < a.k; k += kDistillThreads) {
-        if (top.id[k] < 0) continue;
-        float p = 0.0f;
-        for (int j = 0; j < a.k; ++j) p += top.id[j] == top.id[k] ? top.p[j] : 0.0f;
-        out[top.id[k]] = from_float<T>(c * (expf(top.z[k] - m) * inv_s - p));
+    top_gradients<T>(a, top, out, 0, a.vocab, c, c2, m, inv_s);
+}
+
+// Threads and words of a thread for a block's share of a row.
+struct DistillPlan {
+    int cluster, threads, vecs;  // cluster 0: the kernel for longer rows
+};
+static DistillPlan distill_plan(int64_t n, int64_t words) {
+    DistillPlan p{1, kDistillThreads, 1};
+    while (p.cluster < 8 && words > (int64_t)p.cluster * kDistillThreads * kDistillVecs) p.cluster *= 2;
+    if (words > (int64_t)p.cluster * kDistillThreads * kDistillVecs) {
+        p.threads = 1024;
+        if (words > (int64_t)p.cluster * p.threads * kDistillVecs) p.cluster = 0;
+        p.vecs = kDistillVecs;
+        return p;
     }
+    // few rows: more blocks a row, as long as each of their threads has a word
+    while (p.cluster < 8 && n * p.cluster < 2 * 148 && words >= 2 * p.cluster * kDistillThreads) p.cluster *= 2;
+    const int64_t share = ceil_div(words, p.cluster);
+    while (p.threads > 64 && share <= p.threads / 2) p.threads /= 2;
+    while (p.vecs * p.threads < share) p.vecs *= 2;
+    return p;
 }
 
 }  // namespace cresso
@@ -143,10 +321,38 @@ int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, 
     const DistillArgs a{ids, teacher, weight, vocab, logits_stride, (int)id_bytes, (int)teacher_dtype, (int)k, tau};
     return with_dtype(dtype, [&](auto tz) {
         using T = decltype(tz);
-        distill_kernel<T><<<(unsigned)n, kDistillThreads, 0, (cudaStream_t)stream>>>(a, static_cast<const T*>(logits),
-                                                                                   loss, static_cast<T*>(grad));
-        CRESSO_LAUNCHED("distill_kernel");
-        return (int)CRESSO_OK;
+        constexpr int N = RowWord<T>::kN;
+        const T* z = static_cast<const T*>(logits);
+        T* g = static_cast<T*>(grad);
+        const cudaStream_t s = (cudaStream_t)stream;
+        const DistillPlan p = distill_plan(n, ceil_div(vocab + N - 1, N));  // the most words a row can meet
+        if (p.cluster == 0) {
+            distill_long_kernel<T><<<(unsigned)n, 1024, 0, s>>>(a, z, loss, g);
+            CRESSO_LAUNCHED("distill_long_kernel");
+            return (int)CRESSO_OK;
+        }
+        CRESSO_REQUIRE(n * p.cluster <= CRESSO_TRAIN_MAX_ROWS, CRESSO_EUNSUPPORTED, "distill: too many rows");
+        auto launch = [&](auto kernel) {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3((unsigned)(n * p.cluster));
+            cfg.blockDim = dim3((unsigned)p.threads);
+            cfg.stream = s;
+            cudaLaunchAttribute attr{};
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = (unsigned)p.cluster;
+            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr;
+            cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+            CRESSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, z, loss, g, p.cluster));
+            CRESSO_LAUNCHED("distill_kernel");
+            return (int)CRESSO_OK;
+        };
+        switch (p.vecs) {
+            case 1: return launch(distill_kernel<T, 1>);
+            case 2: return launch(distill_kernel<T, 2>);
+            case 4: return launch(distill_kernel<T, 4>);
+            default: return launch(distill_kernel<T, kDistillVecs>);
+        }
     });
 }
 
