@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
     const TX *dy = k.dy != nullptr ? static_cast<const TX*>(k.dy) + col0 : nullptr;
     TR* dres = static_cast<TR*>(k.dres) + col0;
     TX* dx = x != nullptr ? static_cast<TX*>(k.dx) + col0 : nullptr;
-    const int64_t pitch = align_up(width, 4);
+    const int64_t pitch = align_up(width, 8);
     const int stage_bytes = slots * 2 * (int)(sizeof(TR) + sizeof(TX));
     auto stage_h = [&](int s) { return reinterpret_cast<TR*>(smem + s * stage_bytes); };
     auto stage_dh = [&](int s) { return stage_h(s) + slots; };
@@ -282,8 +282,8 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
                     sum_b[v][j] += ev[j] * gate * q;
                     sum_pre[v][j] += dyv[j] * n;
                 }
-                store_vec<TR, VEC>(dres + r * width + c, ev);
-                if (x != nullptr) store_vec<TX, VEC>(dx + r * width + c, dxv);
+                store_global<TR, VEC>(dres + r * width + c, ev);
+                if (x != nullptr) store_global<TX, VEC>(dx + r * width + c, dxv);
                 if (OWN_GATE)
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) store_any(k.dgate, a.gate_dtype, r * width + col0 + c + j, dgv[j]);
@@ -296,19 +296,19 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 const int c = (v * T + tid) * VEC;
-                if (c < d) store_vec<float, VEC>(k.part_b + u * pitch + col0 + c, sum_b[v]);
+                if (c < d) store_global<float, VEC>(k.part_b + u * pitch + col0 + c, sum_b[v]);
             }
     }
     if (dy != nullptr)
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = (v * T + tid) * VEC;
-            if (c < d) store_vec<float, VEC>(k.part_pre + worker * pitch + col0 + c, sum_pre[v]);
+            if (c < d) store_global<float, VEC>(k.part_pre + worker * pitch + col0 + c, sum_pre[v]);
         }
     if (k.cluster > 1) cooperative_groups::this_cluster().sync();  // a peer may still read this block's sums
 }
 
-// Sums of `count` consecutive rows of `part` (width columns, rows align_up(width, 4)
+// Sums of `count` consecutive rows of `part` (width columns, rows align_up(width, 8)
 // apart) for each group y: a block takes 32 columns, its 8 warps every eighth row.
 //   sum B of the group:  d_gate[y] = scale post B,  and scale gate[y] B into `out` or,
 //                        with more than one group, into row y of `post_rows`
@@ -324,7 +324,7 @@ struct NormColumns {
 __global__ void __launch_bounds__(kThreads) norm_columns_kernel(NormArgs a, NormColumns k) {
     __shared__ float sh[kWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 32 + lane, d = a.width, pitch = align_up(d, 4);
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane, d = a.width, pitch = align_up(d, 8);
     for (int64_t g = blockIdx.y; g < k.groups; g += gridDim.y) {
         float s = 0.0f;
         if (c < d)
@@ -374,7 +374,7 @@ static NormGradPlan norm_grad_plan(int64_t n, int64_t width, int64_t gate_rows) 
     p.units_per_gate = std::min(rows, std::max<int64_t>(1, want / groups));
     p.units = groups * p.units_per_gate;
     p.workers = std::min(p.units, want);
-    const int64_t pitch = 4 * align_up(width, 4);
+    const int64_t pitch = 4 * align_up(width, 8);
     p.off_b = 0;
     p.off_pre = align_up(p.off_b + p.units * pitch, 256);
     p.off_post = align_up(p.off_pre + p.workers * pitch, 256);
@@ -477,7 +477,7 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
     CRESSO_REQUIRE(scratch != nullptr && scratch_bytes >= p.bytes, CRESSO_ESCRATCH,
                    "block_norm_grad: scratch has %lld bytes, %lld are needed", (long long)scratch_bytes,
                    (long long)p.bytes);
-    CRESSO_REQUIRE(aligned_to(scratch, 16), CRESSO_EINVAL, "block_norm_grad: scratch is not 16-byte aligned");
+    CRESSO_REQUIRE(aligned_to(scratch, 32), CRESSO_EINVAL, "block_norm_grad: scratch is not 32-byte aligned");
     NvtxRange range("block_norm_grad n=%lld", (long long)n);
     const bool own = gate != nullptr && gate_rows == n && n > 1;
     const int64_t groups = gate == nullptr || own ? 1 : gate_rows;
@@ -508,7 +508,7 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
     // the widest accesses that the width and the addresses allow
     auto fits = [&](int vec) {
         if (width % vec != 0) return false;
-        const int64_t ar = std::min<int64_t>(16, vec * rb), ax = std::min<int64_t>(16, vec * xb);
+        const int64_t ar = std::min<int64_t>(32, vec * rb), ax = std::min<int64_t>(32, vec * xb);
         return aligned_to(h, ar) && aligned_to(d_h, ar) && aligned_to(d_residual, ar) && aligned_to(x, ax) &&
                aligned_to(d_y, ax) && aligned_to(d_x, ax);
     };

@@ -14,6 +14,8 @@
 
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 namespace cresso {
 
 struct DistillArgs {
@@ -33,7 +35,7 @@ struct TopList {
     int any;                        // a valid entry exists
 };
 
-constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x) {  // relative error 2^-22
     float y;
@@ -121,19 +123,39 @@ constexpr int kDistillThreads = 512;
 constexpr int kDistillVecs = 8;
 
 template <typename T>
-struct RowWord {
-    static constexpr int kN = 16 / (int)sizeof(T);
-    union {
-        uint4 w;
-        T t[kN];
-    };
-    __device__ __forceinline__ RowWord() {}
-};
+constexpr int kWordLogits = 16 / (int)sizeof(T);
+
+// Maximum of the logits of a word; NaN is left out.
+template <typename T>
+__device__ __forceinline__ float word_max(const uint32_t (&w)[4]) {
+    if constexpr (sizeof(T) == 4) {
+        return fmaxf(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])),
+                     fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3])));
+    } else {
+        using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+        auto as2 = [&](int i) { return *reinterpret_cast<const T2*>(&w[i]); };
+        const T2 v = __hmax2(__hmax2(as2(0), as2(1)), __hmax2(as2(2), as2(3)));
+        const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t*>(&v));
+        return fmaxf(f.x, f.y);
+    }
+}
+
+// f(i, pair): the logits of a word two at a time.
+template <typename T, typename F>
+__device__ __forceinline__ void word_pairs(const uint32_t (&w)[4], F f) {
+    if constexpr (sizeof(T) == 4) {
+        f(0, make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])));
+        f(1, make_float2(__uint_as_float(w[2]), __uint_as_float(w[3])));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f(i, unpack2<T>(w[i]));
+    }
+}
 
 template <typename T, int NV>
 __global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
     distill_kernel(DistillArgs a, const T* z, float* __restrict__ loss, T* grad, int cluster) {
-    constexpr int N = RowWord<T>::kN;
+    constexpr int N = kWordLogits<T>;
     __shared__ TopList top;
     __shared__ float2 warp_part[32], block_part;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
@@ -148,19 +170,29 @@ __global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
     const int64_t first = rank * share, last = min(words, first + share);
     const int64_t v0 = max((int64_t)0, first * N - skew), v1 = min(a.vocab, last * N - skew);
     const bool live = w != 0.0f;
-    RowWord<T> x[NV];
+    uint32_t x[NV][4];
     if (live) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int64_t i = first + v * threads + tid, at = i * N - skew;
-            if (i >= last) break;
-            if (at >= 0 && at + N <= a.vocab) {
-                x[v].w = *reinterpret_cast<const uint4*>(row + at);
-            } else {
+            const bool whole = i < last && at >= 0 && at + N <= a.vocab;
+            const uint4 q = whole ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
+            x[v][0] = q.x;
+            x[v][1] = q.y;
+            x[v][2] = q.z;
+            x[v][3] = q.w;
+        }
+        // places outside the row hold -inf; a word that reaches over an end is read by element
 #pragma unroll
-                for (int j = 0; j < N; ++j)
-                    x[v].t[j] = at + j >= 0 && at + j < a.vocab ? row[at + j] : from_float<T>(-INFINITY);
-            }
+        for (int v = 0; v < NV; ++v) {
+            const int64_t i = first + v * threads + tid, at = i * N - skew;
+            if (i < last && at >= 0 && at + N <= a.vocab) continue;
+            T edge[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                edge[j] = i < last && at + j >= 0 && at + j < a.vocab ? row[at + j] : from_float<T>(-INFINITY);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[v][j] = reinterpret_cast<const uint32_t*>(edge)[j];
         }
         if (warp == 0) load_teacher<T>(a, t, row, top);
     }
@@ -168,18 +200,16 @@ __global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
     float m = -INFINITY, s = 0.0f;
     if (live) {
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            if (first + v * threads + tid >= last) break;
+        for (int v = 0; v < NV; ++v) m = fmaxf(m, word_max<T>(x[v]));
+        const float base = m == -INFINITY ? 0.0f : -m;
+        float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int j = 0; j < N; ++j) m = fmaxf(m, to_float(x[v].t[j]));
-        }
-        const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            if (first + v * threads + tid >= last) break;
-#pragma unroll
-            for (int j = 0; j < N; ++j) s += exp2_fast((to_float(x[v].t[j]) - base) * c2);
-        }
+        for (int v = 0; v < NV; ++v)
+            word_pairs<T>(x[v], [&](int, float2 f) {
+                f = mul2(add2(f, make_float2(base, base)), make_float2(c2, c2));
+                sum = add2(sum, make_float2(exp2_fast(f.x), exp2_fast(f.y)));
+            });
+        s = sum.x + sum.y;
         join_warp(m, s, c2);
     }
     if (lane == 0) warp_part[warp] = make_float2(m, s);
@@ -210,16 +240,27 @@ __global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
         for (int v = 0; v < NV; ++v) {
             const int64_t i = first + v * threads + tid, at = i * N - skew;
             if (i >= last) break;
-            RowWord<T> y;
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                y.t[j] = from_float<T>(any ? ci * exp2_fast((to_float(x[v].t[j]) - m) * c2) : 0.0f);
+            uint32_t y[4] = {0, 0, 0, 0};
+            if (any)
+                word_pairs<T>(x[v], [&](int j, float2 f) {
+                    f = mul2(add2(f, make_float2(-m, -m)), make_float2(c2, c2));
+                    f = mul2(make_float2(exp2_fast(f.x), exp2_fast(f.y)), make_float2(ci, ci));
+                    if constexpr (sizeof(T) == 4) {
+                        y[2 * j] = __float_as_uint(f.x);
+                        y[2 * j + 1] = __float_as_uint(f.y);
+                    } else {
+                        y[j] = pack2<T>(f.x, f.y);
+                    }
+                });
             if (same_skew && at >= 0 && at + N <= a.vocab) {
-                *reinterpret_cast<uint4*>(out + at) = y.w;
+                *reinterpret_cast<uint4*>(out + at) = make_uint4(y[0], y[1], y[2], y[3]);
             } else {
+                T edge[N];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(edge)[j] = y[j];
 #pragma unroll
                 for (int j = 0; j < N; ++j)
-                    if (at + j >= 0 && at + j < a.vocab) out[at + j] = y.t[j];
+                    if (at + j >= 0 && at + j < a.vocab) out[at + j] = edge[j];
             }
         }
         if (any) {
@@ -321,7 +362,7 @@ int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, 
     const DistillArgs a{ids, teacher, weight, vocab, logits_stride, (int)id_bytes, (int)teacher_dtype, (int)k, tau};
     return with_dtype(dtype, [&](auto tz) {
         using T = decltype(tz);
-        constexpr int N = RowWord<T>::kN;
+        constexpr int N = kWordLogits<T>;
         const T* z = static_cast<const T*>(logits);
         T* g = static_cast<T*>(grad);
         const cudaStream_t s = (cudaStream_t)stream;

@@ -446,7 +446,7 @@ int cresso_embedding_gather(const void* weight, int64_t weight_dtype, int64_t ro
     });
 }
 
-// scratch: range [rows], order [n], total, partial rows [2 tiles][align_up(width, 4)]
+// scratch: range [rows], order [n], total, partial rows [2 tiles][align_up(width, 8)]
 struct GradScratch {
     int64_t tile, tiles, order, total, partial, bytes;
 };
@@ -457,7 +457,7 @@ static GradScratch grad_scratch(int64_t n, int64_t rows, int64_t width) {
     p.order = align_up(8 * rows, 256);
     p.total = p.order + align_up(8 * n, 256);
     p.partial = p.total + 256;
-    p.bytes = p.partial + (p.tiles > 1 ? 2 * p.tiles * align_up(width, 4) * 4 : 0);
+    p.bytes = p.partial + (p.tiles > 1 ? 2 * p.tiles * align_up(width, 8) * 4 : 0);
     return p;
 }
 
@@ -493,7 +493,7 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
     CRESSO_REQUIRE(grad != nullptr && tokens != nullptr, CRESSO_EINVAL, "embedding_grad: NULL pointer");
     CRESSO_REQUIRE(scratch != nullptr && scratch_bytes >= need, CRESSO_ESCRATCH,
                    "embedding_grad: scratch has %lld bytes, %lld are needed", (long long)scratch_bytes, (long long)need);
-    CRESSO_REQUIRE(aligned_to(scratch, 16), CRESSO_EINVAL, "embedding_grad: scratch is not 16-byte aligned");
+    CRESSO_REQUIRE(aligned_to(scratch, 32), CRESSO_EINVAL, "embedding_grad: scratch is not 32-byte aligned");
     NvtxRange range("embedding_grad n=%lld rows=%lld", (long long)n, (long long)rows);
     const GradScratch at = grad_scratch(n, rows, width);
     unsigned char* base = static_cast<unsigned char*>(scratch);
@@ -518,7 +518,7 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
     const int rs = token_bytes == 8 ? sort(sort_kernel<int64_t>) : sort(sort_kernel<int32_t>);
     if (rs != CRESSO_OK) return rs;
     GradSums k{ranges, order, total, reinterpret_cast<float*>(base + at.partial), rows, width, grad_stride, at.tiles,
-               align_up(width, 4), (float)scale, accumulate != 0, 0, (int)at.tile};
+               align_up(width, 8), (float)scale, accumulate != 0, 0, (int)at.tile};
     const int64_t items = k.tiles + (accumulate ? 0 : ceil_div(rows, kEmptyRows));
     return with_dtype(grad_dtype, [&](auto tg) {
         return with_dtype(out_dtype, [&](auto to) {

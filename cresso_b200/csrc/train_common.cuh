@@ -80,103 +80,160 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
     return s;
 }
 
-// VEC elements of T between memory and float registers, as the widest accesses that
-// VEC * sizeof(T) bytes allow; p is aligned to min(16, VEC * sizeof(T)).
-template <int BYTES>
-struct Word;
+// Two packed 16-bit elements and their float values: one instruction an element to read,
+// one for both to write.
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
 template <>
-struct Word<2> { using type = unsigned short; };
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
 template <>
-struct Word<4> { using type = unsigned int; };
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
-struct Word<8> { using type = uint2; };
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 template <>
-struct Word<16> { using type = uint4; };
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 
-// VEC elements as they lie in memory.
+// Float pairs on the two-lane float32 instructions of sm_100.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+          "l"(reinterpret_cast<const uint64_t&>(c)));
+    return r;
+}
+
+// VEC elements as they lie in memory: 32-bit registers (one 16-bit element in a register of
+// its own).  Global 32-byte accesses exist on sm_100; a warp's access then covers whole
+// sectors.  Pointers are aligned to min(32, VEC * sizeof(T)), in shared memory to 16.
 template <typename T, int VEC>
 struct Raw {
-    static constexpr int kBytes = VEC * (int)sizeof(T) < 16 ? VEC * (int)sizeof(T) : 16;
-    static constexpr int kWords = VEC * (int)sizeof(T) / kBytes;
-    using W = typename Word<kBytes>::type;
-    union {
-        W w[kWords];
-        T t[VEC];
-    };
-    __device__ __forceinline__ Raw() {}
-    __device__ __forceinline__ void load(const T* p) {
+    static constexpr int kBytes = VEC * (int)sizeof(T);
+    static constexpr int kWords = kBytes < 4 ? 1 : kBytes / 4;
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void load(const T* p) {  // any memory
+        if constexpr (kBytes == 2)
+            w[0] = *reinterpret_cast<const unsigned short*>(p);
+        else if constexpr (kBytes == 4)
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        else if constexpr (kBytes == 8)
+            set(0, *reinterpret_cast<const uint2*>(p));
+        else
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const W*>(p)[i];
+            for (int i = 0; i < kBytes / 16; ++i) set(4 * i, reinterpret_cast<const uint4*>(p)[i]);
     }
-    __device__ __forceinline__ void load_once(const T* p) {  // read-only data
+    __device__ __forceinline__ void load_global(const T* p) {  // data that the kernel does not write
+        if constexpr (kBytes == 32)
+            asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                : "l"(p));
+        else if constexpr (kBytes == 2)
+            w[0] = __ldg(reinterpret_cast<const unsigned short*>(p));
+        else if constexpr (kBytes == 4)
+            w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        else if constexpr (kBytes == 8)
+            set(0, __ldg(reinterpret_cast<const uint2*>(p)));
+        else
+            set(0, __ldg(reinterpret_cast<const uint4*>(p)));
+    }
+    __device__ __forceinline__ void store(T* p) const {  // global memory
+        if constexpr (kBytes == 32)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]),
+                         "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+        else if constexpr (kBytes == 2)
+            *reinterpret_cast<unsigned short*>(p) = (unsigned short)w[0];
+        else if constexpr (kBytes == 4)
+            *reinterpret_cast<uint32_t*>(p) = w[0];
+        else if constexpr (kBytes == 8)
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        else
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ __forceinline__ void to(float (&f)[VEC]) const {
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const W*>(p) + i);
+            for (int i = 0; i < VEC; ++i) f[i] = __uint_as_float(w[i]);
+        } else if constexpr (VEC == 1) {
+            f[0] = unpack2<T>(w[0]).x;
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+                const float2 v = unpack2<T>(w[i]);
+                f[2 * i] = v.x;
+                f[2 * i + 1] = v.y;
+            }
+        }
     }
-    __device__ __forceinline__ float get(int i) const { return to_float(t[i]); }
+    __device__ __forceinline__ void from(const float (&f)[VEC]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) w[i] = __float_as_uint(f[i]);
+        } else if constexpr (VEC == 1) {
+            w[0] = pack2<T>(f[0], 0.0f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+        }
+    }
+
+private:
+    __device__ __forceinline__ void set(int i, uint2 v) {
+        w[i] = v.x;
+        w[i + 1] = v.y;
+    }
+    __device__ __forceinline__ void set(int i, uint4 v) {
+        w[i] = v.x;
+        w[i + 1] = v.y;
+        w[i + 2] = v.z;
+        w[i + 3] = v.w;
+    }
 };
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T* p, float (&f)[VEC]) {
     Raw<T, VEC> u;
     u.load(p);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = u.get(i);
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void store_vec(T* p, const float (&f)[VEC]) {
-    constexpr int B = VEC * (int)sizeof(T) < 16 ? VEC * (int)sizeof(T) : 16, N = VEC * (int)sizeof(T) / B;
-    using W = typename Word<B>::type;
-    union {
-        W w[N];
-        T t[VEC];
-    } u;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) u.t[i] = from_float<T>(f[i]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) reinterpret_cast<W*>(p)[i] = u.w[i];
-}
-
-// The same for global memory, with 32-byte accesses (sm_100) where VEC elements have 32
-// bytes: a warp's access then covers whole sectors.  p is aligned to min(32, VEC *
-// sizeof(T)).  load_global reads data that the kernel does not write.
-struct alignas(32) Word32 {
-    uint32_t w[8];
-};
-__device__ __forceinline__ Word32 load_word32(const void* p) {
-    Word32 v;
-    asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-        : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
-        : "l"(p));
-    return v;
-}
-__device__ __forceinline__ void store_word32(void* p, const Word32& v) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v.w[0]), "r"(v.w[1]),
-                 "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]), "r"(v.w[7])
-                 : "memory");
+    u.to(f);
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void load_global(const T* p, float (&f)[VEC]) {
-    if constexpr (VEC * sizeof(T) == 32) {
-        const Word32 v = load_word32(p);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) f[i] = __uint_as_float(v.w[i]);
-    } else {
-        Raw<T, VEC> u;
-        u.load_once(p);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) f[i] = u.get(i);
-    }
+    Raw<T, VEC> u;
+    u.load_global(p);
+    u.to(f);
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void store_global(T* p, const float (&f)[VEC]) {
-    if constexpr (VEC * sizeof(T) == 32) {
-        Word32 v;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v.w[i] = __float_as_uint(f[i]);
-        store_word32(p, v);
-    } else {
-        store_vec<T, VEC>(p, f);
-    }
+    Raw<T, VEC> u;
+    u.from(f);
+    u.store(p);
 }
 
 // Asynchronous copy of VEC elements from global to shared memory in 16-, 8- or 4-byte

@@ -7,7 +7,7 @@
  * counterpart in the reference, whose package holds the optimizer only.
  *
  * The conventions are those of cresso_b200.h: raw device pointers, an int status
- * (the message is read with cresso_last_error), caller-owned scratch (16-byte
+ * (the message is read with cresso_last_error), caller-owned scratch (32-byte
  * aligned) whose size is queried first, work ordered on the given stream of the current device,
  * no allocation and no synchronisation.  Element types are CRESSO_DTYPE_F32,
  * _F16 and _BF16; sums, statistics and norms are float32 and every output is
