@@ -115,9 +115,8 @@ __device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopLis
 
 // ------------------------------------------------------- rows in registers ---
 //
-// A row is cut into the 16-byte words of its memory (the first and the last may reach over
-// its ends) and lies in the registers of a block, NV words a thread, or of a cluster of
-// blocks: read once, written once.  Each thread takes the maximum of its logits and the sum
+// A row is cut into the 16-byte words of its memory and lies in the registers of a block, NV
+// words a thread, or of a cluster of blocks: read once, written once.  Each thread takes the maximum of its logits and the sum
 // relative to it, which are joined over warps, block and cluster in one exchange.
 constexpr int kDistillThreads = 512;
 constexpr int kDistillVecs = 8;
@@ -164,36 +163,32 @@ __global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
     const T* row = z + t * a.stride;
     T* out = grad != nullptr ? grad + t * a.vocab : nullptr;
     const float w = a.weight != nullptr ? a.weight[t] : 1.0f;
-    // words of the row: word i holds the logits i N - skew ...
-    const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-    const int64_t words = (a.vocab + skew + N - 1) / N, share = (words + cluster - 1) / cluster;
-    const int64_t first = rank * share, last = min(words, first + share);
-    const int64_t v0 = max((int64_t)0, first * N - skew), v1 = min(a.vocab, last * N - skew);
+    // the whole words of the row, this block's share of them; up to N - 1 logits before them and
+    // behind them are left to single threads of the first and the last block
+    const int vocab = (int)a.vocab;
+    const int head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / sizeof(T)));
+    const int words = (vocab - head) / N, share = (words + cluster - 1) / cluster;
+    const int first = min(words, rank * share), count = min(words - first, share);
+    const int tail = head + words * N;
+    int edge = -1;
+    if (rank == 0 && tid < head) edge = tid;
+    if (rank == cluster - 1 && tid >= N && tid - N < vocab - tail) edge = tail + tid - N;
+    const T* body = row + head + first * N;
     const bool live = w != 0.0f;
     uint32_t x[NV][4];
+    float edge_x = -INFINITY;
     if (live) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int64_t i = first + v * threads + tid, at = i * N - skew;
-            const bool whole = i < last && at >= 0 && at + N <= a.vocab;
-            const uint4 q = whole ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
+            constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
+            const int i = v * threads + tid;
+            const uint4 q = i < count ? reinterpret_cast<const uint4*>(body)[i] : make_uint4(kNone, kNone, kNone, kNone);
             x[v][0] = q.x;
             x[v][1] = q.y;
             x[v][2] = q.z;
             x[v][3] = q.w;
         }
-        // places outside the row hold -inf; a word that reaches over an end is read by element
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int64_t i = first + v * threads + tid, at = i * N - skew;
-            if (i < last && at >= 0 && at + N <= a.vocab) continue;
-            T edge[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                edge[j] = i < last && at + j >= 0 && at + j < a.vocab ? row[at + j] : from_float<T>(-INFINITY);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[v][j] = reinterpret_cast<const uint32_t*>(edge)[j];
-        }
+        if (edge >= 0) edge_x = to_float(row[edge]);
         if (warp == 0) load_teacher<T>(a, t, row, top);
     }
     const float c2 = kLog2E / a.tau;
@@ -201,6 +196,7 @@ __global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
     if (live) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) m = fmaxf(m, word_max<T>(x[v]));
+        m = fmaxf(m, edge_x);
         const float base = m == -INFINITY ? 0.0f : -m;
         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -209,7 +205,7 @@ __global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
                 f = mul2(add2(f, make_float2(base, base)), make_float2(c2, c2));
                 sum = add2(sum, make_float2(exp2_fast(f.x), exp2_fast(f.y)));
             });
-        s = sum.x + sum.y;
+        s = sum.x + sum.y + exp2_fast((edge_x + base) * c2);
         join_warp(m, s, c2);
     }
     if (lane == 0) warp_part[warp] = make_float2(m, s);
@@ -235,11 +231,12 @@ __global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
     }
     if (out != nullptr) {
         const float inv_s = s == 0.0f ? 0.0f : 1.0f / s, c = any ? w * a.tau : 0.0f, ci = c * inv_s;
-        const bool same_skew = (reinterpret_cast<uintptr_t>(out) & 15) / sizeof(T) == skew;
+        T* out_body = out + head + first * N;
+        const bool aligned = (reinterpret_cast<uintptr_t>(out_body) & 15) == 0;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int64_t i = first + v * threads + tid, at = i * N - skew;
-            if (i >= last) break;
+            const int i = v * threads + tid;
+            if (i >= count) break;
             uint32_t y[4] = {0, 0, 0, 0};
             if (any)
                 word_pairs<T>(x[v], [&](int j, float2 f) {
@@ -252,19 +249,21 @@ __global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
                         y[j] = pack2<T>(f.x, f.y);
                     }
                 });
-            if (same_skew && at >= 0 && at + N <= a.vocab) {
-                *reinterpret_cast<uint4*>(out + at) = make_uint4(y[0], y[1], y[2], y[3]);
-            } else {
-                T edge[N];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(edge)[j] = y[j];
+            if (aligned) {
+                reinterpret_cast<uint4*>(out_body)[i] = make_uint4(y[0], y[1], y[2], y[3]);
+            } else {  // rows of logits that lie further apart than those of the gradient
 #pragma unroll
                 for (int j = 0; j < N; ++j)
-                    if (at + j >= 0 && at + j < a.vocab) out[at + j] = edge[j];
+                    if constexpr (sizeof(T) == 4)
+                        reinterpret_cast<uint32_t*>(out_body)[i * N + j] = y[j];
+                    else
+                        reinterpret_cast<uint16_t*>(out_body)[i * N + j] = (uint16_t)(y[j / 2] >> (16 * (j & 1)));
             }
         }
+        if (edge >= 0) out[edge] = from_float<T>(any ? ci * exp2_fast((edge_x - m) * c2) : 0.0f);
         if (any) {
             __syncthreads();
+            const int v0 = rank == 0 ? 0 : head + first * N, v1 = rank == cluster - 1 ? vocab : head + (first + count) * N;
             top_gradients<T>(a, top, out, v0, v1, c, c2, m, inv_s);
         }
     }
@@ -328,7 +327,7 @@ static DistillPlan distill_plan(int64_t n, int64_t words) {
     while (p.cluster < 8 && n * p.cluster < 2 * 148 && words >= 2 * p.cluster * kDistillThreads) p.cluster *= 2;
     const int64_t share = ceil_div(words, p.cluster);
     while (p.threads > 64 && share <= p.threads / 2) p.threads /= 2;
-    while (p.vecs * p.threads < share) p.vecs *= 2;
+    while ((int64_t)p.vecs * p.threads < share) p.vecs *= 2;
     return p;
 }
 
@@ -366,7 +365,7 @@ int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, 
         const T* z = static_cast<const T*>(logits);
         T* g = static_cast<T*>(grad);
         const cudaStream_t s = (cudaStream_t)stream;
-        const DistillPlan p = distill_plan(n, ceil_div(vocab + N - 1, N));  // the most words a row can meet
+        const DistillPlan p = distill_plan(n, vocab / N);
         if (p.cluster == 0) {
             distill_long_kernel<T><<<(unsigned)n, 1024, 0, s>>>(a, z, loss, g);
             CRESSO_LAUNCHED("distill_long_kernel");
