@@ -6,14 +6,16 @@
 //   p = softmax(u / tau) over the valid entries,  q = softmax(z / tau) over V,
 //   loss = w tau^2 sum_k p_k (log p_k - log q[id_k]),
 //   dz_v = w tau (q_v - P_v),  P_v = sum of p_k with id_k = v.
-// Exponentials are 2^((z - max) log2(e) / tau): the difference first, so that their error
-// stays that of the difference however large the logits are; sums are float32.  A NaN or
-// +inf logit makes its row NaN through the sum; a row of -inf alone has q = 0.  Repeated
+// Exponentials are 2^(z c - B) with c = log2(e) / tau and B = max(z) c rounded: one fused
+// operation, whose error is that of its result, because the same B stands in the sum, in
+// the gradient and in the loss.  Sums are float32.  A NaN or +inf logit makes its row NaN
+// through the sum; a row of -inf alone has q = 0.  Repeated
 // ids: every entry forms the whole P of its id, so that all of them write the same value.
 #include "train_common.cuh"
 
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace cresso {
@@ -26,16 +28,19 @@ struct DistillArgs {
     float tau;
 };
 
-// The teacher's side of a row in shared memory.
+// The teacher's side of a row in shared memory: k ids (-1: not valid), teacher probabilities
+// and student logits at the ids, then the sum of p log p and whether a valid entry exists.
 struct TopList {
-    int id[CRESSO_TRAIN_MAX_TOP];   // -1: not valid
-    float p[CRESSO_TRAIN_MAX_TOP];  // teacher probability
-    float z[CRESSO_TRAIN_MAX_TOP];  // student logit at the id
-    float entropy;                  // sum of p log p
-    int any;                        // a valid entry exists
+    int* id;
+    float *p, *z, *entropy;
+    int* any;
+    __device__ __forceinline__ TopList(unsigned char* at, int k)
+        : id(reinterpret_cast<int*>(at)), p(reinterpret_cast<float*>(at) + k), z(p + k), entropy(z + k),
+          any(reinterpret_cast<int*>(entropy + 1)) {}
 };
+__host__ __device__ constexpr int top_bytes(int k) { return (12 * k + 8 + 15) / 16 * 16; }
 
-constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float exp2_fast(float x) {  // relative error 2^-22
     float y;
@@ -45,18 +50,20 @@ __device__ __forceinline__ float exp2_fast(float x) {  // relative error 2^-22
 
 // Fills the list with one warp; the block sees it after its next barrier.
 template <typename T>
-__device__ __forceinline__ void load_teacher(const DistillArgs& a, int64_t t, const T* row, TopList& top) {
+__device__ __forceinline__ void load_teacher(const DistillArgs& a, int64_t t, const T* row, const TopList& top) {
     const int lane = threadIdx.x & 31;
     float m = -INFINITY;
+#pragma unroll 4
     for (int k = lane; k < a.k; k += 32) {
         const int64_t id = load_id(a.ids, a.id_bytes, t * a.k + k);
         const float u = load_any(a.teacher, a.teacher_dtype, t * a.k + k);
         const bool valid = id >= 0 && id < a.vocab && u != -INFINITY;
         top.id[k] = valid ? (int)id : -1;
         top.p[k] = u;
-        top.z[k] = valid ? to_float(row[id]) : 0.0f;
         if (valid) m = fmaxf(m, u);
     }
+#pragma unroll 4
+    for (int k = lane; k < a.k; k += 32) top.z[k] = top.id[k] >= 0 ? to_float(row[top.id[k]]) : 0.0f;
     m = warp_max(m);
     const float inv_tau = 1.0f / a.tau;
     float s = 0.0f;
@@ -78,194 +85,316 @@ __device__ __forceinline__ void load_teacher(const DistillArgs& a, int64_t t, co
     }
     entropy = warp_sum(entropy);
     if (lane == 0) {
-        top.entropy = entropy;
-        top.any = any;
+        *top.entropy = entropy;
+        *top.any = any;
     }
     __syncwarp();
 }
 
-// Joins (maximum, sum of exponentials relative to it) over a warp.
+// Joins (maximum, sum of 2^(z c - B)) over the lanes of a warp, or of its first WIDTH lanes.
+template <int WIDTH = 32>
 __device__ __forceinline__ void join_warp(float& m, float& s, float c2) {
-    const float top = warp_max(m);
+    float top = m;
+#pragma unroll
+    for (int o = WIDTH / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     // a part without a finite maximum holds 0 or NaN and keeps it
-    s = warp_sum(s * (m == top ? 1.0f : exp2_fast((m - top) * c2)));
+    s *= m == top ? 1.0f : exp2_fast(__fmul_rn(m, c2) - __fmul_rn(top, c2));  // the rounded B of both
+#pragma unroll
+    for (int o = WIDTH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     m = top;
 }
 
-// Loss of the row from its maximum and sum, and the entries' own gradients; one warp for the
-// loss, `threads` threads for the gradients of the ids in [v0, v1).
-__device__ __forceinline__ float row_loss(const DistillArgs& a, const TopList& top, float w, float m, float s) {
-    const float inv_tau = 1.0f / a.tau, log_s = s == 0.0f ? 0.0f : logf(s);
+// -B of a maximum; 0 where there is none.  B's rounding shifts all exponents of a row by up to
+// 2^-24 |B|, which cancels as long as it is small: a row whose |B| is above kFar is formed
+// again from z - max, and a part of another row whose |B| is above twice that adds nothing.
+constexpr float kFar = 16777216.0f;
+__device__ __forceinline__ float minus_b(float m, float c2) {
+    const float b = __fmul_rn(m, c2);
+    return fabsf(b) > 2.0f * kFar ? 0.0f : -b;
+}
+
+// Loss of the row from its base = -B and sum by one warp, and the gradients of the entries' ids in
+// [v0, v1) by `threads` threads.
+__device__ __forceinline__ float row_loss(const DistillArgs& a, const TopList& top, float w, float c2, float base, float s) {
+    const float log_s = s == 0.0f ? 0.0f : logf(s);
     float cross = 0.0f;
     for (int k = threadIdx.x & 31; k < a.k; k += 32)
-        if (top.p[k] != 0.0f) cross += top.p[k] * ((top.z[k] - m) * inv_tau - log_s);
-    return w * a.tau * a.tau * (top.entropy - warp_sum(cross));
+        if (top.p[k] != 0.0f) cross += top.p[k] * (fmaf(top.z[k], c2, base) * kLn2 - log_s);
+    return w * a.tau * a.tau * (*top.entropy - warp_sum(cross));
 }
 template <typename T>
-__device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopList& top, T* out, int64_t v0, int64_t v1,
-                                              float c, float c2, float m, float inv_s) {
-    for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
+__device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopList& top, T* out, int threads, int v0, int v1,
+                                              float c, float c2, float base, float inv_s) {
+    for (int k = threadIdx.x; k < a.k; k += threads) {
         const int id = top.id[k];
         if (id < v0 || id >= v1) continue;
         float p = 0.0f;
         for (int j = 0; j < a.k; ++j) p += top.id[j] == id ? top.p[j] : 0.0f;
-        out[id] = from_float<T>(c * (exp2_fast((top.z[k] - m) * c2) * inv_s - p));
+        out[id] = from_float<T>(c * (exp2_fast(fmaf(top.z[k], c2, base)) * inv_s - p));
     }
 }
 
-// ------------------------------------------------------- rows in registers ---
+// ----------------------------------------------------- rows in shared memory ---
 //
-// A row is cut into the 16-byte words of its memory and lies in the registers of a block, NV
-// words a thread, or of a cluster of blocks: read once, written once.  Each thread takes the maximum of its logits and the sum
-// relative to it, which are joined over warps, block and cluster in one exchange.
-constexpr int kDistillThreads = 512;
-constexpr int kDistillVecs = 8;
+// A row is cut into the 16-byte words of its memory and lies in the shared memory of a block,
+// or of a cluster of blocks: read once, written once.  Each thread copies and reads the same
+// words.  The blocks stay for many rows: a word of the next row takes the place of a word
+// whose gradient is formed, and one further warp prepares the next teacher list, whose chain
+// of dependent loads is as long as a row takes.  Each thread takes the maximum of its logits
+// and the sum relative to it, which are joined over warps, block and cluster in one exchange.
+constexpr int kDistillThreads = 256;          // the teacher's warp among them
+constexpr int kDistillShare = 64 * 1024;      // bytes of a row in a block, three blocks an SM
+constexpr int kDistillLongShare = 128 * 1024; // the same for the longest rows, one block an SM
 
 template <typename T>
 constexpr int kWordLogits = 16 / (int)sizeof(T);
 
-// Maximum of the logits of a word; NaN is left out.
+// Running maximum of the logits of a thread's words; NaN is left out.
 template <typename T>
-__device__ __forceinline__ float word_max(const uint32_t (&w)[4]) {
-    if constexpr (sizeof(T) == 4) {
-        return fmaxf(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])),
-                     fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3])));
-    } else {
-        using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
-        auto as2 = [&](int i) { return *reinterpret_cast<const T2*>(&w[i]); };
-        const T2 v = __hmax2(__hmax2(as2(0), as2(1)), __hmax2(as2(2), as2(3)));
-        const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t*>(&v));
+struct WordMax {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    T2 m;
+    __device__ __forceinline__ WordMax() {
+        const uint32_t none = std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+        m = *reinterpret_cast<const T2*>(&none);
+    }
+    __device__ __forceinline__ void add(const uint4& w) {
+        auto two = [](const uint32_t& v) { return *reinterpret_cast<const T2*>(&v); };
+        m = __hmax2(__hmax2(m, __hmax2(two(w.x), two(w.y))), __hmax2(two(w.z), two(w.w)));
+    }
+    __device__ __forceinline__ float get() const {
+        const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t*>(&m));
         return fmaxf(f.x, f.y);
     }
-}
+};
+template <>
+struct WordMax<float> {
+    float m = -INFINITY;
+    __device__ __forceinline__ void add(const uint4& w) {
+        m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(w.x), __uint_as_float(w.y))),
+                  fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+    }
+    __device__ __forceinline__ float get() const { return m; }
+};
 
 // f(i, pair): the logits of a word two at a time.
 template <typename T, typename F>
-__device__ __forceinline__ void word_pairs(const uint32_t (&w)[4], F f) {
+__device__ __forceinline__ void word_pairs(const uint4& w, F f) {
     if constexpr (sizeof(T) == 4) {
-        f(0, make_float2(__uint_as_float(w[0]), __uint_as_float(w[1])));
-        f(1, make_float2(__uint_as_float(w[2]), __uint_as_float(w[3])));
+        f(0, make_float2(__uint_as_float(w.x), __uint_as_float(w.y)));
+        f(1, make_float2(__uint_as_float(w.z), __uint_as_float(w.w)));
     } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f(i, unpack2<T>(w[i]));
+        f(0, unpack2<T>(w.x));
+        f(1, unpack2<T>(w.y));
+        f(2, unpack2<T>(w.z));
+        f(3, unpack2<T>(w.w));
     }
 }
 
-template <typename T, int NV>
-__global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
-    distill_kernel(DistillArgs a, const T* z, float* __restrict__ loss, T* grad, int cluster) {
+// A row's whole words and a block's share of them; up to N - 1 logits before the words and
+// behind them are left to single threads of the first and the last block.
+struct RowShare {
+    int first, count;  // words
+    int head, edge;    // logits before the words; the thread's single logit or -1
+};
+template <typename T>
+__device__ __forceinline__ RowShare row_share(const T* row, int vocab, int rank, int log_cluster, int tid) {
     constexpr int N = kWordLogits<T>;
-    __shared__ TopList top;
-    __shared__ float2 warp_part[32], block_part;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
-    const int64_t t = blockIdx.x / cluster;
-    const int rank = (int)(blockIdx.x % cluster);
-    const T* row = z + t * a.stride;
-    T* out = grad != nullptr ? grad + t * a.vocab : nullptr;
-    const float w = a.weight != nullptr ? a.weight[t] : 1.0f;
-    // the whole words of the row, this block's share of them; up to N - 1 logits before them and
-    // behind them are left to single threads of the first and the last block
+    const int cluster = 1 << log_cluster;
+    RowShare r;
+    r.head = min(vocab, (int)(((16u - ((uint32_t)reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / sizeof(T)));
+    const int words = (vocab - r.head) / N, share = (words + cluster - 1) >> log_cluster, tail = r.head + words * N;
+    r.first = min(words, rank * share);
+    r.count = min(words - r.first, share);
+    r.edge = -1;
+    if (rank == 0 && tid < r.head) r.edge = tid;
+    if (rank == cluster - 1 && tid >= N && tid - N < vocab - tail) r.edge = tail + tid - N;
+    return r;
+}
+
+// f(i) for the words i = tid, tid + THREADS, ... below count, U at a time.
+template <int THREADS, int U, typename F>
+__device__ __forceinline__ void each_word(int tid, int count, F f) {
+    int i = tid;
+    for (; i + (U - 1) * THREADS < count; i += U * THREADS)
+#pragma unroll
+        for (int u = 0; u < U; ++u) f(i + u * THREADS);
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+        if (i + u * THREADS < count) f(i + u * THREADS);
+}
+
+template <typename T, int BLOCK>
+__global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
+    distill_kernel(DistillArgs a, int64_t rows, const T* z, float* __restrict__ loss, T* grad, int log_cluster) {
+    constexpr int N = kWordLogits<T>, threads = BLOCK - 32, warps = threads / 32;
+    const int cluster = 1 << log_cluster;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float2 warp_part[2][32], block_part[2];
+    uint4* stage = reinterpret_cast<uint4*>(smem + 2 * top_bytes(a.k));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int vocab = (int)a.vocab;
-    const int head = min(vocab, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / sizeof(T)));
-    const int words = (vocab - head) / N, share = (words + cluster - 1) / cluster;
-    const int first = min(words, rank * share), count = min(words - first, share);
-    const int tail = head + words * N;
-    int edge = -1;
-    if (rank == 0 && tid < head) edge = tid;
-    if (rank == cluster - 1 && tid >= N && tid - N < vocab - tail) edge = tail + tid - N;
-    const T* body = row + head + first * N;
-    const bool live = w != 0.0f;
-    uint32_t x[NV][4];
-    float edge_x = -INFINITY;
-    if (live) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
-            const int i = v * threads + tid;
-            const uint4 q = i < count ? reinterpret_cast<const uint4*>(body)[i] : make_uint4(kNone, kNone, kNone, kNone);
-            x[v][0] = q.x;
-            x[v][1] = q.y;
-            x[v][2] = q.z;
-            x[v][3] = q.w;
-        }
-        if (edge >= 0) edge_x = to_float(row[edge]);
-        if (warp == 0) load_teacher<T>(a, t, row, top);
-    }
+    const bool is_teacher = warp == warps;
+    const int rank = (int)blockIdx.x & (cluster - 1);
+    const int64_t workers = gridDim.x >> log_cluster;
     const float c2 = kLog2E / a.tau;
-    float m = -INFINITY, s = 0.0f;
-    if (live) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) m = fmaxf(m, word_max<T>(x[v]));
-        m = fmaxf(m, edge_x);
-        const float base = m == -INFINITY ? 0.0f : -m;
-        float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-            word_pairs<T>(x[v], [&](int, float2 f) {
-                f = mul2(add2(f, make_float2(base, base)), make_float2(c2, c2));
-                sum = add2(sum, make_float2(exp2_fast(f.x), exp2_fast(f.y)));
-            });
-        s = sum.x + sum.y + exp2_fast((edge_x + base) * c2);
-        join_warp(m, s, c2);
+    auto weight = [&](int64_t t) { return t >= rows ? 0.0f : a.weight != nullptr ? a.weight[t] : 1.0f; };
+    int64_t t = blockIdx.x >> log_cluster;
+    float w = weight(t);
+    const T* row = z + t * a.stride;
+    RowShare r = row_share<T>(row, vocab, rank, log_cluster, tid);
+    float edge_x = -INFINITY;
+    if (w != 0.0f) {
+        if (is_teacher) {
+            load_teacher<T>(a, t, row, TopList(smem, a.k));
+        } else {
+            const T* body = row + r.head + r.first * N;
+            each_word<threads, 4>(tid, r.count, [&](int i) { copy_vec<T, N>(reinterpret_cast<T*>(stage + i), body + i * N); });
+            if (r.edge >= 0) edge_x = to_float(row[r.edge]);
+        }
     }
-    if (lane == 0) warp_part[warp] = make_float2(m, s);
-    __syncthreads();
-    m = lane < warps ? warp_part[lane].x : -INFINITY;
-    s = lane < warps ? warp_part[lane].y : 0.0f;
-    join_warp(m, s, c2);
-    if (cluster > 1) {
-        namespace cg = cooperative_groups;
-        cg::cluster_group group = cg::this_cluster();
-        if (tid == 0) block_part = make_float2(m, s);
-        group.sync();
-        const float2 part = lane < cluster ? *group.map_shared_rank(&block_part, lane) : make_float2(-INFINITY, 0.0f);
-        m = part.x;
-        s = part.y;
-        join_warp(m, s, c2);
-    }
-    const bool any = live && top.any;
-    if (m == -INFINITY) m = 0.0f;
-    if (rank == 0 && warp == 0) {
-        const float l = any ? row_loss(a, top, w, m, s) : 0.0f;
-        if (lane == 0) loss[t] = l;
-    }
-    if (out != nullptr) {
-        const float inv_s = s == 0.0f ? 0.0f : 1.0f / s, c = any ? w * a.tau : 0.0f, ci = c * inv_s;
-        T* out_body = out + head + first * N;
-        const bool aligned = (reinterpret_cast<uintptr_t>(out_body) & 15) == 0;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int i = v * threads + tid;
-            if (i >= count) break;
-            uint32_t y[4] = {0, 0, 0, 0};
-            if (any)
-                word_pairs<T>(x[v], [&](int j, float2 f) {
-                    f = mul2(add2(f, make_float2(-m, -m)), make_float2(c2, c2));
-                    f = mul2(make_float2(exp2_fast(f.x), exp2_fast(f.y)), make_float2(ci, ci));
-                    if constexpr (sizeof(T) == 4) {
-                        y[2 * j] = __float_as_uint(f.x);
-                        y[2 * j + 1] = __float_as_uint(f.y);
-                    } else {
-                        y[j] = pack2<T>(f.x, f.y);
-                    }
+    copy_commit();
+    for (int b = 0; t < rows; t += workers, b ^= 1) {
+        const bool live = w != 0.0f;
+        const float w_next = weight(t + workers);
+        const T* row_next = row + workers * a.stride;
+        float m = -INFINITY, s = 0.0f;
+        // sum of the exponentials of the thread's logits
+        auto sum_words = [&](float base) {
+            float2 sum = make_float2(exp2_fast(fmaf(edge_x, c2, base)), 0.0f);
+            each_word<threads, 2>(tid, r.count, [&](int i) {
+                word_pairs<T>(stage[i], [&](int, float2 f) {
+                    f = __ffma2_rn(f, make_float2(c2, c2), make_float2(base, base));
+                    sum = __fadd2_rn(sum, make_float2(exp2_fast(f.x), exp2_fast(f.y)));
                 });
-            if (aligned) {
-                reinterpret_cast<uint4*>(out_body)[i] = make_uint4(y[0], y[1], y[2], y[3]);
-            } else {  // rows of logits that lie further apart than those of the gradient
-#pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if constexpr (sizeof(T) == 4)
-                        reinterpret_cast<uint32_t*>(out_body)[i * N + j] = y[j];
-                    else
-                        reinterpret_cast<uint16_t*>(out_body)[i * N + j] = (uint16_t)(y[j / 2] >> (16 * (j & 1)));
+            });
+            return sum.x + sum.y;
+        };
+        auto join_row = [&] {
+            if (!is_teacher) {
+                join_warp(m, s, c2);
+                if (lane == 0) warp_part[b][warp] = make_float2(m, s);
+            }
+            __syncthreads();
+            auto spread = [&](float2 part) {
+                m = part.x;
+                s = part.y;
+                join_warp<8>(m, s, c2);
+                m = __shfl_sync(0xffffffffu, m, 0);
+                s = __shfl_sync(0xffffffffu, s, 0);
+            };
+            spread(lane < warps ? warp_part[b][lane] : make_float2(-INFINITY, 0.0f));
+            if (cluster > 1) {
+                namespace cg = cooperative_groups;
+                cg::cluster_group group = cg::this_cluster();
+                if (tid == 0) block_part[b] = make_float2(m, s);
+                group.sync();
+                spread(lane < cluster ? *group.map_shared_rank(&block_part[b], lane) : make_float2(-INFINITY, 0.0f));
+            }
+        };
+        if (!is_teacher) {
+            copy_wait<0>();
+            if (live) {
+                WordMax<T> top_word;
+                each_word<threads, 4>(tid, r.count, [&](int i) { top_word.add(stage[i]); });
+                m = fmaxf(top_word.get(), edge_x);
+                s = sum_words(minus_b(m, c2));
             }
         }
-        if (edge >= 0) out[edge] = from_float<T>(any ? ci * exp2_fast((edge_x - m) * c2) : 0.0f);
-        if (any) {
-            __syncthreads();
-            const int v0 = rank == 0 ? 0 : head + first * N, v1 = rank == cluster - 1 ? vocab : head + (first + count) * N;
-            top_gradients<T>(a, top, out, v0, v1, c, c2, m, inv_s);
+        join_row();
+        const TopList top(smem + b * top_bytes(a.k), a.k);
+        const bool any = live && *top.any;
+        if (fabsf(m) != INFINITY && fabsf(m * c2) > kFar) {
+            // every logit is about the type's lowest value, say: the row becomes z - max, whose
+            // rounding such distances do not feel
+            if (!is_teacher) {
+                each_word<threads, 1>(tid, r.count, [&](int i) {
+                    T e[N];
+                    *reinterpret_cast<uint4*>(e) = stage[i];
+#pragma unroll
+                    for (int j = 0; j < N; ++j) e[j] = from_float<T>(to_float(e[j]) - m);
+                    stage[i] = *reinterpret_cast<const uint4*>(e);
+                });
+                edge_x -= m;
+            } else {
+                for (int k = lane; k < a.k; k += 32) top.z[k] -= m;
+            }
+            m = 0.0f;
+            if (!is_teacher) s = sum_words(0.0f);
+            __syncthreads();  // the parts of the first join have been read
+            if (cluster > 1) cooperative_groups::this_cluster().sync();
+            join_row();
         }
+        if (m == INFINITY) s = NAN;
+        const float base = minus_b(m, c2);
+        if (is_teacher) {
+            if (rank == 0) {
+                const float l = any ? row_loss(a, top, w, c2, base, s) : 0.0f;
+                if (lane == 0) loss[t] = l;
+            }
+            if (w_next != 0.0f)
+                load_teacher<T>(a, t + workers, row_next, TopList(smem + (b ^ 1) * top_bytes(a.k), a.k));
+        } else {
+            RowShare n = row_share<T>(row_next, vocab, rank, log_cluster, tid);
+            const int fetched = w_next != 0.0f ? n.count : 0;
+            const T* body_next = row_next + n.head + n.first * N;
+            const float edge_now = edge_x;
+            edge_x = w_next != 0.0f && n.edge >= 0 ? to_float(row_next[n.edge]) : -INFINITY;
+            auto fetch = [&](int i) { copy_vec<T, N>(reinterpret_cast<T*>(stage + i), body_next + i * N); };
+            if (grad == nullptr) {
+                each_word<threads, 4>(tid, fetched, fetch);
+            } else {
+                T* out = grad + t * a.vocab;
+                T* body = out + r.head + r.first * N;
+                const float c = w * a.tau, inv_s = s == 0.0f ? 0.0f : 1.0f / s, ci = c * inv_s;
+                auto gradients = [&](int i) {
+                    uint32_t o[4];
+                    word_pairs<T>(stage[i], [&](int j, float2 f) {
+                        f = __ffma2_rn(f, make_float2(c2, c2), make_float2(base, base));
+                        f = __fmul2_rn(make_float2(exp2_fast(f.x), exp2_fast(f.y)), make_float2(ci, ci));
+                        if constexpr (sizeof(T) == 4) {
+                            o[2 * j] = __float_as_uint(f.x);
+                            o[2 * j + 1] = __float_as_uint(f.y);
+                        } else {
+                            o[j] = pack2<T>(f.x, f.y);
+                        }
+                    });
+                    return make_uint4(o[0], o[1], o[2], o[3]);
+                };
+                if (any && (reinterpret_cast<uintptr_t>(body) & 15) == 0) {
+                    each_word<threads, 2>(tid, r.count, [&](int i) {
+                        reinterpret_cast<uint4*>(body)[i] = gradients(i);
+                        if (i < fetched) fetch(i);
+                    });
+                    // the next row may begin at another alignment and have one word more
+                    if (r.count < fetched && (fetched - 1) % threads == tid) fetch(fetched - 1);
+                } else if (!any && (reinterpret_cast<uintptr_t>(body) & 15) == 0) {
+                    each_word<threads, 4>(tid, r.count, [&](int i) {
+                        reinterpret_cast<uint4*>(body)[i] = make_uint4(0, 0, 0, 0);
+                    });
+                    each_word<threads, 4>(tid, fetched, fetch);
+                } else {  // rows of logits that lie further apart than those of the gradient
+                    each_word<threads, 1>(tid, r.count, [&](int i) {
+                        T e[N];
+                        *reinterpret_cast<uint4*>(e) = any ? gradients(i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                        for (int j = 0; j < N; ++j) body[i * N + j] = e[j];
+                    });
+                    each_word<threads, 4>(tid, fetched, fetch);
+                }
+                if (r.edge >= 0) out[r.edge] = from_float<T>(any ? ci * exp2_fast(fmaf(edge_now, c2, base)) : 0.0f);
+                if (any) {
+                    asm volatile("bar.sync 1, %0;" ::"n"(threads) : "memory");  // the row is written
+                    const int v0 = rank == 0 ? 0 : r.head + r.first * N;
+                    const int v1 = rank == cluster - 1 ? vocab : r.head + (r.first + r.count) * N;
+                    top_gradients<T>(a, top, out, threads, v0, v1, c, c2, base, inv_s);
+                }
+            }
+            copy_commit();
+            r = n;
+        }
+        row = row_next;
+        w = w_next;
     }
     if (cluster > 1) cooperative_groups::this_cluster().sync();  // a peer may still read this block's part
 }
@@ -276,15 +405,16 @@ __global__ void __launch_bounds__(NV == kDistillVecs ? 1024 : kDistillThreads)
 template <typename T>
 __global__ void __launch_bounds__(1024) distill_long_kernel(DistillArgs a, const T* z, float* __restrict__ loss,
                                                             T* grad) {
-    __shared__ TopList top;
+    extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float sh[32];
+    const TopList top(smem, a.k);
     const int64_t t = blockIdx.x;
     const T* row = z + t * a.stride;
     T* out = grad != nullptr ? grad + t * a.vocab : nullptr;
     const float w = a.weight != nullptr ? a.weight[t] : 1.0f;
     if (w != 0.0f && threadIdx.x < 32) load_teacher<T>(a, t, row, top);
     __syncthreads();
-    if (w == 0.0f || !top.any) {
+    if (w == 0.0f || !*top.any) {
         if (out != nullptr)
             for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) out[v] = from_float<T>(0.0f);
         if (threadIdx.x == 0) loss[t] = 0.0f;
@@ -295,39 +425,38 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(DistillArgs a, const
     for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) m = fmaxf(m, to_float(row[v]));
     m = block_max(m, sh);
     if (m == -INFINITY) m = 0.0f;
+    // the difference first: no B that could overflow
+    auto term = [&](float x) { return exp2_fast((x - m) * c2); };
     float s = 0.0f;
-    for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) s += exp2_fast((to_float(row[v]) - m) * c2);
+    for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) s += term(to_float(row[v]));
     s = block_sum(s, sh);
     if (threadIdx.x < 32) {
-        const float l = row_loss(a, top, w, m, s);
+        for (int k = threadIdx.x; k < a.k; k += 32) top.z[k] -= m;
+        __syncwarp();
+        const float l = row_loss(a, top, w, c2, 0.0f, s);
         if (threadIdx.x == 0) loss[t] = l;
     }
     if (out == nullptr) return;
     const float inv_s = s == 0.0f ? 0.0f : 1.0f / s, c = w * a.tau;
-    for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x)
-        out[v] = from_float<T>(c * inv_s * exp2_fast((to_float(row[v]) - m) * c2));
+    for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) out[v] = from_float<T>(c * inv_s * term(to_float(row[v])));
     __syncthreads();
-    top_gradients<T>(a, top, out, 0, a.vocab, c, c2, m, inv_s);
+    top_gradients<T>(a, top, out, (int)blockDim.x, 0, (int)a.vocab, c, c2, 0.0f, inv_s);
 }
 
-// Threads and words of a thread for a block's share of a row.
+// Blocks of a row and their threads.
 struct DistillPlan {
-    int cluster, threads, vecs;  // cluster 0: the kernel for longer rows
+    int cluster, threads;  // cluster 0: the kernel for longer rows
+    int64_t share;         // words of a block
 };
 static DistillPlan distill_plan(int64_t n, int64_t words) {
-    DistillPlan p{1, kDistillThreads, 1};
-    while (p.cluster < 8 && words > (int64_t)p.cluster * kDistillThreads * kDistillVecs) p.cluster *= 2;
-    if (words > (int64_t)p.cluster * kDistillThreads * kDistillVecs) {
-        p.threads = 1024;
-        if (words > (int64_t)p.cluster * p.threads * kDistillVecs) p.cluster = 0;
-        p.vecs = kDistillVecs;
-        return p;
-    }
+    DistillPlan p{1, kDistillThreads, 0};
+    while (p.cluster < 8 && words * 16 > (int64_t)p.cluster * kDistillShare) p.cluster *= 2;
+    if (words * 16 > (int64_t)p.cluster * kDistillLongShare) p.cluster = 0;
+    if (p.cluster == 0) return p;
     // few rows: more blocks a row, as long as each of their threads has a word
     while (p.cluster < 8 && n * p.cluster < 2 * 148 && words >= 2 * p.cluster * kDistillThreads) p.cluster *= 2;
-    const int64_t share = ceil_div(words, p.cluster);
-    while (p.threads > 64 && share <= p.threads / 2) p.threads /= 2;
-    while ((int64_t)p.vecs * p.threads < share) p.vecs *= 2;
+    p.share = ceil_div(words, p.cluster);
+    while (p.threads > kDistillThreads / 4 && p.share <= p.threads / 2) p.threads /= 2;
     return p;
 }
 
@@ -367,32 +496,45 @@ int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, 
         const cudaStream_t s = (cudaStream_t)stream;
         const DistillPlan p = distill_plan(n, vocab / N);
         if (p.cluster == 0) {
-            distill_long_kernel<T><<<(unsigned)n, 1024, 0, s>>>(a, z, loss, g);
+            distill_long_kernel<T><<<(unsigned)n, 1024, top_bytes(a.k), s>>>(a, z, loss, g);
             CRESSO_LAUNCHED("distill_long_kernel");
             return (int)CRESSO_OK;
         }
-        CRESSO_REQUIRE(n * p.cluster <= CRESSO_TRAIN_MAX_ROWS, CRESSO_EUNSUPPORTED, "distill: too many rows");
-        auto launch = [&](auto kernel) {
-            cudaLaunchConfig_t cfg{};
-            cfg.gridDim = dim3((unsigned)(n * p.cluster));
-            cfg.blockDim = dim3((unsigned)p.threads);
-            cfg.stream = s;
-            cudaLaunchAttribute attr{};
-            attr.id = cudaLaunchAttributeClusterDimension;
-            attr.val.clusterDim.x = (unsigned)p.cluster;
-            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-            cfg.attrs = &attr;
-            cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-            CRESSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, z, loss, g, p.cluster));
-            CRESSO_LAUNCHED("distill_kernel");
-            return (int)CRESSO_OK;
-        };
-        switch (p.vecs) {
-            case 1: return launch(distill_kernel<T, 1>);
-            case 2: return launch(distill_kernel<T, 2>);
-            case 4: return launch(distill_kernel<T, 4>);
-            default: return launch(distill_kernel<T, kDistillVecs>);
+        const int smem = (int)p.share * 16 + 2 * top_bytes(a.k);
+        const auto kernel = p.threads == kDistillThreads       ? distill_kernel<T, kDistillThreads>
+                            : p.threads == kDistillThreads / 2 ? distill_kernel<T, kDistillThreads / 2>
+                                                               : distill_kernel<T, kDistillThreads / 4>;
+        if (smem > 48 * 1024)
+            CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             kDistillLongShare + 2 * top_bytes(CRESSO_TRAIN_MAX_TOP)));
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)p.cluster);
+        cfg.blockDim = dim3((unsigned)p.threads);
+        cfg.dynamicSmemBytes = (size_t)smem;
+        cfg.stream = s;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = (unsigned)p.cluster;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+        int64_t workers = n;  // as many as stay on the GPU together
+        if (n * p.cluster > 148) {
+            int fit = 0;
+            if (p.cluster > 1) {
+                CRESSO_CUDA(cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg));
+            } else {
+                CRESSO_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, p.threads, (size_t)smem));
+                fit *= 148;
+            }
+            workers = std::min<int64_t>(n, std::max(1, fit));
         }
+        cfg.gridDim = dim3((unsigned)(workers * p.cluster));
+        int log_cluster = 0;
+        while ((1 << log_cluster) < p.cluster) ++log_cluster;
+        CRESSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, n, z, loss, g, log_cluster));
+        CRESSO_LAUNCHED("distill_kernel");
+        return (int)CRESSO_OK;
     });
 }
 
