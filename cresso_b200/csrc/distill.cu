@@ -10,7 +10,7 @@
 // operation, whose error is that of its result, because the same B stands in the sum, in
 // the gradient and in the loss.  Sums are float32.  A NaN or +inf logit makes its row NaN
 // through the sum; a row of -inf alone has q = 0.  Repeated
-// ids: every entry forms the whole P of its id, so that all of them write the same value.
+// ids: every entry holds the whole P of its id, so that all of them write the same value.
 #include "train_common.cuh"
 
 #include <cooperative_groups.h>
@@ -28,17 +28,25 @@ struct DistillArgs {
     float tau;
 };
 
-// The teacher's side of a row in shared memory: k ids (-1: not valid), teacher probabilities
-// and student logits at the ids, then the sum of p log p and whether a valid entry exists.
+// The teacher's side of a row in shared memory: k ids (-1: not valid), teacher probabilities,
+// their sums over equal ids and student logits at the ids, then the sum of p log p and whether
+// a valid entry exists.
 struct TopList {
     int* id;
-    float *p, *z, *entropy;
+    float *p, *same, *z, *entropy;
     int* any;
     __device__ __forceinline__ TopList(unsigned char* at, int k)
-        : id(reinterpret_cast<int*>(at)), p(reinterpret_cast<float*>(at) + k), z(p + k), entropy(z + k),
+        : id(reinterpret_cast<int*>(at)), p(reinterpret_cast<float*>(at) + k), same(p + k), z(same + k), entropy(z + k),
           any(reinterpret_cast<int*>(entropy + 1)) {}
 };
-__host__ __device__ constexpr int top_bytes(int k) { return (12 * k + 8 + 15) / 16 * 16; }
+__host__ __device__ constexpr int top_bytes(int k) { return (16 * k + 8 + 15) / 16 * 16; }
+
+// One warp's set of bits that finds ids that may occur twice, and the list of those.
+constexpr int kSeenBits = 16384;
+struct Seen {
+    uint32_t bits[kSeenBits / 32];
+    int count, id[CRESSO_TRAIN_MAX_TOP];
+};
 
 constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -48,30 +56,51 @@ __device__ __forceinline__ float exp2_fast(float x) {  // relative error 2^-22
     return y;
 }
 
-// Fills the list with one warp; the block sees it after its next barrier.
+// Fills the list with one warp; the block sees it after its next barrier.  Four entries a lane
+// have their loads in flight together.
 template <typename T>
-__device__ __forceinline__ void load_teacher(const DistillArgs& a, int64_t t, const T* row, const TopList& top) {
+__device__ __forceinline__ void load_teacher(const DistillArgs& a, int64_t t, const T* row, const TopList& top, Seen& seen) {
     const int lane = threadIdx.x & 31;
+    const int64_t at = t * a.k;
     float m = -INFINITY;
-#pragma unroll 4
-    for (int k = lane; k < a.k; k += 32) {
-        const int64_t id = load_id(a.ids, a.id_bytes, t * a.k + k);
-        const float u = load_any(a.teacher, a.teacher_dtype, t * a.k + k);
-        const bool valid = id >= 0 && id < a.vocab && u != -INFINITY;
-        top.id[k] = valid ? (int)id : -1;
-        top.p[k] = u;
-        if (valid) m = fmaxf(m, u);
+    for (int i = lane; i < kSeenBits / 32; i += 32) seen.bits[i] = 0;
+    if (lane == 0) seen.count = 0;
+    for (int k0 = 0; k0 < a.k; k0 += 128) {
+        int64_t id[4];
+        float u[4], z[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = min(k0 + 32 * j + lane, a.k - 1);
+            id[j] = load_id(a.ids, a.id_bytes, at + k);
+            u[j] = load_any(a.teacher, a.teacher_dtype, at + k);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (!(id[j] >= 0 && id[j] < a.vocab && u[j] != -INFINITY)) id[j] = -1;
+            z[j] = to_float(row[max(id[j], (int64_t)0)]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = k0 + 32 * j + lane;
+            if (k >= a.k) break;
+            top.id[k] = (int)id[j];
+            top.p[k] = u[j];
+            top.z[k] = z[j];
+            if (id[j] >= 0) m = fmaxf(m, u[j]);
+        }
     }
-#pragma unroll 4
-    for (int k = lane; k < a.k; k += 32) top.z[k] = top.id[k] >= 0 ? to_float(row[top.id[k]]) : 0.0f;
+    __syncwarp();
     m = warp_max(m);
     const float inv_tau = 1.0f / a.tau;
     float s = 0.0f;
     bool valid_here = false;
     for (int k = lane; k < a.k; k += 32) {
-        if (top.id[k] < 0) continue;
+        const int id = top.id[k];
+        if (id < 0) continue;
         valid_here = true;
         s += expf((top.p[k] - m) * inv_tau);
+        const uint32_t h = ((uint32_t)id * 2654435769u) >> 18;  // multiplicative hash to kSeenBits
+        if (atomicOr(&seen.bits[h >> 5], 1u << (h & 31)) >> (h & 31) & 1u) seen.id[atomicAdd(&seen.count, 1)] = id;
     }
     const bool any = __any_sync(0xffffffffu, valid_here);
     s = warp_sum(s);
@@ -82,11 +111,25 @@ __device__ __forceinline__ void load_teacher(const DistillArgs& a, int64_t t, co
         const float p = top.id[k] >= 0 ? expf(lp) : 0.0f;
         if (p != 0.0f) entropy += p * lp;
         top.p[k] = p;
+        top.same[k] = p;
     }
     entropy = warp_sum(entropy);
     if (lane == 0) {
         *top.entropy = entropy;
         *top.any = any;
+    }
+    __syncwarp();
+    // an id that occurs twice is in seen.id, whatever the order of the insertions was
+    const int count = seen.count;
+    if (count == 0) return;
+    for (int k = lane; k < a.k; k += 32) {
+        const int id = top.id[k];
+        bool twice = false;
+        for (int j = 0; j < count && !twice; ++j) twice = seen.id[j] == id;
+        if (id < 0 || !twice) continue;
+        float p = 0.0f;
+        for (int j = 0; j < a.k; ++j) p += top.id[j] == id ? top.p[j] : 0.0f;
+        top.same[k] = p;
     }
     __syncwarp();
 }
@@ -127,10 +170,8 @@ __device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopLis
                                               float c, float c2, float base, float inv_s) {
     for (int k = threadIdx.x; k < a.k; k += threads) {
         const int id = top.id[k];
-        if (id < v0 || id >= v1) continue;
-        float p = 0.0f;
-        for (int j = 0; j < a.k; ++j) p += top.id[j] == id ? top.p[j] : 0.0f;
-        out[id] = from_float<T>(c * (exp2_fast(fmaf(top.z[k], c2, base)) * inv_s - p));
+        if (id >= v0 && id < v1)
+            out[id] = from_float<T>(c * (exp2_fast(fmaf(top.z[k], c2, base)) * inv_s - top.same[k]));
     }
 }
 
@@ -231,6 +272,7 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
     const int cluster = 1 << log_cluster;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float2 warp_part[2][32], block_part[2];
+    __shared__ Seen seen;
     uint4* stage = reinterpret_cast<uint4*>(smem + 2 * top_bytes(a.k));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int vocab = (int)a.vocab;
@@ -246,7 +288,7 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
     float edge_x = -INFINITY;
     if (w != 0.0f) {
         if (is_teacher) {
-            load_teacher<T>(a, t, row, TopList(smem, a.k));
+            load_teacher<T>(a, t, row, TopList(smem, a.k), seen);
         } else {
             const T* body = row + r.head + r.first * N;
             each_word<threads, 4>(tid, r.count, [&](int i) { copy_vec<T, N>(reinterpret_cast<T*>(stage + i), body + i * N); });
@@ -301,26 +343,30 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
                 s = sum_words(minus_b(m, c2));
             }
         }
+        // the next row
+        const RowShare n = row_share<T>(row_next, vocab, rank, log_cluster, tid);
+        const int fetched = w_next != 0.0f && !is_teacher ? n.count : 0;
+        const T* body_next = row_next + n.head + n.first * N;
+        auto fetch = [&](int i) { copy_vec<T, N>(reinterpret_cast<T*>(stage + i), body_next + i * N); };
+        float edge_now = edge_x;
+        if (!is_teacher) edge_x = w_next != 0.0f && n.edge >= 0 ? to_float(row_next[n.edge]) : -INFINITY;
+        if (grad == nullptr) each_word<threads, 4>(tid, fetched, fetch);
         join_row();
         const TopList top(smem + b * top_bytes(a.k), a.k);
         const bool any = live && *top.any;
-        if (fabsf(m) != INFINITY && fabsf(m * c2) > kFar) {
-            // every logit is about the type's lowest value, say: the row becomes z - max, whose
-            // rounding such distances do not feel
-            if (!is_teacher) {
-                each_word<threads, 1>(tid, r.count, [&](int i) {
-                    T e[N];
-                    *reinterpret_cast<uint4*>(e) = stage[i];
-#pragma unroll
-                    for (int j = 0; j < N; ++j) e[j] = from_float<T>(to_float(e[j]) - m);
-                    stage[i] = *reinterpret_cast<const uint4*>(e);
-                });
-                edge_x -= m;
-            } else {
-                for (int k = lane; k < a.k; k += 32) top.z[k] -= m;
-            }
+        const T* body_now = row + r.head + r.first * N;
+        const float far = fabsf(m) != INFINITY && fabsf(m * c2) > kFar ? m : 0.0f;
+        if (far != 0.0f) {
+            // every logit is about the type's lowest value, say: the exponents of z - max
             m = 0.0f;
-            if (!is_teacher) s = sum_words(0.0f);
+            s = 0.0f;
+            edge_now -= far;
+            if (is_teacher) {
+                for (int k = lane; k < a.k; k += 32) top.z[k] -= far;
+            } else {
+                s = exp2_fast(edge_now * c2);
+                for (int i = tid; i < r.count * N; i += threads) s += exp2_fast((to_float(body_now[i]) - far) * c2);
+            }
             __syncthreads();  // the parts of the first join have been read
             if (cluster > 1) cooperative_groups::this_cluster().sync();
             join_row();
@@ -333,17 +379,9 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
                 if (lane == 0) loss[t] = l;
             }
             if (w_next != 0.0f)
-                load_teacher<T>(a, t + workers, row_next, TopList(smem + (b ^ 1) * top_bytes(a.k), a.k));
+                load_teacher<T>(a, t + workers, row_next, TopList(smem + (b ^ 1) * top_bytes(a.k), a.k), seen);
         } else {
-            RowShare n = row_share<T>(row_next, vocab, rank, log_cluster, tid);
-            const int fetched = w_next != 0.0f ? n.count : 0;
-            const T* body_next = row_next + n.head + n.first * N;
-            const float edge_now = edge_x;
-            edge_x = w_next != 0.0f && n.edge >= 0 ? to_float(row_next[n.edge]) : -INFINITY;
-            auto fetch = [&](int i) { copy_vec<T, N>(reinterpret_cast<T*>(stage + i), body_next + i * N); };
-            if (grad == nullptr) {
-                each_word<threads, 4>(tid, fetched, fetch);
-            } else {
+            if (grad != nullptr) {
                 T* out = grad + t * a.vocab;
                 T* body = out + r.head + r.first * N;
                 const float c = w * a.tau, inv_s = s == 0.0f ? 0.0f : 1.0f / s, ci = c * inv_s;
@@ -361,7 +399,7 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
                     });
                     return make_uint4(o[0], o[1], o[2], o[3]);
                 };
-                if (any && (reinterpret_cast<uintptr_t>(body) & 15) == 0) {
+                if (any && far == 0.0f && (reinterpret_cast<uintptr_t>(body) & 15) == 0) {
                     each_word<threads, 2>(tid, r.count, [&](int i) {
                         reinterpret_cast<uint4*>(body)[i] = gradients(i);
                         if (i < fetched) fetch(i);
@@ -373,12 +411,14 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
                         reinterpret_cast<uint4*>(body)[i] = make_uint4(0, 0, 0, 0);
                     });
                     each_word<threads, 4>(tid, fetched, fetch);
-                } else {  // rows of logits that lie further apart than those of the gradient
+                } else {  // rows of logits that lie further apart than those of the gradient, or far ones
                     each_word<threads, 1>(tid, r.count, [&](int i) {
                         T e[N];
-                        *reinterpret_cast<uint4*>(e) = any ? gradients(i) : make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(e) = stage[i];
 #pragma unroll
-                        for (int j = 0; j < N; ++j) body[i * N + j] = e[j];
+                        for (int j = 0; j < N; ++j)
+                            body[i * N + j] =
+                                from_float<T>(any ? ci * exp2_fast(fmaf(to_float(e[j]) - far, c2, base)) : 0.0f);
                     });
                     each_word<threads, 4>(tid, fetched, fetch);
                 }
@@ -407,12 +447,13 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(DistillArgs a, const
                                                             T* grad) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float sh[32];
+    __shared__ Seen seen;
     const TopList top(smem, a.k);
     const int64_t t = blockIdx.x;
     const T* row = z + t * a.stride;
     T* out = grad != nullptr ? grad + t * a.vocab : nullptr;
     const float w = a.weight != nullptr ? a.weight[t] : 1.0f;
-    if (w != 0.0f && threadIdx.x < 32) load_teacher<T>(a, t, row, top);
+    if (w != 0.0f && threadIdx.x < 32) load_teacher<T>(a, t, row, top, seen);
     __syncthreads();
     if (w == 0.0f || !*top.any) {
         if (out != nullptr)
