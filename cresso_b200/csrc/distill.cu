@@ -267,12 +267,14 @@ __device__ __forceinline__ void each_word(int tid, int count, F f) {
 
 template <typename T, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
-    distill_kernel(DistillArgs a, int64_t rows, const T* z, float* __restrict__ loss, T* grad, int log_cluster) {
+    distill_kernel(DistillArgs a, int64_t rows, const T* z, float* __restrict__ loss, T* grad, int log_cluster,
+                   unsigned long long* tickets) {
     constexpr int N = kWordLogits<T>, threads = BLOCK - 32, warps = threads / 32;
     const int cluster = 1 << log_cluster;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float2 warp_part[2][32], block_part[2];
     __shared__ Seen seen;
+    __shared__ int64_t ticket[2];
     uint4* stage = reinterpret_cast<uint4*>(smem + 2 * top_bytes(a.k));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int vocab = (int)a.vocab;
@@ -281,9 +283,15 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
     const int64_t workers = gridDim.x >> log_cluster;
     const float c2 = kLog2E / a.tau;
     auto weight = [&](int64_t t) { return t >= rows ? 0.0f : a.weight != nullptr ? a.weight[t] : 1.0f; };
-    int64_t t = blockIdx.x >> log_cluster;
+    // The first two rows of a block (cluster) are its own, the others come by ticket, since masked
+    // rows take no time.  The ticket of a row is taken two rows ahead.
+    int64_t t = blockIdx.x >> log_cluster, t1 = t + workers, pending = rows;
     float w = weight(t);
     const T* row = z + t * a.stride;
+    auto take = [&](bool more) {
+        if (is_teacher && lane == 0 && rank == 0) pending = more ? 2 * workers + (int64_t)atomicAdd(tickets, 1ull) : rows;
+    };
+    take(t1 < rows);
     RowShare r = row_share<T>(row, vocab, rank, log_cluster, tid);
     float edge_x = -INFINITY;
     if (w != 0.0f) {
@@ -296,10 +304,11 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
         }
     }
     copy_commit();
-    for (int b = 0; t < rows; t += workers, b ^= 1) {
+    for (int b = 0; t < rows; b ^= 1) {
         const bool live = w != 0.0f;
-        const float w_next = weight(t + workers);
-        const T* row_next = row + workers * a.stride;
+        const float w_next = weight(t1);
+        const T* row_next = z + t1 * a.stride;
+        if (is_teacher && lane == 0) ticket[b] = pending;
         float m = -INFINITY, s = 0.0f;
         // sum of the exponentials of the thread's logits
         auto sum_words = [&](float base) {
@@ -352,6 +361,8 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
         if (!is_teacher) edge_x = w_next != 0.0f && n.edge >= 0 ? to_float(row_next[n.edge]) : -INFINITY;
         if (grad == nullptr) each_word<threads, 4>(tid, fetched, fetch);
         join_row();
+        const int64_t t2 =
+            cluster > 1 ? *cooperative_groups::this_cluster().map_shared_rank(&ticket[b], 0) : ticket[b];
         const TopList top(smem + b * top_bytes(a.k), a.k);
         const bool any = live && *top.any;
         const T* body_now = row + r.head + r.first * N;
@@ -378,8 +389,9 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
                 const float l = any ? row_loss(a, top, w, c2, base, s) : 0.0f;
                 if (lane == 0) loss[t] = l;
             }
+            take(t2 < rows);
             if (w_next != 0.0f)
-                load_teacher<T>(a, t + workers, row_next, TopList(smem + (b ^ 1) * top_bytes(a.k), a.k), seen);
+                load_teacher<T>(a, t1, row_next, TopList(smem + (b ^ 1) * top_bytes(a.k), a.k), seen);
         } else {
             if (grad != nullptr) {
                 T* out = grad + t * a.vocab;
@@ -433,6 +445,8 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
             copy_commit();
             r = n;
         }
+        t = t1;
+        t1 = t2;
         row = row_next;
         w = w_next;
     }
@@ -484,6 +498,8 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(DistillArgs a, const
     top_gradients<T>(a, top, out, (int)blockDim.x, 0, (int)a.vocab, c, c2, 0.0f, inv_s);
 }
 
+constexpr int64_t kDistillScratch = 32;  // the ticket counter
+
 // Blocks of a row and their threads.
 struct DistillPlan {
     int cluster, threads;  // cluster 0: the kernel for longer rows
@@ -507,9 +523,17 @@ using namespace cresso;
 
 extern "C" {
 
+int cresso_distill_scratch_bytes(int64_t n, int64_t vocab, int64_t* bytes) {
+    CRESSO_REQUIRE(bytes != nullptr, CRESSO_EINVAL, "distill_scratch_bytes: NULL result");
+    CRESSO_REQUIRE(n >= 0 && vocab >= 1, CRESSO_EINVAL, "distill: negative size, or an empty vocabulary");
+    *bytes = kDistillScratch;
+    return CRESSO_OK;
+}
+
 int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, int64_t logits_stride, const void* ids,
                    int64_t id_bytes, const void* teacher, int64_t teacher_dtype, int64_t k, const float* weight,
-                   double temperature, float* loss, void* grad, cresso_stream_t stream) {
+                   double temperature, float* loss, void* grad, void* scratch, int64_t scratch_bytes,
+                   cresso_stream_t stream) {
     CRESSO_REQUIRE(train_dtype_ok(dtype) && train_dtype_ok(teacher_dtype), CRESSO_EUNSUPPORTED,
                    "distill: element types are float32, float16 and bfloat16");
     CRESSO_REQUIRE(id_bytes == 4 || id_bytes == 8, CRESSO_EINVAL, "distill: ids are int32 or int64");
@@ -525,6 +549,10 @@ int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, 
     if (n == 0) return CRESSO_OK;
     CRESSO_REQUIRE(logits != nullptr && loss != nullptr && (k == 0 || (ids != nullptr && teacher != nullptr)),
                    CRESSO_EINVAL, "distill: NULL pointer");
+    CRESSO_REQUIRE(scratch != nullptr && scratch_bytes >= kDistillScratch, CRESSO_ESCRATCH,
+                   "distill: scratch has %lld bytes, %lld are needed", (long long)scratch_bytes,
+                   (long long)kDistillScratch);
+    CRESSO_REQUIRE(aligned_to(scratch, 32), CRESSO_EINVAL, "distill: scratch is not 32-byte aligned");
     CRESSO_REQUIRE(grad != logits || logits_stride == vocab, CRESSO_EINVAL,
                    "distill: a gradient in place of the logits needs contiguous rows");
     NvtxRange range("distill n=%lld", (long long)n);
@@ -573,7 +601,9 @@ int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, 
         cfg.gridDim = dim3((unsigned)(workers * p.cluster));
         int log_cluster = 0;
         while ((1 << log_cluster) < p.cluster) ++log_cluster;
-        CRESSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, n, z, loss, g, log_cluster));
+        unsigned long long* tickets = static_cast<unsigned long long*>(scratch);
+        if (n > workers) CRESSO_CUDA(cudaMemsetAsync(tickets, 0, 8, s));
+        CRESSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, n, z, loss, g, log_cluster, tickets));
         CRESSO_LAUNCHED("distill_kernel");
         return (int)CRESSO_OK;
     });

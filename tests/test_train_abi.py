@@ -47,7 +47,8 @@ def _egrad(**kw):
 @pytest.mark.parametrize("kw,status", [
     (dict(gd=3), 2), (dict(od=9), 2), (dict(tb=1), 1), (dict(stride=7), 1), (dict(n=-1), 1), (dict(rows=-2), 1),
     (dict(n=2**31), 2), (dict(rows=2**31), 2), (dict(out=0), 1), (dict(grad=0), 1), (dict(tokens=0), 1),
-    (dict(scratch=0), 4), (dict(nbytes=16), 4), (dict(rows=0, out=0), 0), (dict(width=0, stride=0, out=0), 0),
+    (dict(scratch=0), 4), (dict(nbytes=16), 4), (dict(scratch=4104), 1), (dict(width=4194241, stride=4194241), 2),
+    (dict(rows=0, out=0), 0), (dict(width=0, stride=0, out=0), 0),
     (dict(n=0, accumulate=1), 0)])
 def test_embedding_grad_status(kw, status):
     assert _egrad(**kw) == status, _lib.last_error()
@@ -91,14 +92,15 @@ def _ngrad(**kw):
     (dict(rd=1, ad=2), 2), (dict(wd=4), 2), (dict(n=-1), 1), (dict(gate_rows=4), 1), (dict(h=0), 1),
     (dict(dres=0), 1), (dict(dh=0, dy=0, dpre=0), 1), (dict(pre=0), 1), (dict(x=0), 1), (dict(dx=0), 1),
     (dict(dpost=0), 1), (dict(dpre=0), 1), (dict(dgate=0), 1), (dict(post=0), 1), (dict(gate=0), 1),
-    (dict(scratch=0), 4), (dict(nbytes=8), 4), (dict(eps=-1.0), 1), (dict(width=0), 0)])
+    (dict(scratch=0), 4), (dict(nbytes=8), 4), (dict(scratch=4104), 1), (dict(width=65537), 2), (dict(eps=-1.0), 1),
+    (dict(width=0), 0)])
 def test_block_norm_grad_status(kw, status):
     assert _ngrad(**kw) == status, _lib.last_error()
 
 
 def _distill(**kw):
     a = dict(logits=4096, dt=0, n=4, vocab=10, stride=10, ids=4096, ib=8, teacher=4096, td=0, k=3, weight=0, tau=1.0,
-             loss=4096, grad=8192)
+             loss=4096, grad=8192, scratch=4096, nbytes=64)
     a.update(kw)
     return _lib.lib().cresso_distill(*a.values(), None)
 
@@ -107,7 +109,8 @@ def _distill(**kw):
     (dict(dt=3), 2), (dict(td=3), 2), (dict(ib=2), 1), (dict(n=-1), 1), (dict(vocab=0), 1), (dict(stride=9), 1),
     (dict(k=-1), 1), (dict(k=1025), 2), (dict(n=2**31), 2), (dict(tau=0.0), 1), (dict(tau=-1.0), 1),
     (dict(tau=float("nan")), 1), (dict(tau=float("inf")), 1), (dict(logits=0), 1), (dict(loss=0), 1),
-    (dict(ids=0), 1), (dict(teacher=0), 1), (dict(stride=12, grad=4096), 1), (dict(n=0), 0)])
+    (dict(ids=0), 1), (dict(teacher=0), 1), (dict(stride=12, grad=4096), 1), (dict(scratch=0), 4),
+    (dict(nbytes=8), 4), (dict(scratch=4104), 1), (dict(n=0), 0)])
 def test_distill_status(kw, status):
     assert _distill(**kw) == status, _lib.last_error()
 
