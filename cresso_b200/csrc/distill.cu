@@ -6,11 +6,14 @@
 //   p = softmax(u / tau) over the valid entries,  q = softmax(z / tau) over V,
 //   loss = w tau^2 sum_k p_k (log p_k - log q[id_k]),
 //   dz_v = w tau (q_v - P_v),  P_v = sum of p_k with id_k = v.
-// Exponentials are 2^(z c - B) with c = log2(e) / tau and B = max(z) c rounded: one fused
-// operation, whose error is that of its result, because the same B stands in the sum, in
-// the gradient and in the loss.  Sums are float32.  A NaN or +inf logit makes its row NaN
-// through the sum; a row of -inf alone has q = 0.  Repeated
-// ids: every entry holds the whole P of its id, so that all of them write the same value.
+// Exponentials are 2^(z c - B) with c = log2(e) / tau and one B for the whole row: a fused
+// operation, whose error is that of its result, because the same rounded B stands in the sum,
+// in the gradient and in the loss.  B needs no maximum over the row: it is r c for the largest
+// student logit r at the teacher's ids, so the sum is at least 1, and only a row with a logit
+// about 40 tau above r (or far from zero, or without a finite r) overflows; such a row is
+// computed again from its maximum.  Sums are float32.  A NaN or +inf logit makes its row NaN
+// through the sum; a row of -inf alone has q = 0.  Repeated ids: every entry holds the whole P
+// of its id, so that all of them write the same value.
 #include "train_common.cuh"
 
 #include <cooperative_groups.h>
@@ -29,17 +32,18 @@ struct DistillArgs {
 };
 
 // The teacher's side of a row in shared memory: k ids (-1: not valid), teacher probabilities,
-// their sums over equal ids and student logits at the ids, then the sum of p log p and whether
-// a valid entry exists.
+// their sums over equal ids and student logits at the ids, then the sum of p log p, whether a
+// valid entry exists, and the largest of the logits.
 struct TopList {
     int* id;
     float *p, *same, *z, *entropy;
     int* any;
+    float* reference;
     __device__ __forceinline__ TopList(unsigned char* at, int k)
         : id(reinterpret_cast<int*>(at)), p(reinterpret_cast<float*>(at) + k), same(p + k), z(same + k), entropy(z + k),
-          any(reinterpret_cast<int*>(entropy + 1)) {}
+          any(reinterpret_cast<int*>(entropy + 1)), reference(entropy + 2) {}
 };
-__host__ __device__ constexpr int top_bytes(int k) { return (16 * k + 8 + 15) / 16 * 16; }
+__host__ __device__ constexpr int top_bytes(int k) { return (16 * k + 12 + 15) / 16 * 16; }
 
 // One warp's set of bits that finds ids that may occur twice, and the list of those.
 constexpr int kSeenBits = 16384;
@@ -56,15 +60,13 @@ __device__ __forceinline__ float exp2_fast(float x) {  // relative error 2^-22
     return y;
 }
 
-// Fills the list with one warp; the block sees it after its next barrier.  Four entries a lane
-// have their loads in flight together.
+// Fills the list with one warp; the block sees it after its next barrier.  First the loads, four
+// entries a lane in flight together, and the reference; returns the largest teacher logit.
 template <typename T>
-__device__ __forceinline__ void load_teacher(const DistillArgs& a, int64_t t, const T* row, const TopList& top, Seen& seen) {
+__device__ __forceinline__ float load_teacher(const DistillArgs& a, int64_t t, const T* row, const TopList& top) {
     const int lane = threadIdx.x & 31;
     const int64_t at = t * a.k;
-    float m = -INFINITY;
-    for (int i = lane; i < kSeenBits / 32; i += 32) seen.bits[i] = 0;
-    if (lane == 0) seen.count = 0;
+    float m = -INFINITY, r = -INFINITY;
     for (int k0 = 0; k0 < a.k; k0 += 128) {
         int64_t id[4];
         float u[4], z[4];
@@ -86,11 +88,23 @@ __device__ __forceinline__ void load_teacher(const DistillArgs& a, int64_t t, co
             top.id[k] = (int)id[j];
             top.p[k] = u[j];
             top.z[k] = z[j];
-            if (id[j] >= 0) m = fmaxf(m, u[j]);
+            if (id[j] >= 0) {
+                m = fmaxf(m, u[j]);
+                r = fmaxf(r, z[j]);
+            }
         }
     }
+    r = warp_max(r);
+    if (lane == 0) *top.reference = r;
     __syncwarp();
-    m = warp_max(m);
+    return warp_max(m);
+}
+// Then the probabilities.
+__device__ __forceinline__ void finish_teacher(const DistillArgs& a, const TopList& top, float m, Seen& seen) {
+    const int lane = threadIdx.x & 31;
+    for (int i = lane; i < kSeenBits / 32; i += 32) seen.bits[i] = 0;
+    if (lane == 0) seen.count = 0;
+    __syncwarp();
     const float inv_tau = 1.0f / a.tau;
     float s = 0.0f;
     bool valid_here = false;
@@ -134,27 +148,24 @@ __device__ __forceinline__ void load_teacher(const DistillArgs& a, int64_t t, co
     __syncwarp();
 }
 
-// Joins (maximum, sum of 2^(z c - B)) over the lanes of a warp, or of its first WIDTH lanes.
-template <int WIDTH = 32>
+// Joins (maximum, sum relative to it) over the first WIDTH lanes of a warp; all lanes get it.
+template <int WIDTH>
 __device__ __forceinline__ void join_warp(float& m, float& s, float c2) {
     float top = m;
 #pragma unroll
     for (int o = WIDTH / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     // a part without a finite maximum holds 0 or NaN and keeps it
-    s *= m == top ? 1.0f : exp2_fast(__fmul_rn(m, c2) - __fmul_rn(top, c2));  // the rounded B of both
+    s *= m == top ? 1.0f : exp2_fast((m - top) * c2);
 #pragma unroll
     for (int o = WIDTH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    m = top;
+    m = __shfl_sync(0xffffffffu, top, 0);
+    s = __shfl_sync(0xffffffffu, s, 0);
 }
 
-// -B of a maximum; 0 where there is none.  B's rounding shifts all exponents of a row by up to
-// 2^-24 |B|, which cancels as long as it is small: a row whose |B| is above kFar is formed
-// again from z - max, and a part of another row whose |B| is above twice that adds nothing.
+// B's rounding shifts all exponents of a row by up to 2^-24 |B|, which cancels as long as it
+// is small.
 constexpr float kFar = 16777216.0f;
-__device__ __forceinline__ float minus_b(float m, float c2) {
-    const float b = __fmul_rn(m, c2);
-    return fabsf(b) > 2.0f * kFar ? 0.0f : -b;
-}
+constexpr float kLargeSum = 1e18f;  // its reciprocal, times a small weight, stays a normal number
 
 // Loss of the row from its base = -B and sum by one warp, and the gradients of the entries' ids in
 // [v0, v1) by `threads` threads.
@@ -180,43 +191,14 @@ __device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopLis
 // A row is cut into the 16-byte words of its memory and lies in the shared memory of a block,
 // or of a cluster of blocks: read once, written once.  Each thread copies and reads the same
 // words.  The blocks stay for many rows: a word of the next row takes the place of a word
-// whose gradient is formed, and one further warp prepares the next teacher list, whose chain
-// of dependent loads is as long as a row takes.  Each thread takes the maximum of its logits
-// and the sum relative to it, which are joined over warps, block and cluster in one exchange.
+// whose gradient is formed, and one further warp prepares the teacher lists two rows ahead,
+// whose chain of dependent loads is about as long as a row takes.
 constexpr int kDistillThreads = 256;          // the teacher's warp among them
 constexpr int kDistillShare = 64 * 1024;      // bytes of a row in a block, three blocks an SM
 constexpr int kDistillLongShare = 128 * 1024; // the same for the longest rows, one block an SM
 
 template <typename T>
 constexpr int kWordLogits = 16 / (int)sizeof(T);
-
-// Running maximum of the logits of a thread's words; NaN is left out.
-template <typename T>
-struct WordMax {
-    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
-    T2 m;
-    __device__ __forceinline__ WordMax() {
-        const uint32_t none = std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;  // -inf
-        m = *reinterpret_cast<const T2*>(&none);
-    }
-    __device__ __forceinline__ void add(const uint4& w) {
-        auto two = [](const uint32_t& v) { return *reinterpret_cast<const T2*>(&v); };
-        m = __hmax2(__hmax2(m, __hmax2(two(w.x), two(w.y))), __hmax2(two(w.z), two(w.w)));
-    }
-    __device__ __forceinline__ float get() const {
-        const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t*>(&m));
-        return fmaxf(f.x, f.y);
-    }
-};
-template <>
-struct WordMax<float> {
-    float m = -INFINITY;
-    __device__ __forceinline__ void add(const uint4& w) {
-        m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(w.x), __uint_as_float(w.y))),
-                  fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
-    }
-    __device__ __forceinline__ float get() const { return m; }
-};
 
 // f(i, pair): the logits of a word two at a time.
 template <typename T, typename F>
@@ -270,14 +252,14 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
     distill_kernel(DistillArgs a, int64_t rows, const T* z, float* __restrict__ loss, T* grad, int log_cluster,
                    unsigned long long* tickets) {
     constexpr int N = kWordLogits<T>, threads = BLOCK - 32, warps = threads / 32;
-    const int cluster = 1 << log_cluster;
+    namespace cg = cooperative_groups;
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ float2 warp_part[2][32], block_part[2];
+    __shared__ float2 warp_part[2][warps], block_part[2];
     __shared__ Seen seen;
     __shared__ int64_t ticket[2];
-    uint4* stage = reinterpret_cast<uint4*>(smem + 2 * top_bytes(a.k));
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int vocab = (int)a.vocab;
+    uint4* stage = reinterpret_cast<uint4*>(smem + 3 * top_bytes(a.k));
+    auto list = [&](int i) { return TopList(smem + i * top_bytes(a.k), a.k); };
+    const int cluster = 1 << log_cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, vocab = (int)a.vocab;
     const bool is_teacher = warp == warps;
     const int rank = (int)blockIdx.x & (cluster - 1);
     const int64_t workers = gridDim.x >> log_cluster;
@@ -286,17 +268,18 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
     // The first two rows of a block (cluster) are its own, the others come by ticket, since masked
     // rows take no time.  The ticket of a row is taken two rows ahead.
     int64_t t = blockIdx.x >> log_cluster, t1 = t + workers, pending = rows;
-    float w = weight(t);
-    const T* row = z + t * a.stride;
     auto take = [&](bool more) {
         if (is_teacher && lane == 0 && rank == 0) pending = more ? 2 * workers + (int64_t)atomicAdd(tickets, 1ull) : rows;
     };
     take(t1 < rows);
+    float w = weight(t), w1 = weight(t1);
+    const T* row = z + t * a.stride;
     RowShare r = row_share<T>(row, vocab, rank, log_cluster, tid);
     float edge_x = -INFINITY;
+    float teacher_top = -INFINITY;
     if (w != 0.0f) {
         if (is_teacher) {
-            load_teacher<T>(a, t, row, TopList(smem, a.k), seen);
+            teacher_top = load_teacher<T>(a, t, row, list(0));
         } else {
             const T* body = row + r.head + r.first * N;
             each_word<threads, 4>(tid, r.count, [&](int i) { copy_vec<T, N>(reinterpret_cast<T*>(stage + i), body + i * N); });
@@ -304,121 +287,128 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
         }
     }
     copy_commit();
-    for (int b = 0; t < rows; b ^= 1) {
+    __syncthreads();  // the reference of the first row
+    if (is_teacher) {
+        if (w != 0.0f) finish_teacher(a, list(0), teacher_top, seen);
+        if (w1 != 0.0f) finish_teacher(a, list(1), load_teacher<T>(a, t1, z + t1 * a.stride, list(1)), seen);
+    }
+    for (int b = 0, l = 0; t < rows; b ^= 1, l = l == 2 ? 0 : l + 1) {
         const bool live = w != 0.0f;
-        const float w_next = weight(t1);
+        const TopList top = list(l);
         const T* row_next = z + t1 * a.stride;
+        const T* body_now = row + r.head + r.first * N;
         if (is_teacher && lane == 0) ticket[b] = pending;
-        float m = -INFINITY, s = 0.0f;
-        // sum of the exponentials of the thread's logits
-        auto sum_words = [&](float base) {
-            float2 sum = make_float2(exp2_fast(fmaf(edge_x, c2, base)), 0.0f);
-            each_word<threads, 2>(tid, r.count, [&](int i) {
-                word_pairs<T>(stage[i], [&](int, float2 f) {
-                    f = __ffma2_rn(f, make_float2(c2, c2), make_float2(base, base));
-                    sum = __fadd2_rn(sum, make_float2(exp2_fast(f.x), exp2_fast(f.y)));
-                });
-            });
-            return sum.x + sum.y;
-        };
-        auto join_row = [&] {
-            if (!is_teacher) {
-                join_warp(m, s, c2);
-                if (lane == 0) warp_part[b][warp] = make_float2(m, s);
-            }
-            __syncthreads();
-            auto spread = [&](float2 part) {
-                m = part.x;
-                s = part.y;
-                join_warp<8>(m, s, c2);
-                m = __shfl_sync(0xffffffffu, m, 0);
-                s = __shfl_sync(0xffffffffu, s, 0);
-            };
-            spread(lane < warps ? warp_part[b][lane] : make_float2(-INFINITY, 0.0f));
-            if (cluster > 1) {
-                namespace cg = cooperative_groups;
-                cg::cluster_group group = cg::this_cluster();
-                if (tid == 0) block_part[b] = make_float2(m, s);
-                group.sync();
-                spread(lane < cluster ? *group.map_shared_rank(&block_part[b], lane) : make_float2(-INFINITY, 0.0f));
-            }
-        };
+        const float reference = live ? *top.reference : 0.0f;
+        float base = -__fmul_rn(reference, c2), s = 0.0f;
         if (!is_teacher) {
             copy_wait<0>();
             if (live) {
-                WordMax<T> top_word;
-                each_word<threads, 4>(tid, r.count, [&](int i) { top_word.add(stage[i]); });
-                m = fmaxf(top_word.get(), edge_x);
-                s = sum_words(minus_b(m, c2));
+                float2 sum = make_float2(exp2_fast(fmaf(edge_x, c2, base)), 0.0f);
+                each_word<threads, 2>(tid, r.count, [&](int i) {
+                    word_pairs<T>(stage[i], [&](int, float2 f) {
+                        f = __ffma2_rn(f, make_float2(c2, c2), make_float2(base, base));
+                        sum = __fadd2_rn(sum, make_float2(exp2_fast(f.x), exp2_fast(f.y)));
+                    });
+                });
+                s = warp_sum(sum.x + sum.y);
             }
+            if (lane == 0) warp_part[b][warp] = make_float2(0.0f, s);
         }
         // the next row
         const RowShare n = row_share<T>(row_next, vocab, rank, log_cluster, tid);
-        const int fetched = w_next != 0.0f && !is_teacher ? n.count : 0;
+        const int fetched = w1 != 0.0f && !is_teacher ? n.count : 0;
         const T* body_next = row_next + n.head + n.first * N;
         auto fetch = [&](int i) { copy_vec<T, N>(reinterpret_cast<T*>(stage + i), body_next + i * N); };
         float edge_now = edge_x;
-        if (!is_teacher) edge_x = w_next != 0.0f && n.edge >= 0 ? to_float(row_next[n.edge]) : -INFINITY;
+        if (!is_teacher) edge_x = w1 != 0.0f && n.edge >= 0 ? to_float(row_next[n.edge]) : -INFINITY;
         if (grad == nullptr) each_word<threads, 4>(tid, fetched, fetch);
-        join_row();
-        const int64_t t2 =
-            cluster > 1 ? *cooperative_groups::this_cluster().map_shared_rank(&ticket[b], 0) : ticket[b];
-        const TopList top(smem + b * top_bytes(a.k), a.k);
-        const bool any = live && *top.any;
-        const T* body_now = row + r.head + r.first * N;
-        const float far = fabsf(m) != INFINITY && fabsf(m * c2) > kFar ? m : 0.0f;
-        if (far != 0.0f) {
-            // every logit is about the type's lowest value, say: the exponents of z - max
-            m = 0.0f;
+        __syncthreads();
+        s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < warps; ++i) s += warp_part[b][i].y;
+        int64_t t2 = ticket[b];
+        if (cluster > 1) {
+            cg::cluster_group group = cg::this_cluster();
+            if (tid == 0) block_part[b] = make_float2(0.0f, s);
+            group.sync();
             s = 0.0f;
-            edge_now -= far;
-            if (is_teacher) {
-                for (int k = lane; k < a.k; k += 32) top.z[k] -= far;
-            } else {
-                s = exp2_fast(edge_now * c2);
-                for (int i = tid; i < r.count * N; i += threads) s += exp2_fast((to_float(body_now[i]) - far) * c2);
-            }
-            __syncthreads();  // the parts of the first join have been read
-            if (cluster > 1) cooperative_groups::this_cluster().sync();
-            join_row();
+            for (int i = 0; i < cluster; ++i) s += group.map_shared_rank(&block_part[b], i)->y;
+            t2 = *group.map_shared_rank(&ticket[b], 0);
         }
-        if (m == INFINITY) s = NAN;
-        const float base = minus_b(m, c2);
+        const bool any = live && *top.any;
+        const float w2 = weight(t2);
+        float far = 0.0f;
+        if (any && !(s < kLargeSum && fabsf(base) <= kFar)) {
+            // no usable reference: from the row's maximum, over the logits in memory
+            float m = -INFINITY;
+            s = 0.0f;
+            if (!is_teacher) {
+                m = edge_now;
+                for (int i = tid; i < r.count * N; i += threads) m = fmaxf(m, to_float(body_now[i]));
+                const float from = m == -INFINITY ? 0.0f : m;
+                s = exp2_fast((edge_now - from) * c2);
+                for (int i = tid; i < r.count * N; i += threads) s += exp2_fast((to_float(body_now[i]) - from) * c2);
+                join_warp<32>(m, s, c2);
+            }
+            __syncthreads();  // the parts of the first exchange have been read
+            if (!is_teacher && lane == 0) warp_part[b][warp] = make_float2(m, s);
+            __syncthreads();
+            m = lane < warps ? warp_part[b][lane].x : -INFINITY;
+            s = lane < warps ? warp_part[b][lane].y : 0.0f;
+            join_warp<8>(m, s, c2);
+            if (cluster > 1) {
+                cg::cluster_group group = cg::this_cluster();
+                group.sync();
+                if (tid == 0) block_part[b] = make_float2(m, s);
+                group.sync();
+                const float2 part = lane < cluster ? *group.map_shared_rank(&block_part[b], lane) : make_float2(-INFINITY, 0.0f);
+                m = part.x;
+                s = part.y;
+                join_warp<8>(m, s, c2);
+            }
+            if (m == INFINITY) s = NAN;
+            far = m == -INFINITY ? 0.0f : m;
+            base = 0.0f;
+            edge_now -= far;
+            if (is_teacher)
+                for (int k = lane; k < a.k; k += 32) top.z[k] -= far;
+            __syncthreads();
+        }
         if (is_teacher) {
             if (rank == 0) {
-                const float l = any ? row_loss(a, top, w, c2, base, s) : 0.0f;
-                if (lane == 0) loss[t] = l;
+                const float v = any ? row_loss(a, top, w, c2, base, s) : 0.0f;
+                if (lane == 0) loss[t] = v;
             }
             take(t2 < rows);
-            if (w_next != 0.0f)
-                load_teacher<T>(a, t1, row_next, TopList(smem + (b ^ 1) * top_bytes(a.k), a.k), seen);
+            if (w2 != 0.0f) {
+                const TopList ahead = list(l == 0 ? 2 : l - 1);
+                finish_teacher(a, ahead, load_teacher<T>(a, t2, z + t2 * a.stride, ahead), seen);
+            }
         } else {
             if (grad != nullptr) {
                 T* out = grad + t * a.vocab;
                 T* body = out + r.head + r.first * N;
+                const bool aligned = (reinterpret_cast<uintptr_t>(body) & 15) == 0;
                 const float c = w * a.tau, inv_s = s == 0.0f ? 0.0f : 1.0f / s, ci = c * inv_s;
-                auto gradients = [&](int i) {
-                    uint32_t o[4];
-                    word_pairs<T>(stage[i], [&](int j, float2 f) {
-                        f = __ffma2_rn(f, make_float2(c2, c2), make_float2(base, base));
-                        f = __fmul2_rn(make_float2(exp2_fast(f.x), exp2_fast(f.y)), make_float2(ci, ci));
-                        if constexpr (sizeof(T) == 4) {
-                            o[2 * j] = __float_as_uint(f.x);
-                            o[2 * j + 1] = __float_as_uint(f.y);
-                        } else {
-                            o[j] = pack2<T>(f.x, f.y);
-                        }
-                    });
-                    return make_uint4(o[0], o[1], o[2], o[3]);
-                };
-                if (any && far == 0.0f && (reinterpret_cast<uintptr_t>(body) & 15) == 0) {
+                if (any && far == 0.0f && aligned) {
                     each_word<threads, 2>(tid, r.count, [&](int i) {
-                        reinterpret_cast<uint4*>(body)[i] = gradients(i);
+                        uint32_t o[4];
+                        word_pairs<T>(stage[i], [&](int j, float2 f) {
+                            f = __ffma2_rn(f, make_float2(c2, c2), make_float2(base, base));
+                            f = __fmul2_rn(make_float2(exp2_fast(f.x), exp2_fast(f.y)), make_float2(ci, ci));
+                            if constexpr (sizeof(T) == 4) {
+                                o[2 * j] = __float_as_uint(f.x);
+                                o[2 * j + 1] = __float_as_uint(f.y);
+                            } else {
+                                o[j] = pack2<T>(f.x, f.y);
+                            }
+                        });
+                        reinterpret_cast<uint4*>(body)[i] = make_uint4(o[0], o[1], o[2], o[3]);
                         if (i < fetched) fetch(i);
                     });
                     // the next row may begin at another alignment and have one word more
                     if (r.count < fetched && (fetched - 1) % threads == tid) fetch(fetched - 1);
-                } else if (!any && (reinterpret_cast<uintptr_t>(body) & 15) == 0) {
+                } else if (!any && aligned) {
                     each_word<threads, 4>(tid, r.count, [&](int i) {
                         reinterpret_cast<uint4*>(body)[i] = make_uint4(0, 0, 0, 0);
                     });
@@ -443,14 +433,15 @@ __global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
                 }
             }
             copy_commit();
-            r = n;
         }
+        r = n;
         t = t1;
         t1 = t2;
         row = row_next;
-        w = w_next;
+        w = w1;
+        w1 = w2;
     }
-    if (cluster > 1) cooperative_groups::this_cluster().sync();  // a peer may still read this block's part
+    if (cluster > 1) cg::this_cluster().sync();  // a peer may still read this block's part
 }
 
 // ------------------------------------------------------------- longer rows ---
@@ -467,7 +458,7 @@ __global__ void __launch_bounds__(1024) distill_long_kernel(DistillArgs a, const
     const T* row = z + t * a.stride;
     T* out = grad != nullptr ? grad + t * a.vocab : nullptr;
     const float w = a.weight != nullptr ? a.weight[t] : 1.0f;
-    if (w != 0.0f && threadIdx.x < 32) load_teacher<T>(a, t, row, top, seen);
+    if (w != 0.0f && threadIdx.x < 32) finish_teacher(a, top, load_teacher<T>(a, t, row, top), seen);
     __syncthreads();
     if (w == 0.0f || !*top.any) {
         if (out != nullptr)
@@ -569,13 +560,13 @@ int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, 
             CRESSO_LAUNCHED("distill_long_kernel");
             return (int)CRESSO_OK;
         }
-        const int smem = (int)p.share * 16 + 2 * top_bytes(a.k);
+        const int smem = (int)p.share * 16 + 3 * top_bytes(a.k);
         const auto kernel = p.threads == kDistillThreads       ? distill_kernel<T, kDistillThreads>
                             : p.threads == kDistillThreads / 2 ? distill_kernel<T, kDistillThreads / 2>
                                                                : distill_kernel<T, kDistillThreads / 4>;
         if (smem > 48 * 1024)
             CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             kDistillLongShare + 2 * top_bytes(CRESSO_TRAIN_MAX_TOP)));
+                                             kDistillLongShare + 3 * top_bytes(CRESSO_TRAIN_MAX_TOP)));
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)p.cluster);
         cfg.blockDim = dim3((unsigned)p.threads);
