@@ -71,8 +71,7 @@ EXPORTS = (
 # entry points of include/cresso_b200_train.h
 TRAIN_EXPORTS = (
     "cresso_embedding_gather", "cresso_embedding_grad_scratch_bytes", "cresso_embedding_grad", "cresso_block_norm",
-    "cresso_block_norm_grad_scratch_bytes", "cresso_block_norm_grad", "cresso_distill_scratch_bytes",
-    "cresso_distill",
+    "cresso_block_norm_grad_scratch_bytes", "cresso_block_norm_grad", "cresso_distill",
 )
 TRAIN_MAX_TOP = 1024  # CRESSO_TRAIN_MAX_TOP
 
@@ -126,9 +125,8 @@ def _declare(lib) -> None:
         "cresso_block_norm": (ctypes.c_int, [_p] * 5 + [_i64] * 7 + [_dbl, _dbl, _p, _p, _p]),
         "cresso_block_norm_grad_scratch_bytes": (ctypes.c_int, [_i64, _i64, _i64, _pi64]),
         "cresso_block_norm_grad": (ctypes.c_int, [_p] * 7 + [_i64] * 7 + [_dbl, _dbl] + [_p] * 6 + [_i64, _p]),
-        "cresso_distill_scratch_bytes": (ctypes.c_int, [_i64, _i64, _pi64]),
-        "cresso_distill": (ctypes.c_int, [_p, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _dbl, _p, _p, _p,
-                                          _i64, _p]),
+        "cresso_distill": (ctypes.c_int, [_p, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _dbl, _p, _p,
+                                          _p]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

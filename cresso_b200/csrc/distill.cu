@@ -186,16 +186,16 @@ __device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopLis
     }
 }
 
-// ----------------------------------------------------- rows in shared memory ---
+// ------------------------------------------------------------------ the rows ---
 //
-// A row is cut into the 16-byte words of its memory and lies in the shared memory of a block,
-// or of a cluster of blocks: read once, written once.  Each thread copies and reads the same
-// words.  The blocks stay for many rows: a word of the next row takes the place of a word
-// whose gradient is formed, and one further warp prepares the teacher lists two rows ahead,
-// whose chain of dependent loads is about as long as a row takes.
-constexpr int kDistillThreads = 256;          // the teacher's warp among them
-constexpr int kDistillShare = 64 * 1024;      // bytes of a row in a block, three blocks an SM
-constexpr int kDistillLongShare = 128 * 1024; // the same for the longest rows, one block an SM
+// A row belongs to a block, or to a cluster of blocks that hold a part of it each.  It is cut
+// into the 16-byte words of its memory and read twice: once for the sum, from DRAM, and once for
+// the gradient, while it is still in L2 (the rows at work at a time are a third of it).  No
+// storage on the SM means many blocks an SM, in different phases: their loads overlap the others'
+// exponentials, barriers and teacher lists.  One further warp prepares the teacher's list.
+constexpr int kDistillThreads = 256;         // without the teacher's warp
+constexpr int kDistillShare = 64 * 1024;     // bytes of a row that a block is given at least
+constexpr int kDistillCluster = 8;
 
 template <typename T>
 constexpr int kWordLogits = 16 / (int)sizeof(T);
@@ -235,277 +235,153 @@ __device__ __forceinline__ RowShare row_share(const T* row, int vocab, int rank,
     return r;
 }
 
-// f(i) for the words i = tid, tid + THREADS, ... below count, U at a time.
-template <int THREADS, int U, typename F>
-__device__ __forceinline__ void each_word(int tid, int count, F f) {
+// f(i, get(i)) for the words i = tid, tid + THREADS, ... below count; U of them are fetched
+// before the first is used.
+template <int THREADS, int U, typename G, typename F>
+__device__ __forceinline__ void each_word(int tid, int count, G get, F f) {
     int i = tid;
-    for (; i + (U - 1) * THREADS < count; i += U * THREADS)
+    for (; i + (U - 1) * THREADS < count; i += U * THREADS) {
+        uint4 x[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) f(i + u * THREADS);
+        for (int u = 0; u < U; ++u) x[u] = get(i + u * THREADS);
 #pragma unroll
-    for (int u = 0; u < U - 1; ++u)
-        if (i + u * THREADS < count) f(i + u * THREADS);
+        for (int u = 0; u < U; ++u) f(i + u * THREADS, x[u]);
+    }
+    for (; i < count; i += THREADS) f(i, get(i));
 }
 
-template <typename T, int BLOCK>
-__global__ void __launch_bounds__(BLOCK, 3 * kDistillThreads / BLOCK)
-    distill_kernel(DistillArgs a, int64_t rows, const T* z, float* __restrict__ loss, T* grad, int log_cluster,
-                   unsigned long long* tickets) {
-    constexpr int N = kWordLogits<T>, threads = BLOCK - 32, warps = threads / 32;
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS + 32)
+    distill_kernel(DistillArgs a, const T* z, float* __restrict__ loss, T* grad, int log_cluster) {
+    constexpr int N = kWordLogits<T>, warps = THREADS / 32;
     namespace cg = cooperative_groups;
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ float2 warp_part[2][warps], block_part[2];
+    __shared__ float2 warp_part[warps], block_part;
     __shared__ Seen seen;
-    __shared__ int64_t ticket[2];
-    uint4* stage = reinterpret_cast<uint4*>(smem + 3 * top_bytes(a.k));
-    auto list = [&](int i) { return TopList(smem + i * top_bytes(a.k), a.k); };
+    const TopList top(smem, a.k);
     const int cluster = 1 << log_cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, vocab = (int)a.vocab;
     const bool is_teacher = warp == warps;
     const int rank = (int)blockIdx.x & (cluster - 1);
-    const int64_t workers = gridDim.x >> log_cluster;
-    const float c2 = kLog2E / a.tau;
-    auto weight = [&](int64_t t) { return t >= rows ? 0.0f : a.weight != nullptr ? a.weight[t] : 1.0f; };
-    // The first two rows of a block (cluster) are its own, the others come by ticket, since masked
-    // rows take no time.  The ticket of a row is taken two rows ahead.
-    int64_t t = blockIdx.x >> log_cluster, t1 = t + workers, pending = rows;
-    auto take = [&](bool more) {
-        if (is_teacher && lane == 0 && rank == 0) pending = more ? 2 * workers + (int64_t)atomicAdd(tickets, 1ull) : rows;
-    };
-    take(t1 < rows);
-    float w = weight(t), w1 = weight(t1);
+    const int64_t t = blockIdx.x >> log_cluster;
     const T* row = z + t * a.stride;
-    RowShare r = row_share<T>(row, vocab, rank, log_cluster, tid);
-    float edge_x = -INFINITY;
-    float teacher_top = -INFINITY;
+    const RowShare r = row_share<T>(row, vocab, rank, log_cluster, tid);
+    const uint4* words = reinterpret_cast<const uint4*>(row + r.head + r.first * N);
+    T* out = grad != nullptr ? grad + t * a.vocab : nullptr;
+    T* body = out + r.head + r.first * N;
+    const bool aligned = (reinterpret_cast<uintptr_t>(body) & 15) == 0;
+    const float w = a.weight != nullptr ? a.weight[t] : 1.0f;
+    const float c2 = kLog2E / a.tau;
+    bool any = false;
+    float s = 0.0f, base = 0.0f, far = 0.0f, edge = -INFINITY;
     if (w != 0.0f) {
+        float teacher_top = 0.0f;
+        if (is_teacher)
+            teacher_top = load_teacher<T>(a, t, row, top);
+        else if (r.edge >= 0)
+            edge = to_float(row[r.edge]);
+        __syncthreads();  // the reference
+        base = -__fmul_rn(*top.reference, c2);
         if (is_teacher) {
-            teacher_top = load_teacher<T>(a, t, row, list(0));
+            finish_teacher(a, top, teacher_top, seen);
         } else {
-            const T* body = row + r.head + r.first * N;
-            each_word<threads, 4>(tid, r.count, [&](int i) { copy_vec<T, N>(reinterpret_cast<T*>(stage + i), body + i * N); });
-            if (r.edge >= 0) edge_x = to_float(row[r.edge]);
-        }
-    }
-    copy_commit();
-    __syncthreads();  // the reference of the first row
-    if (is_teacher) {
-        if (w != 0.0f) finish_teacher(a, list(0), teacher_top, seen);
-        if (w1 != 0.0f) finish_teacher(a, list(1), load_teacher<T>(a, t1, z + t1 * a.stride, list(1)), seen);
-    }
-    for (int b = 0, l = 0; t < rows; b ^= 1, l = l == 2 ? 0 : l + 1) {
-        const bool live = w != 0.0f;
-        const TopList top = list(l);
-        const T* row_next = z + t1 * a.stride;
-        const T* body_now = row + r.head + r.first * N;
-        if (is_teacher && lane == 0) ticket[b] = pending;
-        const float reference = live ? *top.reference : 0.0f;
-        float base = -__fmul_rn(reference, c2), s = 0.0f;
-        if (!is_teacher) {
-            copy_wait<0>();
-            if (live) {
-                float2 sum = make_float2(exp2_fast(fmaf(edge_x, c2, base)), 0.0f);
-                each_word<threads, 2>(tid, r.count, [&](int i) {
-                    word_pairs<T>(stage[i], [&](int, float2 f) {
-                        f = __ffma2_rn(f, make_float2(c2, c2), make_float2(base, base));
-                        sum = __fadd2_rn(sum, make_float2(exp2_fast(f.x), exp2_fast(f.y)));
-                    });
+            float2 sum = make_float2(exp2_fast(fmaf(edge, c2, base)), 0.0f);
+            each_word<THREADS, 4>(tid, r.count, [&](int i) { return words[i]; }, [&](int, const uint4& x) {
+                word_pairs<T>(x, [&](int, float2 f) {
+                    f = __ffma2_rn(f, make_float2(c2, c2), make_float2(base, base));
+                    sum = __fadd2_rn(sum, make_float2(exp2_fast(f.x), exp2_fast(f.y)));
                 });
-                s = warp_sum(sum.x + sum.y);
-            }
-            if (lane == 0) warp_part[b][warp] = make_float2(0.0f, s);
+            });
+            s = warp_sum(sum.x + sum.y);
+            if (lane == 0) warp_part[warp] = make_float2(0.0f, s);
         }
-        // the next row
-        const RowShare n = row_share<T>(row_next, vocab, rank, log_cluster, tid);
-        const int fetched = w1 != 0.0f && !is_teacher ? n.count : 0;
-        const T* body_next = row_next + n.head + n.first * N;
-        auto fetch = [&](int i) { copy_vec<T, N>(reinterpret_cast<T*>(stage + i), body_next + i * N); };
-        float edge_now = edge_x;
-        if (!is_teacher) edge_x = w1 != 0.0f && n.edge >= 0 ? to_float(row_next[n.edge]) : -INFINITY;
-        if (grad == nullptr) each_word<threads, 4>(tid, fetched, fetch);
         __syncthreads();
         s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < warps; ++i) s += warp_part[b][i].y;
-        int64_t t2 = ticket[b];
+        for (int i = 0; i < warps; ++i) s += warp_part[i].y;
         if (cluster > 1) {
             cg::cluster_group group = cg::this_cluster();
-            if (tid == 0) block_part[b] = make_float2(0.0f, s);
+            if (tid == 0) block_part = make_float2(0.0f, s);
             group.sync();
             s = 0.0f;
-            for (int i = 0; i < cluster; ++i) s += group.map_shared_rank(&block_part[b], i)->y;
-            t2 = *group.map_shared_rank(&ticket[b], 0);
+            for (int i = 0; i < cluster; ++i) s += group.map_shared_rank(&block_part, i)->y;
         }
-        const bool any = live && *top.any;
-        const float w2 = weight(t2);
-        float far = 0.0f;
+        any = *top.any;
         if (any && !(s < kLargeSum && fabsf(base) <= kFar)) {
-            // no usable reference: from the row's maximum, over the logits in memory
+            // no usable reference: from the row's maximum
+            const T* part = reinterpret_cast<const T*>(words);
             float m = -INFINITY;
             s = 0.0f;
             if (!is_teacher) {
-                m = edge_now;
-                for (int i = tid; i < r.count * N; i += threads) m = fmaxf(m, to_float(body_now[i]));
+                m = edge;
+                for (int i = tid; i < r.count * N; i += THREADS) m = fmaxf(m, to_float(part[i]));
                 const float from = m == -INFINITY ? 0.0f : m;
-                s = exp2_fast((edge_now - from) * c2);
-                for (int i = tid; i < r.count * N; i += threads) s += exp2_fast((to_float(body_now[i]) - from) * c2);
+                s = exp2_fast((edge - from) * c2);
+                for (int i = tid; i < r.count * N; i += THREADS) s += exp2_fast((to_float(part[i]) - from) * c2);
                 join_warp<32>(m, s, c2);
             }
             __syncthreads();  // the parts of the first exchange have been read
-            if (!is_teacher && lane == 0) warp_part[b][warp] = make_float2(m, s);
+            if (!is_teacher && lane == 0) warp_part[warp] = make_float2(m, s);
             __syncthreads();
-            m = lane < warps ? warp_part[b][lane].x : -INFINITY;
-            s = lane < warps ? warp_part[b][lane].y : 0.0f;
+            m = lane < warps ? warp_part[lane].x : -INFINITY;
+            s = lane < warps ? warp_part[lane].y : 0.0f;
             join_warp<8>(m, s, c2);
             if (cluster > 1) {
                 cg::cluster_group group = cg::this_cluster();
                 group.sync();
-                if (tid == 0) block_part[b] = make_float2(m, s);
+                if (tid == 0) block_part = make_float2(m, s);
                 group.sync();
-                const float2 part = lane < cluster ? *group.map_shared_rank(&block_part[b], lane) : make_float2(-INFINITY, 0.0f);
-                m = part.x;
-                s = part.y;
+                const float2 p = lane < cluster ? *group.map_shared_rank(&block_part, lane) : make_float2(-INFINITY, 0.0f);
+                m = p.x;
+                s = p.y;
                 join_warp<8>(m, s, c2);
             }
             if (m == INFINITY) s = NAN;
             far = m == -INFINITY ? 0.0f : m;
             base = 0.0f;
-            edge_now -= far;
+            edge -= far;
             if (is_teacher)
                 for (int k = lane; k < a.k; k += 32) top.z[k] -= far;
             __syncthreads();
         }
-        if (is_teacher) {
-            if (rank == 0) {
-                const float v = any ? row_loss(a, top, w, c2, base, s) : 0.0f;
-                if (lane == 0) loss[t] = v;
-            }
-            take(t2 < rows);
-            if (w2 != 0.0f) {
-                const TopList ahead = list(l == 0 ? 2 : l - 1);
-                finish_teacher(a, ahead, load_teacher<T>(a, t2, z + t2 * a.stride, ahead), seen);
-            }
-        } else {
-            if (grad != nullptr) {
-                T* out = grad + t * a.vocab;
-                T* body = out + r.head + r.first * N;
-                const bool aligned = (reinterpret_cast<uintptr_t>(body) & 15) == 0;
-                const float c = w * a.tau, inv_s = s == 0.0f ? 0.0f : 1.0f / s, ci = c * inv_s;
-                if (any && far == 0.0f && aligned) {
-                    each_word<threads, 2>(tid, r.count, [&](int i) {
-                        uint32_t o[4];
-                        word_pairs<T>(stage[i], [&](int j, float2 f) {
-                            f = __ffma2_rn(f, make_float2(c2, c2), make_float2(base, base));
-                            f = __fmul2_rn(make_float2(exp2_fast(f.x), exp2_fast(f.y)), make_float2(ci, ci));
-                            if constexpr (sizeof(T) == 4) {
-                                o[2 * j] = __float_as_uint(f.x);
-                                o[2 * j + 1] = __float_as_uint(f.y);
-                            } else {
-                                o[j] = pack2<T>(f.x, f.y);
-                            }
-                        });
-                        reinterpret_cast<uint4*>(body)[i] = make_uint4(o[0], o[1], o[2], o[3]);
-                        if (i < fetched) fetch(i);
-                    });
-                    // the next row may begin at another alignment and have one word more
-                    if (r.count < fetched && (fetched - 1) % threads == tid) fetch(fetched - 1);
-                } else if (!any && aligned) {
-                    each_word<threads, 4>(tid, r.count, [&](int i) {
-                        reinterpret_cast<uint4*>(body)[i] = make_uint4(0, 0, 0, 0);
-                    });
-                    each_word<threads, 4>(tid, fetched, fetch);
-                } else {  // rows of logits that lie further apart than those of the gradient, or far ones
-                    each_word<threads, 1>(tid, r.count, [&](int i) {
-                        T e[N];
-                        *reinterpret_cast<uint4*>(e) = stage[i];
-#pragma unroll
-                        for (int j = 0; j < N; ++j)
-                            body[i * N + j] =
-                                from_float<T>(any ? ci * exp2_fast(fmaf(to_float(e[j]) - far, c2, base)) : 0.0f);
-                    });
-                    each_word<threads, 4>(tid, fetched, fetch);
-                }
-                if (r.edge >= 0) out[r.edge] = from_float<T>(any ? ci * exp2_fast(fmaf(edge_now, c2, base)) : 0.0f);
-                if (any) {
-                    asm volatile("bar.sync 1, %0;" ::"n"(threads) : "memory");  // the row is written
-                    const int v0 = rank == 0 ? 0 : r.head + r.first * N;
-                    const int v1 = rank == cluster - 1 ? vocab : r.head + (r.first + r.count) * N;
-                    top_gradients<T>(a, top, out, threads, v0, v1, c, c2, base, inv_s);
-                }
-            }
-            copy_commit();
+    }
+    if (is_teacher) {
+        if (rank == 0) {
+            const float v = any ? row_loss(a, top, w, c2, base, s) : 0.0f;
+            if (lane == 0) loss[t] = v;
         }
-        r = n;
-        t = t1;
-        t1 = t2;
-        row = row_next;
-        w = w1;
-        w1 = w2;
+    } else if (out != nullptr) {
+        const float c = w * a.tau, inv_s = s == 0.0f ? 0.0f : 1.0f / s, ci = c * inv_s;
+        if (any && far == 0.0f && aligned) {
+            each_word<THREADS, 2>(tid, r.count, [&](int i) { return words[i]; }, [&](int i, const uint4& x) {
+                uint32_t o[4];
+                word_pairs<T>(x, [&](int j, float2 f) {
+                    f = __ffma2_rn(f, make_float2(c2, c2), make_float2(base, base));
+                    f = __fmul2_rn(make_float2(exp2_fast(f.x), exp2_fast(f.y)), make_float2(ci, ci));
+                    if constexpr (sizeof(T) == 4) {
+                        o[2 * j] = __float_as_uint(f.x);
+                        o[2 * j + 1] = __float_as_uint(f.y);
+                    } else {
+                        o[j] = pack2<T>(f.x, f.y);
+                    }
+                });
+                __stcs(reinterpret_cast<uint4*>(body) + i, make_uint4(o[0], o[1], o[2], o[3]));
+            });
+        } else if (!any && aligned) {
+            for (int i = tid; i < r.count; i += THREADS) __stcs(reinterpret_cast<uint4*>(body) + i, make_uint4(0, 0, 0, 0));
+        } else {  // rows of logits that lie further apart than those of the gradient, or far ones
+            const T* part = reinterpret_cast<const T*>(words);
+            for (int i = tid; i < r.count * N; i += THREADS)
+                body[i] = from_float<T>(any ? ci * exp2_fast(fmaf(to_float(part[i]) - far, c2, base)) : 0.0f);
+        }
+        if (r.edge >= 0) out[r.edge] = from_float<T>(any ? ci * exp2_fast(fmaf(edge, c2, base)) : 0.0f);
+        if (any) {
+            asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");  // the row is written
+            const int v0 = rank == 0 ? 0 : r.head + r.first * N;
+            const int v1 = rank == cluster - 1 ? vocab : r.head + (r.first + r.count) * N;
+            top_gradients<T>(a, top, out, THREADS, v0, v1, c, c2, base, inv_s);
+        }
     }
     if (cluster > 1) cg::this_cluster().sync();  // a peer may still read this block's part
-}
-
-// ------------------------------------------------------------- longer rows ---
-//
-// A row beyond the registers of a cluster of eight blocks: one block reads it three times.
-template <typename T>
-__global__ void __launch_bounds__(1024) distill_long_kernel(DistillArgs a, const T* z, float* __restrict__ loss,
-                                                            T* grad) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ float sh[32];
-    __shared__ Seen seen;
-    const TopList top(smem, a.k);
-    const int64_t t = blockIdx.x;
-    const T* row = z + t * a.stride;
-    T* out = grad != nullptr ? grad + t * a.vocab : nullptr;
-    const float w = a.weight != nullptr ? a.weight[t] : 1.0f;
-    if (w != 0.0f && threadIdx.x < 32) finish_teacher(a, top, load_teacher<T>(a, t, row, top), seen);
-    __syncthreads();
-    if (w == 0.0f || !*top.any) {
-        if (out != nullptr)
-            for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) out[v] = from_float<T>(0.0f);
-        if (threadIdx.x == 0) loss[t] = 0.0f;
-        return;
-    }
-    const float c2 = kLog2E / a.tau;
-    float m = -INFINITY;
-    for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) m = fmaxf(m, to_float(row[v]));
-    m = block_max(m, sh);
-    if (m == -INFINITY) m = 0.0f;
-    // the difference first: no B that could overflow
-    auto term = [&](float x) { return exp2_fast((x - m) * c2); };
-    float s = 0.0f;
-    for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) s += term(to_float(row[v]));
-    s = block_sum(s, sh);
-    if (threadIdx.x < 32) {
-        for (int k = threadIdx.x; k < a.k; k += 32) top.z[k] -= m;
-        __syncwarp();
-        const float l = row_loss(a, top, w, c2, 0.0f, s);
-        if (threadIdx.x == 0) loss[t] = l;
-    }
-    if (out == nullptr) return;
-    const float inv_s = s == 0.0f ? 0.0f : 1.0f / s, c = w * a.tau;
-    for (int64_t v = threadIdx.x; v < a.vocab; v += blockDim.x) out[v] = from_float<T>(c * inv_s * term(to_float(row[v])));
-    __syncthreads();
-    top_gradients<T>(a, top, out, (int)blockDim.x, 0, (int)a.vocab, c, c2, 0.0f, inv_s);
-}
-
-constexpr int64_t kDistillScratch = 32;  // the ticket counter
-
-// Blocks of a row and their threads.
-struct DistillPlan {
-    int cluster, threads;  // cluster 0: the kernel for longer rows
-    int64_t share;         // words of a block
-};
-static DistillPlan distill_plan(int64_t n, int64_t words) {
-    DistillPlan p{1, kDistillThreads, 0};
-    while (p.cluster < 8 && words * 16 > (int64_t)p.cluster * kDistillShare) p.cluster *= 2;
-    if (words * 16 > (int64_t)p.cluster * kDistillLongShare) p.cluster = 0;
-    if (p.cluster == 0) return p;
-    // few rows: more blocks a row, as long as each of their threads has a word
-    while (p.cluster < 8 && n * p.cluster < 2 * 148 && words >= 2 * p.cluster * kDistillThreads) p.cluster *= 2;
-    p.share = ceil_div(words, p.cluster);
-    while (p.threads > kDistillThreads / 4 && p.share <= p.threads / 2) p.threads /= 2;
-    return p;
 }
 
 }  // namespace cresso
@@ -514,17 +390,9 @@ using namespace cresso;
 
 extern "C" {
 
-int cresso_distill_scratch_bytes(int64_t n, int64_t vocab, int64_t* bytes) {
-    CRESSO_REQUIRE(bytes != nullptr, CRESSO_EINVAL, "distill_scratch_bytes: NULL result");
-    CRESSO_REQUIRE(n >= 0 && vocab >= 1, CRESSO_EINVAL, "distill: negative size, or an empty vocabulary");
-    *bytes = kDistillScratch;
-    return CRESSO_OK;
-}
-
 int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, int64_t logits_stride, const void* ids,
                    int64_t id_bytes, const void* teacher, int64_t teacher_dtype, int64_t k, const float* weight,
-                   double temperature, float* loss, void* grad, void* scratch, int64_t scratch_bytes,
-                   cresso_stream_t stream) {
+                   double temperature, float* loss, void* grad, cresso_stream_t stream) {
     CRESSO_REQUIRE(train_dtype_ok(dtype) && train_dtype_ok(teacher_dtype), CRESSO_EUNSUPPORTED,
                    "distill: element types are float32, float16 and bfloat16");
     CRESSO_REQUIRE(id_bytes == 4 || id_bytes == 8, CRESSO_EINVAL, "distill: ids are int32 or int64");
@@ -540,10 +408,6 @@ int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, 
     if (n == 0) return CRESSO_OK;
     CRESSO_REQUIRE(logits != nullptr && loss != nullptr && (k == 0 || (ids != nullptr && teacher != nullptr)),
                    CRESSO_EINVAL, "distill: NULL pointer");
-    CRESSO_REQUIRE(scratch != nullptr && scratch_bytes >= kDistillScratch, CRESSO_ESCRATCH,
-                   "distill: scratch has %lld bytes, %lld are needed", (long long)scratch_bytes,
-                   (long long)kDistillScratch);
-    CRESSO_REQUIRE(aligned_to(scratch, 32), CRESSO_EINVAL, "distill: scratch is not 32-byte aligned");
     CRESSO_REQUIRE(grad != logits || logits_stride == vocab, CRESSO_EINVAL,
                    "distill: a gradient in place of the logits needs contiguous rows");
     NvtxRange range("distill n=%lld", (long long)n);
@@ -554,47 +418,28 @@ int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, 
         const T* z = static_cast<const T*>(logits);
         T* g = static_cast<T*>(grad);
         const cudaStream_t s = (cudaStream_t)stream;
-        const DistillPlan p = distill_plan(n, vocab / N);
-        if (p.cluster == 0) {
-            distill_long_kernel<T><<<(unsigned)n, 1024, top_bytes(a.k), s>>>(a, z, loss, g);
-            CRESSO_LAUNCHED("distill_long_kernel");
-            return (int)CRESSO_OK;
-        }
-        const int smem = (int)p.share * 16 + 3 * top_bytes(a.k);
-        const auto kernel = p.threads == kDistillThreads       ? distill_kernel<T, kDistillThreads>
-                            : p.threads == kDistillThreads / 2 ? distill_kernel<T, kDistillThreads / 2>
-                                                               : distill_kernel<T, kDistillThreads / 4>;
-        if (smem > 48 * 1024)
-            CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             kDistillLongShare + 3 * top_bytes(CRESSO_TRAIN_MAX_TOP)));
+        // blocks of a row: as many as its length asks for, and more where there are few rows
+        const int64_t words = vocab / N;
+        int log_cluster = 0;
+        while ((1 << log_cluster) < kDistillCluster &&
+               (words * 16 > ((int64_t)kDistillShare << log_cluster) ||
+                ((n << log_cluster) < 2 * 148 && words >= (int64_t)(2 << log_cluster) * kDistillThreads)))
+            ++log_cluster;
+        CRESSO_REQUIRE((n << log_cluster) <= CRESSO_TRAIN_MAX_ROWS, CRESSO_EUNSUPPORTED, "distill: too many rows");
+        const bool small = (words >> log_cluster) <= kDistillThreads / 4;
+        const auto kernel = small ? distill_kernel<T, kDistillThreads / 4> : distill_kernel<T, kDistillThreads>;
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)p.cluster);
-        cfg.blockDim = dim3((unsigned)p.threads);
-        cfg.dynamicSmemBytes = (size_t)smem;
+        cfg.gridDim = dim3((unsigned)(n << log_cluster));
+        cfg.blockDim = dim3((unsigned)(small ? kDistillThreads / 4 : kDistillThreads) + 32);
+        cfg.dynamicSmemBytes = (size_t)top_bytes(a.k);
         cfg.stream = s;
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = (unsigned)p.cluster;
+        attr.val.clusterDim.x = 1u << log_cluster;
         attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
         cfg.attrs = &attr;
-        cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-        int64_t workers = n;  // as many as stay on the GPU together
-        if (n * p.cluster > 148) {
-            int fit = 0;
-            if (p.cluster > 1) {
-                CRESSO_CUDA(cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg));
-            } else {
-                CRESSO_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, p.threads, (size_t)smem));
-                fit *= 148;
-            }
-            workers = std::min<int64_t>(n, std::max(1, fit));
-        }
-        cfg.gridDim = dim3((unsigned)(workers * p.cluster));
-        int log_cluster = 0;
-        while ((1 << log_cluster) < p.cluster) ++log_cluster;
-        unsigned long long* tickets = static_cast<unsigned long long*>(scratch);
-        if (n > workers) CRESSO_CUDA(cudaMemsetAsync(tickets, 0, 8, s));
-        CRESSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, n, z, loss, g, log_cluster, tickets));
+        cfg.numAttrs = log_cluster > 0 ? 1 : 0;
+        CRESSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, z, loss, g, log_cluster));
         CRESSO_LAUNCHED("distill_kernel");
         return (int)CRESSO_OK;
     });

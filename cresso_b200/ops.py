@@ -400,11 +400,9 @@ def _distill(what: str, logits: Tensor, ids: Tensor, teacher: Tensor, weight: Op
     loss = torch.empty(lead, dtype=torch.float32, device=device)
     grad = None if not backward else logits if inplace else torch.empty(logits.shape, dtype=logits.dtype,
                                                                        device=device)
-    L = _lib.lib()
-    scratch = _train_scratch(what, L.cresso_distill_scratch_bytes, device, n, vocab)
-    _train_call(what, L.cresso_distill, device, rows.data_ptr(), ld, n, vocab, stride, ids.data_ptr(),
+    _train_call(what, _lib.lib().cresso_distill, device, rows.data_ptr(), ld, n, vocab, stride, ids.data_ptr(),
                 _ID_BYTES[ids.dtype], teacher.data_ptr(), td, k, _address(weight), temperature, loss.data_ptr(),
-                _address(grad), scratch.data_ptr(), scratch.numel())
+                _address(grad))
     return loss, grad
 
 

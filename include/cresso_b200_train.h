@@ -95,11 +95,10 @@ CRESSO_API int cresso_block_norm_grad(const void* h, const void* x, const void* 
  * weight float32 (n) or NULL (1); loss is float32 (n); grad has the logits'
  * type, contiguous (n, vocab), and may be the logits themselves when their rows
  * are contiguous; grad NULL computes the loss only. */
-CRESSO_API int cresso_distill_scratch_bytes(int64_t n, int64_t vocab, int64_t* bytes);
 CRESSO_API int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, int64_t logits_stride,
                               const void* ids, int64_t id_bytes, const void* teacher, int64_t teacher_dtype, int64_t k,
-                              const float* weight, double temperature, float* loss, void* grad, void* scratch,
-                              int64_t scratch_bytes, cresso_stream_t stream);
+                              const float* weight, double temperature, float* loss, void* grad,
+                              cresso_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -100,7 +100,7 @@ def test_block_norm_grad_status(kw, status):
 
 def _distill(**kw):
     a = dict(logits=4096, dt=0, n=4, vocab=10, stride=10, ids=4096, ib=8, teacher=4096, td=0, k=3, weight=0, tau=1.0,
-             loss=4096, grad=8192, scratch=4096, nbytes=64)
+             loss=4096, grad=8192)
     a.update(kw)
     return _lib.lib().cresso_distill(*a.values(), None)
 
@@ -109,8 +109,7 @@ def _distill(**kw):
     (dict(dt=3), 2), (dict(td=3), 2), (dict(ib=2), 1), (dict(n=-1), 1), (dict(vocab=0), 1), (dict(stride=9), 1),
     (dict(k=-1), 1), (dict(k=1025), 2), (dict(n=2**31), 2), (dict(tau=0.0), 1), (dict(tau=-1.0), 1),
     (dict(tau=float("nan")), 1), (dict(tau=float("inf")), 1), (dict(logits=0), 1), (dict(loss=0), 1),
-    (dict(ids=0), 1), (dict(teacher=0), 1), (dict(stride=12, grad=4096), 1), (dict(scratch=0), 4),
-    (dict(nbytes=8), 4), (dict(scratch=4104), 1), (dict(n=0), 0)])
+    (dict(ids=0), 1), (dict(teacher=0), 1), (dict(stride=12, grad=4096), 1), (dict(n=0), 0)])
 def test_distill_status(kw, status):
     assert _distill(**kw) == status, _lib.last_error()
 
