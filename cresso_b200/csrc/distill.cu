@@ -8,12 +8,13 @@
 //   dz_v = w tau (q_v - P_v),  P_v = sum of p_k with id_k = v.
 // Exponentials are 2^(z c - B) with c = log2(e) / tau and one B for the whole row: a fused
 // operation, whose error is that of its result, because the same rounded B stands in the sum,
-// in the gradient and in the loss.  B needs no maximum over the row: it is r c for the largest
-// student logit r at the teacher's ids, so the sum is at least 1, and only a row with a logit
-// about 40 tau above r (or far from zero, or without a finite r) overflows; such a row is
-// computed again from its maximum.  Sums are float32.  A NaN or +inf logit makes its row NaN
-// through the sum; a row of -inf alone has q = 0.  Repeated ids: every entry holds the whole P
-// of its id, so that all of them write the same value.
+// in the gradient and in the loss.  B needs no maximum over the row, only a reference near it:
+// every warp takes the largest of the first logits it reads, sums relative to that, and the
+// parts are joined relative to the largest reference.  A row whose sum leaves [1e-18, 1e18]
+// (a later logit about 40 tau above its warp's reference, a row far from zero or without
+// finite logits) is computed again from its maximum.  Sums are float32.  A NaN or +inf logit
+// makes its row NaN through the sum; a row of -inf alone has q = 0.  Repeated ids: every entry
+// holds the whole P of its id, so that all of them write the same value.
 #include "train_common.cuh"
 
 #include <cooperative_groups.h>
@@ -32,18 +33,17 @@ struct DistillArgs {
 };
 
 // The teacher's side of a row in shared memory: k ids (-1: not valid), teacher probabilities,
-// their sums over equal ids and student logits at the ids, then the sum of p log p, whether a
-// valid entry exists, and the largest of the logits.
+// their sums over equal ids and student logits at the ids, then the sum of p log p and whether
+// a valid entry exists.
 struct TopList {
     int* id;
     float *p, *same, *z, *entropy;
     int* any;
-    float* reference;
     __device__ __forceinline__ TopList(unsigned char* at, int k)
         : id(reinterpret_cast<int*>(at)), p(reinterpret_cast<float*>(at) + k), same(p + k), z(same + k), entropy(z + k),
-          any(reinterpret_cast<int*>(entropy + 1)), reference(entropy + 2) {}
+          any(reinterpret_cast<int*>(entropy + 1)) {}
 };
-__host__ __device__ constexpr int top_bytes(int k) { return (16 * k + 12 + 15) / 16 * 16; }
+__host__ __device__ constexpr int top_bytes(int k) { return (16 * k + 8 + 15) / 16 * 16; }
 
 // One warp's set of bits that finds ids that may occur twice, and the list of those.
 constexpr int kSeenBits = 16384;
@@ -61,12 +61,14 @@ __device__ __forceinline__ float exp2_fast(float x) {  // relative error 2^-22
 }
 
 // Fills the list with one warp; the block sees it after its next barrier.  First the loads, four
-// entries a lane in flight together, and the reference; returns the largest teacher logit.
+// entries a lane in flight together.
 template <typename T>
-__device__ __forceinline__ float load_teacher(const DistillArgs& a, int64_t t, const T* row, const TopList& top) {
+__device__ __forceinline__ void load_teacher(const DistillArgs& a, int64_t t, const T* row, const TopList& top, Seen& seen) {
     const int lane = threadIdx.x & 31;
     const int64_t at = t * a.k;
-    float m = -INFINITY, r = -INFINITY;
+    float m = -INFINITY;
+    for (int i = lane; i < kSeenBits / 32; i += 32) seen.bits[i] = 0;
+    if (lane == 0) seen.count = 0;
     for (int k0 = 0; k0 < a.k; k0 += 128) {
         int64_t id[4];
         float u[4], z[4];
@@ -88,23 +90,11 @@ __device__ __forceinline__ float load_teacher(const DistillArgs& a, int64_t t, c
             top.id[k] = (int)id[j];
             top.p[k] = u[j];
             top.z[k] = z[j];
-            if (id[j] >= 0) {
-                m = fmaxf(m, u[j]);
-                r = fmaxf(r, z[j]);
-            }
+            if (id[j] >= 0) m = fmaxf(m, u[j]);
         }
     }
-    r = warp_max(r);
-    if (lane == 0) *top.reference = r;
     __syncwarp();
-    return warp_max(m);
-}
-// Then the probabilities.
-__device__ __forceinline__ void finish_teacher(const DistillArgs& a, const TopList& top, float m, Seen& seen) {
-    const int lane = threadIdx.x & 31;
-    for (int i = lane; i < kSeenBits / 32; i += 32) seen.bits[i] = 0;
-    if (lane == 0) seen.count = 0;
-    __syncwarp();
+    m = warp_max(m);
     const float inv_tau = 1.0f / a.tau;
     float s = 0.0f;
     bool valid_here = false;
@@ -148,14 +138,16 @@ __device__ __forceinline__ void finish_teacher(const DistillArgs& a, const TopLi
     __syncwarp();
 }
 
-// Joins (maximum, sum relative to it) over the first WIDTH lanes of a warp; all lanes get it.
-template <int WIDTH>
+// Joins (reference, sum relative to it) over the first WIDTH lanes of a warp; all lanes get it.
+// The sums are relative to the rounded B of their references, or (FAR) to the maxima themselves,
+// whose B may overflow.
+template <int WIDTH, bool FAR = false>
 __device__ __forceinline__ void join_warp(float& m, float& s, float c2) {
     float top = m;
 #pragma unroll
     for (int o = WIDTH / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    // a part without a finite maximum holds 0 or NaN and keeps it
-    s *= m == top ? 1.0f : exp2_fast((m - top) * c2);
+    // a part without a finite reference holds 0 or NaN and keeps it
+    s *= m == top ? 1.0f : exp2_fast(FAR ? (m - top) * c2 : __fmul_rn(m, c2) - __fmul_rn(top, c2));
 #pragma unroll
     for (int o = WIDTH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     m = __shfl_sync(0xffffffffu, top, 0);
@@ -194,11 +186,42 @@ __device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopLis
 // storage on the SM means many blocks an SM, in different phases: their loads overlap the others'
 // exponentials, barriers and teacher lists.  One further warp prepares the teacher's list.
 constexpr int kDistillThreads = 256;         // without the teacher's warp
-constexpr int kDistillShare = 64 * 1024;     // bytes of a row that a block is given at least
+// Bytes of a row that a block is given at least.  With the gradient, more of them are in L2 for
+// longer and fewer blocks are better: 64 KB.  The loss alone is bound by what a block does before
+// and after its part: 128 KB (1023 rows of 100003 float16: 41 us, 49 with 64 KB).
+constexpr int64_t kDistillShare = 64 * 1024, kDistillLossShare = 128 * 1024;
 constexpr int kDistillCluster = 8;
 
 template <typename T>
 constexpr int kWordLogits = 16 / (int)sizeof(T);
+
+// Running maximum of the logits of words; NaN is left out.
+template <typename T>
+struct WordMax {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    T2 m;
+    __device__ __forceinline__ WordMax() {
+        const uint32_t none = std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+        m = *reinterpret_cast<const T2*>(&none);
+    }
+    __device__ __forceinline__ void add(const uint4& w) {
+        auto two = [](const uint32_t& v) { return *reinterpret_cast<const T2*>(&v); };
+        m = __hmax2(__hmax2(m, __hmax2(two(w.x), two(w.y))), __hmax2(two(w.z), two(w.w)));
+    }
+    __device__ __forceinline__ float get() const {
+        const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t*>(&m));
+        return fmaxf(f.x, f.y);
+    }
+};
+template <>
+struct WordMax<float> {
+    float m = -INFINITY;
+    __device__ __forceinline__ void add(const uint4& w) {
+        m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(w.x), __uint_as_float(w.y))),
+                  fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+    }
+    __device__ __forceinline__ float get() const { return m; }
+};
 
 // f(i, pair): the logits of a word two at a time.
 template <typename T, typename F>
@@ -235,11 +258,10 @@ __device__ __forceinline__ RowShare row_share(const T* row, int vocab, int rank,
     return r;
 }
 
-// f(i, get(i)) for the words i = tid, tid + THREADS, ... below count; U of them are fetched
-// before the first is used.
+// f(i, get(i)) for the words i, i + THREADS, ... below count; U of them are fetched before
+// the first is used.
 template <int THREADS, int U, typename G, typename F>
-__device__ __forceinline__ void each_word(int tid, int count, G get, F f) {
-    int i = tid;
+__device__ __forceinline__ void each_word(int i, int count, G get, F f) {
     for (; i + (U - 1) * THREADS < count; i += U * THREADS) {
         uint4 x[U];
 #pragma unroll
@@ -271,45 +293,59 @@ __global__ void __launch_bounds__(THREADS + 32)
     const bool aligned = (reinterpret_cast<uintptr_t>(body) & 15) == 0;
     const float w = a.weight != nullptr ? a.weight[t] : 1.0f;
     const float c2 = kLog2E / a.tau;
+    constexpr int U = 4;
+    constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+    uint4 x[U];  // the first words, on their way before the weight is known
+    float edge = -INFINITY;
+    if (!is_teacher) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            x[u] = tid + u * THREADS < r.count ? words[tid + u * THREADS] : make_uint4(kNone, kNone, kNone, kNone);
+        if (r.edge >= 0) edge = to_float(row[r.edge]);
+    }
     bool any = false;
-    float s = 0.0f, base = 0.0f, far = 0.0f, edge = -INFINITY;
+    float m = 0.0f, s = 0.0f, far = 0.0f;
     if (w != 0.0f) {
-        float teacher_top = 0.0f;
-        if (is_teacher)
-            teacher_top = load_teacher<T>(a, t, row, top);
-        else if (r.edge >= 0)
-            edge = to_float(row[r.edge]);
-        __syncthreads();  // the reference
-        base = -__fmul_rn(*top.reference, c2);
         if (is_teacher) {
-            finish_teacher(a, top, teacher_top, seen);
+            load_teacher<T>(a, t, row, top, seen);
         } else {
+            WordMax<T> first;
+#pragma unroll
+            for (int u = 0; u < U; ++u) first.add(x[u]);
+            m = warp_max(fmaxf(first.get(), edge));
+            if (!(fabsf(m * c2) <= kFar)) m = 0.0f;
+            const float base = -__fmul_rn(m, c2);
             float2 sum = make_float2(exp2_fast(fmaf(edge, c2, base)), 0.0f);
-            each_word<THREADS, 4>(tid, r.count, [&](int i) { return words[i]; }, [&](int, const uint4& x) {
-                word_pairs<T>(x, [&](int, float2 f) {
+            auto add = [&](int, const uint4& y) {
+                word_pairs<T>(y, [&](int, float2 f) {
                     f = __ffma2_rn(f, make_float2(c2, c2), make_float2(base, base));
                     sum = __fadd2_rn(sum, make_float2(exp2_fast(f.x), exp2_fast(f.y)));
                 });
-            });
+            };
+#pragma unroll
+            for (int u = 0; u < U; ++u) add(0, x[u]);
+            each_word<THREADS, U>(tid + U * THREADS, r.count, [&](int i) { return words[i]; }, add);
             s = warp_sum(sum.x + sum.y);
-            if (lane == 0) warp_part[warp] = make_float2(0.0f, s);
+            if (lane == 0) warp_part[warp] = make_float2(m, s);
         }
         __syncthreads();
-        s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < warps; ++i) s += warp_part[i].y;
+        m = lane < warps ? warp_part[lane].x : -INFINITY;
+        s = lane < warps ? warp_part[lane].y : 0.0f;
+        join_warp<8>(m, s, c2);
         if (cluster > 1) {
             cg::cluster_group group = cg::this_cluster();
-            if (tid == 0) block_part = make_float2(0.0f, s);
+            if (tid == 0) block_part = make_float2(m, s);
             group.sync();
-            s = 0.0f;
-            for (int i = 0; i < cluster; ++i) s += group.map_shared_rank(&block_part, i)->y;
+            const float2 p = lane < cluster ? *group.map_shared_rank(&block_part, lane) : make_float2(-INFINITY, 0.0f);
+            m = p.x;
+            s = p.y;
+            join_warp<8>(m, s, c2);
         }
         any = *top.any;
-        if (any && !(s < kLargeSum && fabsf(base) <= kFar)) {
+        if (any && !(s < kLargeSum && s > 1.0f / kLargeSum)) {
             // no usable reference: from the row's maximum
             const T* part = reinterpret_cast<const T*>(words);
-            float m = -INFINITY;
+            m = -INFINITY;
             s = 0.0f;
             if (!is_teacher) {
                 m = edge;
@@ -317,14 +353,14 @@ __global__ void __launch_bounds__(THREADS + 32)
                 const float from = m == -INFINITY ? 0.0f : m;
                 s = exp2_fast((edge - from) * c2);
                 for (int i = tid; i < r.count * N; i += THREADS) s += exp2_fast((to_float(part[i]) - from) * c2);
-                join_warp<32>(m, s, c2);
+                join_warp<32, true>(m, s, c2);
             }
             __syncthreads();  // the parts of the first exchange have been read
             if (!is_teacher && lane == 0) warp_part[warp] = make_float2(m, s);
             __syncthreads();
             m = lane < warps ? warp_part[lane].x : -INFINITY;
             s = lane < warps ? warp_part[lane].y : 0.0f;
-            join_warp<8>(m, s, c2);
+            join_warp<8, true>(m, s, c2);
             if (cluster > 1) {
                 cg::cluster_group group = cg::this_cluster();
                 group.sync();
@@ -333,17 +369,18 @@ __global__ void __launch_bounds__(THREADS + 32)
                 const float2 p = lane < cluster ? *group.map_shared_rank(&block_part, lane) : make_float2(-INFINITY, 0.0f);
                 m = p.x;
                 s = p.y;
-                join_warp<8>(m, s, c2);
+                join_warp<8, true>(m, s, c2);
             }
             if (m == INFINITY) s = NAN;
             far = m == -INFINITY ? 0.0f : m;
-            base = 0.0f;
+            m = 0.0f;
             edge -= far;
             if (is_teacher)
                 for (int k = lane; k < a.k; k += 32) top.z[k] -= far;
             __syncthreads();
         }
     }
+    const float base = -__fmul_rn(m, c2);
     if (is_teacher) {
         if (rank == 0) {
             const float v = any ? row_loss(a, top, w, c2, base, s) : 0.0f;
@@ -422,7 +459,7 @@ int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, 
         const int64_t words = vocab / N;
         int log_cluster = 0;
         while ((1 << log_cluster) < kDistillCluster &&
-               (words * 16 > ((int64_t)kDistillShare << log_cluster) ||
+               (words * 16 > ((g != nullptr ? kDistillShare : kDistillLossShare) << log_cluster) ||
                 ((n << log_cluster) < 2 * 148 && words >= (int64_t)(2 << log_cluster) * kDistillThreads)))
             ++log_cluster;
         CRESSO_REQUIRE((n << log_cluster) <= CRESSO_TRAIN_MAX_ROWS, CRESSO_EUNSUPPORTED, "distill: too many rows");
