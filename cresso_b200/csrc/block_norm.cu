@@ -23,43 +23,123 @@ struct NormArgs {
     float scale, eps;
 };
 
-template <typename TR, typename TX>
-__global__ void __launch_bounds__(kThreads) norm_kernel(NormArgs a, const TR* __restrict__ res,
-                                                        const TX* __restrict__ x, TR* __restrict__ h,
-                                                        TX* __restrict__ y) {
-    __shared__ float sh[32];
-    const int64_t t = blockIdx.x, d = a.width;
-    const int64_t g0 = a.gate != nullptr ? t / a.rows_per_gate * d : 0;
-    const float inv_d = 1.0f / (float)d;
-    float rx = 1.0f;
-    if (x != nullptr && a.post_w != nullptr) {
-        float s = 0.0f;
-        for (int64_t c = threadIdx.x; c < d; c += kThreads) {
-            const float v = to_float(x[t * d + c]);
-            s += v * v;
+constexpr int kNormElems = 16;                         // columns of a thread
+constexpr int kNormBlockWidth = 512 * kNormElems;      // columns of a block
+constexpr int kNormMaxWidth = CRESSO_TRAIN_MAX_NORM_WIDTH;  // columns of a cluster of 8
+
+// Blocks and threads of a row: a row of more than 8192 columns is cut over a cluster of 2 to 8
+// blocks, which add their sums through distributed shared memory.
+struct NormShape {
+    int threads, cluster, block_width;
+};
+static NormShape norm_shape(int64_t width) {
+    NormShape p{};
+    p.cluster = pow2_ceil(ceil_div(width, kNormBlockWidth));
+    p.block_width = (int)(p.cluster > 1 ? align_up(ceil_div(width, p.cluster), 8) : width);
+    p.threads = std::max(32, pow2_ceil(ceil_div(p.block_width, kNormElems)));
+    return p;
+}
+
+// ----------------------------------------------------------------- forward ---
+//
+// A row lies in the registers of a block (of a warp up to 512 columns, four rows a block), 16
+// columns a thread: x and residual are read once, h and y written once, two reductions between.
+// Weights and gate come from L1 for every row.  Many small blocks an SM, each at another point
+// of its row, keep the memory busy without any staging.
+template <typename TR, typename TX, int VEC>
+__global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __restrict__ res,
+                                                      const TX* __restrict__ x, TR* __restrict__ h,
+                                                      TX* __restrict__ y, int cluster, int block_width) {
+    constexpr int NV = kNormElems / VEC;
+    namespace cg = cooperative_groups;
+    __shared__ float red[2][32], peer[2];
+    const int64_t width = a.width;
+    const int rank = cluster > 1 ? (int)(blockIdx.x % cluster) : 0;
+    const int64_t col0 = (int64_t)rank * block_width;
+    const int d = (int)min((int64_t)block_width, width - col0);
+    const int T = blockDim.x, tid = threadIdx.x, warps = T >> 5;  // blockDim.y rows, one warp each, when T is 32
+    const int64_t t = (int64_t)(blockIdx.x / cluster) * blockDim.y + threadIdx.y;
+    if (t >= a.n) return;  // a whole warp of the last block
+    const float inv_d = 1.0f / (float)width;
+    auto row_sum = [&](float v, int k) {
+        v = warp_sum(v);
+        if (warps > 1) {
+            if ((tid & 31) == 0) red[k][tid >> 5] = v;
+            __syncthreads();
+            v = warp_sum((tid & 31) < warps ? red[k][tid & 31] : 0.0f);
         }
-        rx = rsqrtf(block_sum(s, sh) * inv_d + a.eps);
-    }
-    auto value = [&](int64_t c) {
-        float v = to_float(res[t * d + c]);
-        if (x != nullptr) {
-            float p = to_float(x[t * d + c]) * rx;
-            if (a.post_w != nullptr) p *= load_any(a.post_w, a.w_dtype, c);
-            if (a.gate != nullptr) p *= load_any(a.gate, a.gate_dtype, g0 + c);
-            v += a.scale * p;
+        if (cluster > 1) {
+            cg::cluster_group group = cg::this_cluster();
+            if (tid == 0) peer[k] = v;
+            group.sync();
+            v = 0.0f;
+            for (int i = 0; i < cluster; ++i) v += *group.map_shared_rank(&peer[k], i);
         }
         return v;
     };
-    float s = 0.0f;
-    for (int64_t c = threadIdx.x; c < d; c += kThreads) {
-        const float v = value(c);
-        s += v * v;
-        if (x != nullptr) h[t * d + c] = from_float<TR>(v);
+    float hv[NV][VEC], xv[NV][VEC];
+    const int64_t at = t * width + col0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const int c = (v * T + tid) * VEC;
+        if (c >= d) break;
+        if (x != nullptr) load_global<TX, VEC>(x + at + c, xv[v]);
+        load_global<TR, VEC>(res + at + c, hv[v]);
     }
-    if (y == nullptr) return;
-    const float rh = rsqrtf(block_sum(s, sh) * inv_d + a.eps);
-    for (int64_t c = threadIdx.x; c < d; c += kThreads)
-        y[t * d + c] = from_float<TX>(value(c) * rh * load_any(a.pre_w, a.w_dtype, c));
+    if (x != nullptr) {
+        float rx = 1.0f;
+        if (a.post_w != nullptr) {
+            float s = 0.0f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                if ((v * T + tid) * VEC >= d) break;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) s += xv[v][j] * xv[v][j];
+            }
+            rx = rsqrtf(row_sum(s, 0) * inv_d + a.eps);
+        }
+        const int64_t g0 = a.gate != nullptr ? t / a.rows_per_gate * width + col0 : 0;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = (v * T + tid) * VEC;
+            if (c >= d) break;
+            float f[VEC];
+            if (a.post_w != nullptr) {
+                load_any_vec<VEC>(a.post_w, a.w_dtype, col0 + c, f);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) xv[v][j] *= rx * f[j];
+            }
+            if (a.gate != nullptr) {
+                load_any_vec<VEC>(a.gate, a.gate_dtype, g0 + c, f);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) xv[v][j] *= f[j];
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) hv[v][j] += a.scale * xv[v][j];
+            store_global<TR, VEC>(h + at + c, hv[v]);
+        }
+    }
+    if (y != nullptr) {
+        float s = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if ((v * T + tid) * VEC >= d) break;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s += hv[v][j] * hv[v][j];
+        }
+        const float rh = rsqrtf(row_sum(s, 1) * inv_d + a.eps);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int c = (v * T + tid) * VEC;
+            if (c >= d) break;
+            float f[VEC];
+            load_any_vec<VEC>(a.pre_w, a.w_dtype, col0 + c, f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] *= hv[v][j] * rh;
+            store_global<TX, VEC>(y + at + c, f);
+        }
+    }
+    if (cluster > 1) cg::this_cluster().sync();  // a peer may still read this block's sums
 }
 
 // ---------------------------------------------------------------- backward ---
@@ -73,13 +153,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(NormArgs a, const TR* __
 //   d_gate = scale w_post B,  d_post = scale gate B
 // (a gate with a row of its own for each row: d_gate per row, B over e q gate).
 // Rows come through `stages` stages of shared memory that cp.async fills ahead; each
-// thread copies and reads the same columns.  A row of more than 8192 columns is cut
-// over a cluster of 2 to 8 blocks, which add their six sums through distributed shared
-// memory.
-constexpr int kNormElems = 16;                         // columns of a thread
-constexpr int kNormBlockWidth = 512 * kNormElems;      // columns of a block
-constexpr int kNormMaxWidth = CRESSO_TRAIN_MAX_NORM_WIDTH;  // columns of a cluster of 8
-
+// thread copies and reads the same columns.
 struct NormGrad {
     NormArgs a;
     const void *h, *x, *dh, *dy;
@@ -358,16 +432,14 @@ __global__ void __launch_bounds__(kThreads) norm_columns_kernel(NormArgs a, Norm
 // Threads of a block, resident blocks to fill and the units of a backward pass, from
 // the sizes alone.
 struct NormGradPlan {
-    int threads, cluster, block_width;
+    NormShape shape;
     int64_t workers, units, units_per_gate;  // workers: blocks or clusters
     int64_t off_b, off_pre, off_post, bytes;
 };
 static NormGradPlan norm_grad_plan(int64_t n, int64_t width, int64_t gate_rows) {
     NormGradPlan p{};
-    p.cluster = pow2_ceil(ceil_div(width, kNormBlockWidth));
-    p.block_width = (int)(p.cluster > 1 ? align_up(ceil_div(width, p.cluster), 8) : width);
-    p.threads = std::max(32, pow2_ceil(ceil_div(p.block_width, kNormElems)));
-    const int64_t want = 148 * std::max(1, 512 / p.threads) / p.cluster;
+    p.shape = norm_shape(width);
+    const int64_t want = 148 * std::max(1, 512 / p.shape.threads) / p.shape.cluster;
     const bool own = gate_rows == n && n > 1;
     const int64_t groups = own || gate_rows < 1 ? 1 : gate_rows;
     const int64_t rows = n / groups;
@@ -420,19 +492,46 @@ int cresso_block_norm(const void* residual, const void* x, const void* post_weig
     CRESSO_REQUIRE(x != nullptr || (post_weight == nullptr && gate == nullptr) || n == 0 || width == 0, CRESSO_EINVAL,
                    "block_norm: a post weight or a gate needs x");
     if (n == 0 || width == 0) return CRESSO_OK;
+    CRESSO_REQUIRE(width <= kNormMaxWidth && n <= CRESSO_TRAIN_MAX_ROWS / 8, CRESSO_EUNSUPPORTED,
+                   "block_norm: more than %d columns or 2^28 - 32 rows", kNormMaxWidth);
     CRESSO_REQUIRE(residual != nullptr && (x == nullptr || h != nullptr) && (pre_weight == nullptr) == (y == nullptr) &&
                        (x != nullptr || y != nullptr),
                    CRESSO_EINVAL, "block_norm: NULL pointer, or y without pre_weight");
     NvtxRange range("block_norm n=%lld", (long long)n);
     const NormArgs a{post_weight, pre_weight, gate, n, width, gate != nullptr ? n / gate_rows : n,
                      (int)weight_dtype, (int)gate_dtype, (float)scale, (float)eps};
+    const NormShape p = norm_shape(width);
+    const int64_t rb = dtype_bytes(res_dtype), xb = dtype_bytes(act_dtype), wb = dtype_bytes(weight_dtype),
+                  gb = dtype_bytes(gate_dtype);
+    // the widest accesses that the width and the addresses allow
+    auto fits = [&](int64_t vec) {
+        auto ok = [&](const void* q, int64_t bytes) { return aligned_to(q, std::min<int64_t>(32, vec * bytes)); };
+        return width % vec == 0 && ok(residual, rb) && ok(h, rb) && ok(x, xb) && ok(y, xb) && ok(post_weight, wb) &&
+               ok(pre_weight, wb) && ok(gate, gb);
+    };
     return with_norm_types(res_dtype, act_dtype, [&](auto tr, auto tx) {
         using TR = decltype(tr);
         using TX = decltype(tx);
-        norm_kernel<TR, TX><<<(unsigned)n, kThreads, 0, (cudaStream_t)stream>>>(
-            a, static_cast<const TR*>(residual), static_cast<const TX*>(x), static_cast<TR*>(h), static_cast<TX*>(y));
-        CRESSO_LAUNCHED("norm_kernel");
-        return (int)CRESSO_OK;
+        auto launch = [&](auto kernel) {
+            const int rows = p.threads == 32 ? 4 : 1;
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3((unsigned)(ceil_div(n, rows) * p.cluster));
+            cfg.blockDim = dim3((unsigned)p.threads, (unsigned)rows);
+            cfg.stream = (cudaStream_t)stream;
+            cudaLaunchAttribute attr{};
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = (unsigned)p.cluster;
+            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr;
+            cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+            CRESSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, static_cast<const TR*>(residual), static_cast<const TX*>(x),
+                                           static_cast<TR*>(h), static_cast<TX*>(y), p.cluster, p.block_width));
+            CRESSO_LAUNCHED("norm_kernel");
+            return (int)CRESSO_OK;
+        };
+        if (fits(8)) return launch(norm_kernel<TR, TX, 8>);
+        if (fits(2)) return launch(norm_kernel<TR, TX, 2>);
+        return launch(norm_kernel<TR, TX, 1>);
     });
 }
 
@@ -464,7 +563,8 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
             CRESSO_CUDA(cudaMemsetAsync(d_gate, 0, (size_t)(gate_rows * width * dtype_bytes(gate_dtype)), s));
         return CRESSO_OK;
     }
-    CRESSO_REQUIRE(width <= kNormMaxWidth, CRESSO_EUNSUPPORTED, "block_norm_grad: width above %d", kNormMaxWidth);
+    CRESSO_REQUIRE(width <= kNormMaxWidth && n <= CRESSO_TRAIN_MAX_ROWS / 8, CRESSO_EUNSUPPORTED,
+                   "block_norm_grad: more than %d columns or 2^28 - 32 rows", kNormMaxWidth);
     CRESSO_REQUIRE(x != nullptr || (post_weight == nullptr && gate == nullptr), CRESSO_EINVAL,
                    "block_norm_grad: a post weight or a gate needs x");
     CRESSO_REQUIRE(h != nullptr && d_residual != nullptr && (d_h != nullptr || d_y != nullptr) &&
@@ -496,13 +596,13 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
     k.part_pre = reinterpret_cast<float*>(base + p.off_pre);
     k.units = p.units;
     k.units_per_gate = p.units_per_gate;
-    k.cluster = p.cluster;
-    k.block_width = p.block_width;
+    k.cluster = p.shape.cluster;
+    k.block_width = p.shape.block_width;
     const int64_t rb = dtype_bytes(res_dtype), xb = dtype_bytes(act_dtype);
-    const int stage = (int)(align_up(p.block_width, 8) * 2 * (rb + xb));
+    const int stage = (int)(align_up(p.shape.block_width, 8) * 2 * (rb + xb));
     // as many blocks an SM as the registers admit where each of them has two stages, else
     // as many stages as fit for one block
-    const int share = 220 * 1024 / std::max(1, 512 / p.threads) - 2048;
+    const int share = 220 * 1024 / std::max(1, 512 / p.shape.threads) - 2048;
     k.stages = 2 * stage <= share ? std::min(4, share / stage) : std::min(4, 220 * 1024 / stage);
     const int smem = k.stages * stage;
     // the widest accesses that the width and the addresses allow
@@ -518,16 +618,16 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
         auto launch = [&](auto kernel) {
             CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
             cudaLaunchConfig_t cfg{};
-            cfg.gridDim = dim3((unsigned)(p.workers * p.cluster));
-            cfg.blockDim = dim3((unsigned)p.threads);
+            cfg.gridDim = dim3((unsigned)(p.workers * p.shape.cluster));
+            cfg.blockDim = dim3((unsigned)p.shape.threads);
             cfg.dynamicSmemBytes = (size_t)smem;
             cfg.stream = s;
             cudaLaunchAttribute attr{};
             attr.id = cudaLaunchAttributeClusterDimension;
-            attr.val.clusterDim.x = (unsigned)p.cluster;
+            attr.val.clusterDim.x = (unsigned)p.shape.cluster;
             attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
             cfg.attrs = &attr;
-            cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+            cfg.numAttrs = p.shape.cluster > 1 ? 1 : 0;
             CRESSO_CUDA(cudaLaunchKernelEx(&cfg, kernel, k));
             CRESSO_LAUNCHED("norm_grad_kernel");
             return (int)CRESSO_OK;

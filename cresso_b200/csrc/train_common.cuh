@@ -212,6 +212,17 @@ __device__ __forceinline__ void store_global(T* p, const float (&f)[VEC]) {
     u.store(p);
 }
 
+// VEC elements of an array whose type is only known at run time; the branch is uniform.
+template <int VEC>
+__device__ __forceinline__ void load_any_vec(const void* p, int dtype, int64_t i, float (&f)[VEC]) {
+    if (dtype == CRESSO_DTYPE_F32)
+        load_global<float, VEC>(static_cast<const float*>(p) + i, f);
+    else if (dtype == CRESSO_DTYPE_F16)
+        load_global<__half, VEC>(static_cast<const __half*>(p) + i, f);
+    else
+        load_global<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(p) + i, f);
+}
+
 // Asynchronous copy of VEC elements from global to shared memory in 16-, 8- or 4-byte
 // pieces, counted by copy_commit / copy_wait; 2-byte pieces are copied at once.
 template <typename T, int VEC>
