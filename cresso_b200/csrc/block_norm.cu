@@ -203,52 +203,87 @@ __device__ __forceinline__ void sum8(float (&v)[8], float* red, int warps) {
     }
 }
 
-template <typename TR, typename TX, int VEC, bool OWN_GATE>
+// Eight columns of a thread, held as pairs for the two-lane float32 instructions: the accesses
+// [chunk 8 / VEC, (chunk + 1) 8 / VEC) of VEC columns, the accesses of a row T VEC columns apart.
+// `c` is the thread's first column, d the row's end; WHOLE: every column is inside.
+template <int VEC, bool WHOLE, typename L>
+__device__ __forceinline__ void get8(int chunk, int c, int stride, int d, float2 (&f)[4], L load) {
+#pragma unroll
+    for (int i = 0; i < 8 / VEC; ++i) {
+        const int col = c + (chunk * (8 / VEC) + i) * stride;
+        float v[VEC];
+        if (!WHOLE)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = 0.0f;
+        if (WHOLE || col < d) load(col, v);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) (((i * VEC + j) & 1) ? f[(i * VEC + j) / 2].y : f[(i * VEC + j) / 2].x) = v[j];
+    }
+}
+template <int VEC, bool WHOLE, typename S>
+__device__ __forceinline__ void put8(int chunk, int c, int stride, int d, const float2 (&f)[4], S store) {
+#pragma unroll
+    for (int i = 0; i < 8 / VEC; ++i) {
+        const int col = c + (chunk * (8 / VEC) + i) * stride;
+        float v[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = ((i * VEC + j) & 1) ? f[(i * VEC + j) / 2].y : f[(i * VEC + j) / 2].x;
+        if (WHOLE || col < d) store(col, v);
+    }
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// WHOLE: x, d_h, d_y and post_weight are there, and the threads' columns are the row's.
+template <typename TR, typename TX, int VEC, bool OWN_GATE, bool WHOLE>
 __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
-    constexpr int NV = kNormElems / VEC;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(16) float red[2][16 * 8];
+    __shared__ __align__(16) float peer_sums[2][8];
+    namespace cg = cooperative_groups;
     const NormArgs& a = k.a;
     const int tid = threadIdx.x, T = blockDim.x, warps = T >> 5;
-    __shared__ __align__(16) float peer_sums[2][8];
     const int64_t width = a.width;
     const int rank = k.cluster > 1 ? (int)(blockIdx.x % k.cluster) : 0;
     const int64_t col0 = (int64_t)rank * k.block_width, worker = blockIdx.x / k.cluster, workers = gridDim.x / k.cluster;
-    const int d = (int)min((int64_t)k.block_width, width - col0);  // columns of this block
-    const int slots = (d + 7) / 8 * 8;
+    const int d = (int)min((int64_t)k.block_width, width - col0);  // columns of this block, counted from col0
+    const int slots = (d + 7) / 8 * 8, c = tid * VEC, stride = T * VEC;
     const float inv_d = 1.0f / (float)width;
-    // columns are counted from the block's first one: rows of `width` from here on
-    const TR *h = static_cast<const TR*>(k.h) + col0, *dh = k.dh != nullptr ? static_cast<const TR*>(k.dh) + col0 : nullptr;
-    const TX *x = k.x != nullptr ? static_cast<const TX*>(k.x) + col0 : nullptr;
-    const TX *dy = k.dy != nullptr ? static_cast<const TX*>(k.dy) + col0 : nullptr;
-    TR* dres = static_cast<TR*>(k.dres) + col0;
-    TX* dx = x != nullptr ? static_cast<TX*>(k.dx) + col0 : nullptr;
+    const bool has_x = WHOLE || k.x != nullptr, has_dh = WHOLE || k.dh != nullptr, has_dy = WHOLE || k.dy != nullptr;
+    const bool has_post = WHOLE || a.post_w != nullptr;
     const int64_t pitch = align_up(width, 8);
+    // a stage: h, dh, x, dy
     const int stage_bytes = slots * 2 * (int)(sizeof(TR) + sizeof(TX));
-    auto stage_h = [&](int s) { return reinterpret_cast<TR*>(smem + s * stage_bytes); };
-    auto stage_dh = [&](int s) { return stage_h(s) + slots; };
-    auto stage_x = [&](int s) { return reinterpret_cast<TX*>(stage_h(s) + 2 * slots); };
-    auto stage_dy = [&](int s) { return stage_x(s) + slots; };
+    auto stage_r = [&](int s, int i) { return reinterpret_cast<TR*>(smem + s * stage_bytes) + i * slots; };
+    auto stage_x = [&](int s, int i) {
+        return reinterpret_cast<TX*>(smem + s * stage_bytes + 2 * slots * (int)sizeof(TR)) + i * slots;
+    };
     auto fetch = [&](int s, int64_t r) {
+        const int64_t at = r * width + col0;
+        const TR *h = static_cast<const TR*>(k.h) + at, *dh = static_cast<const TR*>(k.dh) + at;
+        const TX *x = static_cast<const TX*>(k.x) + at, *dy = static_cast<const TX*>(k.dy) + at;
+        TR *sh = stage_r(s, 0), *sdh = stage_r(s, 1);
+        TX *sx = stage_x(s, 0), *sdy = stage_x(s, 1);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int c = (v * T + tid) * VEC;
-            if (c >= d) break;
-            copy_vec<TR, VEC>(stage_h(s) + c, h + r * width + c);
-            if (x != nullptr) copy_vec<TX, VEC>(stage_x(s) + c, x + r * width + c);
-            if (dh != nullptr) copy_vec<TR, VEC>(stage_dh(s) + c, dh + r * width + c);
-            if (dy != nullptr) copy_vec<TX, VEC>(stage_dy(s) + c, dy + r * width + c);
+        for (int i = 0; i < kNormElems / VEC; ++i) {
+            const int col = c + i * stride;
+            if (!WHOLE && col >= d) break;
+            copy_vec<TR, VEC>(sh + col, h + col);
+            if (has_x) copy_vec<TX, VEC>(sx + col, x + col);
+            if (has_dh) copy_vec<TR, VEC>(sdh + col, dh + col);
+            if (has_dy) copy_vec<TX, VEC>(sdy + col, dy + col);
         }
     };
-    float pre[NV][VEC], post[NV][VEC], sum_b[NV][VEC], sum_pre[NV][VEC];
+    constexpr int Q = kNormElems / 8;
+    float2 pre[Q][4], post[Q][4], sum_b[Q][4], sum_pre[Q][4];
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int q = 0; q < Q; ++q) {
+        get8<VEC, WHOLE>(q, c, stride, d, pre[q], [&](int col, float (&f)[VEC]) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const int c = (v * T + tid) * VEC + j;
-            pre[v][j] = dy != nullptr && c < d ? load_any(a.pre_w, a.w_dtype, col0 + c) : 0.0f;
-            sum_pre[v][j] = 0.0f;
-        }
+            for (int j = 0; j < VEC; ++j) f[j] = has_dy ? load_any(a.pre_w, a.w_dtype, col0 + col + j) : 0.0f;
+        });
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum_pre[q][j] = both(0.0f);
+    }
     int parity = 0;
     for (int64_t u = worker; u < k.units; u += workers) {
         const int64_t g = u / k.units_per_gate, part = u % k.units_per_gate;
@@ -259,16 +294,18 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
             copy_commit();
         }
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+        for (int q = 0; q < Q; ++q) {
+            get8<VEC, WHOLE>(q, c, stride, d, post[q], [&](int col, float (&f)[VEC]) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const int c = (v * T + tid) * VEC + j;
-                float f = x != nullptr && c < d ? a.scale : 0.0f;
-                if (c < d && a.post_w != nullptr) f *= load_any(a.post_w, a.w_dtype, col0 + c);
-                if (c < d && a.gate != nullptr && !OWN_GATE) f *= load_any(a.gate, a.gate_dtype, g * width + col0 + c);
-                post[v][j] = f;  // A of above; with OWN_GATE without the gate
-                sum_b[v][j] = 0.0f;
-            }
+                for (int j = 0; j < VEC; ++j) {
+                    f[j] = has_x ? a.scale : 0.0f;
+                    if (has_post) f[j] *= load_any(a.post_w, a.w_dtype, col0 + col + j);
+                    if (a.gate != nullptr && !OWN_GATE) f[j] *= load_any(a.gate, a.gate_dtype, g * width + col0 + col + j);
+                }
+            });  // A of above; with OWN_GATE without the gate
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum_b[q][j] = both(0.0f);
+        }
         int s = 0;
         for (int64_t r = r0; r < r1; ++r) {
             if (k.stages == 1) {
@@ -281,32 +318,46 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
                 copy_wait<1>();
             else
                 copy_wait<0>();
-            float t[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            const int64_t at = r * width + col0;
+            const TR *sh = stage_r(s, 0), *sdh = stage_r(s, 1);
+            const TX *sx = stage_x(s, 0), *sdy = stage_x(s, 1);
+            auto load_r = [&](int q, const TR* p, bool has, float2 (&f)[4]) {
+                get8<VEC, WHOLE>(q, c, stride, has ? d : 0, f, [&](int col, float (&v)[VEC]) { load_vec<TR, VEC>(p + col, v); });
+            };
+            auto load_x = [&](int q, const TX* p, bool has, float2 (&f)[4]) {
+                get8<VEC, WHOLE>(q, c, stride, has ? d : 0, f, [&](int col, float (&v)[VEC]) { load_vec<TX, VEC>(p + col, v); });
+            };
+            auto load_gate = [&](int q, float2 (&f)[4]) {
+                get8<VEC, WHOLE>(q, c, stride, d, f,
+                          [&](int col, float (&v)[VEC]) { load_any_vec<VEC>(a.gate, a.gate_dtype, at + col, v); });
+            };
+            float2 t2[6] = {};
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const int c = (v * T + tid) * VEC;
-                if (c >= d) break;
-                float hv[VEC], xv[VEC] = {}, dhv[VEC] = {}, dyv[VEC] = {};
-                load_vec<TR, VEC>(stage_h(s) + c, hv);
-                if (x != nullptr) load_vec<TX, VEC>(stage_x(s) + c, xv);
-                if (dh != nullptr) load_vec<TR, VEC>(stage_dh(s) + c, dhv);
-                if (dy != nullptr) load_vec<TX, VEC>(stage_dy(s) + c, dyv);
+            for (int q = 0; q < Q; ++q) {
+                float2 h[4], x[4], dh[4], dy[4], gate[4];
+                load_r(q, sh, true, h);
+                load_x(q, sx, has_x, x);
+                load_r(q, sdh, has_dh, dh);
+                load_x(q, sdy, has_dy, dy);
+                if (OWN_GATE) load_gate(q, gate);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float dn = dyv[j] * pre[v][j];
-                    float ax = post[v][j] * xv[j];
-                    if (OWN_GATE) ax *= load_any(a.gate, a.gate_dtype, r * width + col0 + c + j);
-                    t[0] += hv[j] * hv[j];
-                    t[1] += xv[j] * xv[j];
-                    t[2] += dn * hv[j];
-                    t[3] += ax * dhv[j];
-                    t[4] += ax * dn;
-                    t[5] += ax * hv[j];
+                for (int j = 0; j < 4; ++j) {
+                    const float2 dn = __fmul2_rn(dy[j], pre[q][j]);
+                    float2 ax = __fmul2_rn(post[q][j], x[j]);
+                    if (OWN_GATE) ax = __fmul2_rn(ax, gate[j]);
+                    t2[0] = __ffma2_rn(h[j], h[j], t2[0]);
+                    t2[1] = __ffma2_rn(x[j], x[j], t2[1]);
+                    t2[2] = __ffma2_rn(dn, h[j], t2[2]);
+                    t2[3] = __ffma2_rn(ax, dh[j], t2[3]);
+                    t2[4] = __ffma2_rn(ax, dn, t2[4]);
+                    t2[5] = __ffma2_rn(ax, h[j], t2[5]);
                 }
             }
+            float t[8] = {};
+#pragma unroll
+            for (int i = 0; i < 6; ++i) t[i] = t2[i].x + t2[i].y;
             sum8(t, red[parity], warps);
             if (k.cluster > 1) {
-                namespace cg = cooperative_groups;
                 cg::cluster_group cluster = cg::this_cluster();
                 if (tid == 0)
 #pragma unroll
@@ -322,64 +373,74 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
             }
             parity ^= 1;
             // every thread has left the previous row: its stage takes the row stages - 1 ahead
-            const int free_stage = s == 0 ? k.stages - 1 : s - 1;
             if (k.stages > 1) {
+                const int free_stage = s == 0 ? k.stages - 1 : s - 1;
                 if (r + k.stages - 1 < r1) fetch(free_stage, r + k.stages - 1);
                 copy_commit();
             }
             const float rh = rsqrtf(t[0] * inv_d + a.eps);
             const float m1 = t[2] * rh * inv_d;
             float rx = 1.0f, m2 = 0.0f;
-            if (a.post_w != nullptr) {
+            if (has_post) {
                 rx = rsqrtf(t[1] * inv_d + a.eps);
                 m2 = rx * inv_d * (t[3] + rh * (t[4] - rh * m1 * t[5]));
             }
+            const float2 minus_m1 = both(-m1), minus_m2 = both(-m2), rh2 = both(rh), rx2 = both(rx);
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const int c = (v * T + tid) * VEC;
-                if (c >= d) break;
-                float hv[VEC], xv[VEC] = {}, ev[VEC] = {}, dyv[VEC] = {};
-                load_vec<TR, VEC>(stage_h(s) + c, hv);
-                if (x != nullptr) load_vec<TX, VEC>(stage_x(s) + c, xv);
-                if (dh != nullptr) load_vec<TR, VEC>(stage_dh(s) + c, ev);
-                if (dy != nullptr) load_vec<TX, VEC>(stage_dy(s) + c, dyv);
-                float dxv[VEC], dgv[VEC];
+            for (int q = 0; q < Q; ++q) {
+                float2 h[4], x[4], e[4], dy[4], gate[4];
+                load_r(q, sh, true, h);
+                load_x(q, sx, has_x, x);
+                load_r(q, sdh, has_dh, e);
+                load_x(q, sdy, has_dy, dy);
+                if (OWN_GATE) load_gate(q, gate);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float n = hv[j] * rh, q = xv[j] * rx;
-                    ev[j] += rh * (dyv[j] * pre[v][j] - n * m1);
-                    float gate = 1.0f;
-                    if (OWN_GATE) gate = load_any(a.gate, a.gate_dtype, r * width + col0 + c + j);
-                    const float dq = post[v][j] * gate * ev[j];
-                    dxv[j] = rx * (dq - q * m2);
-                    dgv[j] = post[v][j] * ev[j] * q;
-                    sum_b[v][j] += ev[j] * gate * q;
-                    sum_pre[v][j] += dyv[j] * n;
+                for (int j = 0; j < 4; ++j) {
+                    const float2 n = __fmul2_rn(h[j], rh2), p = __fmul2_rn(x[j], rx2);
+                    e[j] = __ffma2_rn(rh2, __ffma2_rn(n, minus_m1, __fmul2_rn(dy[j], pre[q][j])), e[j]);
+                    float2 dq = __fmul2_rn(post[q][j], e[j]);
+                    if (OWN_GATE) {
+                        dy[j] = __fmul2_rn(dy[j], n);
+                        sum_pre[q][j] = __fadd2_rn(sum_pre[q][j], dy[j]);
+                        dy[j] = __fmul2_rn(dq, p);  // d_gate
+                        dq = __fmul2_rn(dq, gate[j]);
+                        sum_b[q][j] = __ffma2_rn(__fmul2_rn(e[j], gate[j]), p, sum_b[q][j]);
+                    } else {
+                        sum_pre[q][j] = __ffma2_rn(dy[j], n, sum_pre[q][j]);
+                        sum_b[q][j] = __ffma2_rn(e[j], p, sum_b[q][j]);
+                    }
+                    x[j] = __fmul2_rn(rx2, __ffma2_rn(p, minus_m2, dq));  // d_x
                 }
-                store_global<TR, VEC>(dres + r * width + c, ev);
-                if (x != nullptr) store_global<TX, VEC>(dx + r * width + c, dxv);
+                put8<VEC, WHOLE>(q, c, stride, d, e, [&](int col, const float (&v)[VEC]) {
+                    store_global<TR, VEC>(static_cast<TR*>(k.dres) + at + col, v);
+                });
+                if (has_x)
+                    put8<VEC, WHOLE>(q, c, stride, d, x, [&](int col, const float (&v)[VEC]) {
+                        store_global<TX, VEC>(static_cast<TX*>(k.dx) + at + col, v);
+                    });
                 if (OWN_GATE)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) store_any(k.dgate, a.gate_dtype, r * width + col0 + c + j, dgv[j]);
+                    put8<VEC, WHOLE>(q, c, stride, d, dy, [&](int col, const float (&v)[VEC]) {
+                        store_any_vec<VEC>(k.dgate, a.gate_dtype, at + col, v);
+                    });
             }
             s = s == k.stages - 1 ? 0 : s + 1;
         }
         copy_wait<0>();
         if (warps > 1) __syncthreads();  // the next unit fills the stages again
-        if (x != nullptr)
+        if (has_x)
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const int c = (v * T + tid) * VEC;
-                if (c < d) store_global<float, VEC>(k.part_b + u * pitch + col0 + c, sum_b[v]);
-            }
+            for (int q = 0; q < Q; ++q)
+                put8<VEC, WHOLE>(q, c, stride, d, sum_b[q], [&](int col, const float (&v)[VEC]) {
+                    store_global<float, VEC>(k.part_b + u * pitch + col0 + col, v);
+                });
     }
-    if (dy != nullptr)
+    if (has_dy)
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int c = (v * T + tid) * VEC;
-            if (c < d) store_global<float, VEC>(k.part_pre + worker * pitch + col0 + c, sum_pre[v]);
-        }
-    if (k.cluster > 1) cooperative_groups::this_cluster().sync();  // a peer may still read this block's sums
+        for (int q = 0; q < Q; ++q)
+            put8<VEC, WHOLE>(q, c, stride, d, sum_pre[q], [&](int col, const float (&v)[VEC]) {
+                store_global<float, VEC>(k.part_pre + worker * pitch + col0 + col, v);
+            });
+    if (k.cluster > 1) cg::this_cluster().sync();  // a peer may still read this block's sums
 }
 
 // Sums of `count` consecutive rows of `part` (width columns, rows align_up(width, 8)
@@ -598,7 +659,7 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
     k.units_per_gate = p.units_per_gate;
     k.cluster = p.shape.cluster;
     k.block_width = p.shape.block_width;
-    const int64_t rb = dtype_bytes(res_dtype), xb = dtype_bytes(act_dtype);
+    const int64_t rb = dtype_bytes(res_dtype), xb = dtype_bytes(act_dtype), gb = dtype_bytes(gate_dtype);
     const int stage = (int)(align_up(p.shape.block_width, 8) * 2 * (rb + xb));
     // as many blocks an SM as the registers admit where each of them has two stages, else
     // as many stages as fit for one block
@@ -610,7 +671,8 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
         if (width % vec != 0) return false;
         const int64_t ar = std::min<int64_t>(32, vec * rb), ax = std::min<int64_t>(32, vec * xb);
         return aligned_to(h, ar) && aligned_to(d_h, ar) && aligned_to(d_residual, ar) && aligned_to(x, ax) &&
-               aligned_to(d_y, ax) && aligned_to(d_x, ax);
+               aligned_to(d_y, ax) && aligned_to(d_x, ax) &&
+               (!own || (aligned_to(gate, std::min<int64_t>(32, vec * gb)) && aligned_to(d_gate, std::min<int64_t>(32, vec * gb))));
     };
     const int rc = with_norm_types(res_dtype, act_dtype, [&](auto tr, auto tx) {
         using TR = decltype(tr);
@@ -632,9 +694,15 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
             CRESSO_LAUNCHED("norm_grad_kernel");
             return (int)CRESSO_OK;
         };
-        if (fits(8)) return own ? launch(norm_grad_kernel<TR, TX, 8, true>) : launch(norm_grad_kernel<TR, TX, 8, false>);
-        if (fits(2)) return own ? launch(norm_grad_kernel<TR, TX, 2, true>) : launch(norm_grad_kernel<TR, TX, 2, false>);
-        return own ? launch(norm_grad_kernel<TR, TX, 1, true>) : launch(norm_grad_kernel<TR, TX, 1, false>);
+        if (fits(8)) {
+            const bool whole = x != nullptr && d_h != nullptr && d_y != nullptr && post_weight != nullptr &&
+                               p.shape.cluster == 1 && width == (int64_t)p.shape.threads * kNormElems;
+            if (whole && !own) return launch(norm_grad_kernel<TR, TX, 8, false, true>);
+            return own ? launch(norm_grad_kernel<TR, TX, 8, true, false>) : launch(norm_grad_kernel<TR, TX, 8, false, false>);
+        }
+        if (fits(2))
+            return own ? launch(norm_grad_kernel<TR, TX, 2, true, false>) : launch(norm_grad_kernel<TR, TX, 2, false, false>);
+        return own ? launch(norm_grad_kernel<TR, TX, 1, true, false>) : launch(norm_grad_kernel<TR, TX, 1, false, false>);
     });
     if (rc != CRESSO_OK) return rc;
     auto columns = [&](const float* part, int64_t count, int64_t grp, int which, void* out, void* dgate) {

@@ -223,6 +223,16 @@ __device__ __forceinline__ void load_any_vec(const void* p, int dtype, int64_t i
         load_global<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(p) + i, f);
 }
 
+template <int VEC>
+__device__ __forceinline__ void store_any_vec(void* p, int dtype, int64_t i, const float (&f)[VEC]) {
+    if (dtype == CRESSO_DTYPE_F32)
+        store_global<float, VEC>(static_cast<float*>(p) + i, f);
+    else if (dtype == CRESSO_DTYPE_F16)
+        store_global<__half, VEC>(static_cast<__half*>(p) + i, f);
+    else
+        store_global<__nv_bfloat16, VEC>(static_cast<__nv_bfloat16*>(p) + i, f);
+}
+
 // Asynchronous copy of VEC elements from global to shared memory in 16-, 8- or 4-byte
 // pieces, counted by copy_commit / copy_wait; 2-byte pieces are copied at once.
 template <typename T, int VEC>
