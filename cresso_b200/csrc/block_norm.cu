@@ -13,6 +13,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cresso {
 
@@ -36,7 +37,7 @@ static NormShape norm_shape(int64_t width) {
     NormShape p{};
     p.cluster = pow2_ceil(ceil_div(width, kNormBlockWidth));
     p.block_width = (int)(p.cluster > 1 ? align_up(ceil_div(width, p.cluster), 8) : width);
-    p.threads = std::max(32, pow2_ceil(ceil_div(p.block_width, kNormElems)));
+    p.threads = (int)align_up(ceil_div(p.block_width, kNormElems), 32);
     return p;
 }
 
@@ -86,8 +87,25 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __re
         if (x != nullptr) load_global<TX, VEC>(x + at + c, xv[v]);
         load_global<TR, VEC>(res + at + c, hv[v]);
     }
+    // v *= an array's values at the thread's columns; all its loads are in flight together
+    auto multiply = [&](float (&v)[NV][VEC], const void* p, int dtype, int64_t from) {
+        with_any(p, dtype, [&](auto* w) {
+            using T0 = std::remove_cv_t<std::remove_pointer_t<decltype(w)>>;
+            float f[NV][VEC];
+#pragma unroll
+            for (int v0 = 0; v0 < NV; ++v0) {
+                const int c = (v0 * T + tid) * VEC;
+                if (c < d) load_global<T0, VEC>(w + from + c, f[v0]);
+            }
+#pragma unroll
+            for (int v0 = 0; v0 < NV; ++v0)
+                if ((v0 * T + tid) * VEC < d)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[v0][j] *= f[v0][j];
+        });
+    };
     if (x != nullptr) {
-        float rx = 1.0f;
+        float rx = a.scale;
         if (a.post_w != nullptr) {
             float s = 0.0f;
 #pragma unroll
@@ -96,26 +114,16 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __re
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) s += xv[v][j] * xv[v][j];
             }
-            rx = rsqrtf(row_sum(s, 0) * inv_d + a.eps);
+            multiply(xv, a.post_w, a.w_dtype, col0);  // on the way while the sum is formed
+            rx *= rsqrtf(row_sum(s, 0) * inv_d + a.eps);
         }
-        const int64_t g0 = a.gate != nullptr ? t / a.rows_per_gate * width + col0 : 0;
+        if (a.gate != nullptr) multiply(xv, a.gate, a.gate_dtype, t / a.rows_per_gate * width + col0);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = (v * T + tid) * VEC;
             if (c >= d) break;
-            float f[VEC];
-            if (a.post_w != nullptr) {
-                load_any_vec<VEC>(a.post_w, a.w_dtype, col0 + c, f);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) xv[v][j] *= rx * f[j];
-            }
-            if (a.gate != nullptr) {
-                load_any_vec<VEC>(a.gate, a.gate_dtype, g0 + c, f);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) xv[v][j] *= f[j];
-            }
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) hv[v][j] += a.scale * xv[v][j];
+            for (int j = 0; j < VEC; ++j) hv[v][j] += rx * xv[v][j];
             store_global<TR, VEC>(h + at + c, hv[v]);
         }
     }
@@ -127,16 +135,15 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __re
 #pragma unroll
             for (int j = 0; j < VEC; ++j) s += hv[v][j] * hv[v][j];
         }
+        multiply(hv, a.pre_w, a.w_dtype, col0);
         const float rh = rsqrtf(row_sum(s, 1) * inv_d + a.eps);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int c = (v * T + tid) * VEC;
             if (c >= d) break;
-            float f[VEC];
-            load_any_vec<VEC>(a.pre_w, a.w_dtype, col0 + c, f);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) f[j] *= hv[v][j] * rh;
-            store_global<TX, VEC>(y + at + c, f);
+            for (int j = 0; j < VEC; ++j) hv[v][j] *= rh;
+            store_global<TX, VEC>(y + at + c, hv[v]);
         }
     }
     if (cluster > 1) cg::this_cluster().sync();  // a peer may still read this block's sums
@@ -275,15 +282,30 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
     };
     constexpr int Q = kNormElems / 8;
     float2 pre[Q][4], post[Q][4], sum_b[Q][4], sum_pre[Q][4];
+    // factors of the thread's columns: v = 1, then v *= each array
+    auto factors = [&](float2 (&v)[Q][4], float start) {
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-        get8<VEC, WHOLE>(q, c, stride, d, pre[q], [&](int col, float (&f)[VEC]) {
+        for (int q = 0; q < Q; ++q)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) f[j] = has_dy ? load_any(a.pre_w, a.w_dtype, col0 + col + j) : 0.0f;
+            for (int j = 0; j < 4; ++j) v[q][j] = both(start);
+    };
+    auto multiply = [&](float2 (&v)[Q][4], const void* p, int dtype, int64_t at) {
+        with_any(p, dtype, [&](auto* w) {
+            using T0 = std::remove_cv_t<std::remove_pointer_t<decltype(w)>>;
+            float2 f[Q][4];
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+                get8<VEC, WHOLE>(q, c, stride, d, f[q],
+                                 [&](int col, float (&x)[VEC]) { load_global<T0, VEC>(w + at + col, x); });
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[q][j] = __fmul2_rn(v[q][j], f[q][j]);
         });
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum_pre[q][j] = both(0.0f);
-    }
+    };
+    factors(pre, has_dy ? 1.0f : 0.0f);
+    if (has_dy) multiply(pre, a.pre_w, a.w_dtype, col0);
+    factors(sum_pre, 0.0f);
     int parity = 0;
     for (int64_t u = worker; u < k.units; u += workers) {
         const int64_t g = u / k.units_per_gate, part = u % k.units_per_gate;
@@ -293,19 +315,10 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
             if (r0 + i < r1) fetch(i, r0 + i);
             copy_commit();
         }
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            get8<VEC, WHOLE>(q, c, stride, d, post[q], [&](int col, float (&f)[VEC]) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    f[j] = has_x ? a.scale : 0.0f;
-                    if (has_post) f[j] *= load_any(a.post_w, a.w_dtype, col0 + col + j);
-                    if (a.gate != nullptr && !OWN_GATE) f[j] *= load_any(a.gate, a.gate_dtype, g * width + col0 + col + j);
-                }
-            });  // A of above; with OWN_GATE without the gate
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sum_b[q][j] = both(0.0f);
-        }
+        factors(post, has_x ? a.scale : 0.0f);  // A of above; with OWN_GATE without the gate
+        if (has_post) multiply(post, a.post_w, a.w_dtype, col0);
+        if (a.gate != nullptr && !OWN_GATE) multiply(post, a.gate, a.gate_dtype, g * width + col0);
+        factors(sum_b, 0.0f);
         int s = 0;
         for (int64_t r = r0; r < r1; ++r) {
             if (k.stages == 1) {
@@ -670,9 +683,11 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
     auto fits = [&](int vec) {
         if (width % vec != 0) return false;
         const int64_t ar = std::min<int64_t>(32, vec * rb), ax = std::min<int64_t>(32, vec * xb);
+        const int64_t ag = std::min<int64_t>(32, vec * gb), aw = std::min<int64_t>(32, vec * dtype_bytes(weight_dtype));
         return aligned_to(h, ar) && aligned_to(d_h, ar) && aligned_to(d_residual, ar) && aligned_to(x, ax) &&
                aligned_to(d_y, ax) && aligned_to(d_x, ax) &&
-               (!own || (aligned_to(gate, std::min<int64_t>(32, vec * gb)) && aligned_to(d_gate, std::min<int64_t>(32, vec * gb))));
+               aligned_to(gate, ag) && (!own || aligned_to(d_gate, ag)) && aligned_to(post_weight, aw) &&
+               aligned_to(pre_weight, aw);
     };
     const int rc = with_norm_types(res_dtype, act_dtype, [&](auto tr, auto tx) {
         using TR = decltype(tr);

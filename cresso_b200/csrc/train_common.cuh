@@ -212,6 +212,17 @@ __device__ __forceinline__ void store_global(T* p, const float (&f)[VEC]) {
     u.store(p);
 }
 
+// f(p) with a pointer of the array's run-time type: one uniform branch for all its loads.
+template <typename F>
+__device__ __forceinline__ void with_any(const void* p, int dtype, F f) {
+    if (dtype == CRESSO_DTYPE_F32)
+        f(static_cast<const float*>(p));
+    else if (dtype == CRESSO_DTYPE_F16)
+        f(static_cast<const __half*>(p));
+    else
+        f(static_cast<const __nv_bfloat16*>(p));
+}
+
 // VEC elements of an array whose type is only known at run time; the branch is uniform.
 template <int VEC>
 __device__ __forceinline__ void load_any_vec(const void* p, int dtype, int64_t i, float (&f)[VEC]) {
