@@ -24,34 +24,36 @@ struct NormArgs {
     float scale, eps;
 };
 
-constexpr int kNormElems = 16;                         // columns of a thread
-constexpr int kNormBlockWidth = 512 * kNormElems;      // columns of a block
-constexpr int kNormMaxWidth = CRESSO_TRAIN_MAX_NORM_WIDTH;  // columns of a cluster of 8
+constexpr int kNormMaxWidth = CRESSO_TRAIN_MAX_NORM_WIDTH;
 
-// Blocks and threads of a row: a row of more than 8192 columns is cut over a cluster of 2 to 8
-// blocks, which add their sums through distributed shared memory.
+// Columns of a thread (EL, 16 or 8), threads and blocks of a row: a row of more than 512 EL
+// columns is cut over a cluster of 2 to 8 blocks, which add their sums through distributed
+// shared memory.
 struct NormShape {
-    int threads, cluster, block_width;
+    int elems, threads, cluster, block_width;
 };
-static NormShape norm_shape(int64_t width) {
+static NormShape norm_shape(int64_t width, int elems) {
     NormShape p{};
-    p.cluster = pow2_ceil(ceil_div(width, kNormBlockWidth));
+    p.elems = width > 512 * 8 ? 16 : elems;
+    p.cluster = pow2_ceil(ceil_div(width, 512 * p.elems));
     p.block_width = (int)(p.cluster > 1 ? align_up(ceil_div(width, p.cluster), 8) : width);
-    p.threads = (int)align_up(ceil_div(p.block_width, kNormElems), 32);
+    p.threads = (int)align_up(ceil_div(p.block_width, p.elems), 32);
     return p;
 }
+// Few rows are a matter of latency, for which 8 columns a thread are better: one row of 4096
+// takes 4.2 us instead of 6.2, and 16384 rows 142 us instead of 139.
+constexpr int64_t kNormFewRows = 8 * 148;
 
 // ----------------------------------------------------------------- forward ---
 //
-// A row lies in the registers of a block (of a warp up to 512 columns, four rows a block), 16
-// columns a thread: x and residual are read once, h and y written once, two reductions between.
+// A row lies in the registers of a block (of a warp up to 512 columns, four rows a block): x and residual are read once, h and y written once, two reductions between.
 // Weights and gate come from L1 for every row.  Many small blocks an SM, each at another point
 // of its row, keep the memory busy without any staging.
-template <typename TR, typename TX, int VEC>
+template <typename TR, typename TX, int VEC, int EL>
 __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __restrict__ res,
                                                       const TX* __restrict__ x, TR* __restrict__ h,
                                                       TX* __restrict__ y, int cluster, int block_width) {
-    constexpr int NV = kNormElems / VEC;
+    constexpr int NV = EL / VEC;
     namespace cg = cooperative_groups;
     __shared__ float red[2][32], peer[2];
     const int64_t width = a.width;
@@ -241,8 +243,9 @@ __device__ __forceinline__ void put8(int chunk, int c, int stride, int d, const 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // WHOLE: x, d_h, d_y and post_weight are there, and the threads' columns are the row's.
-template <typename TR, typename TX, int VEC, bool OWN_GATE, bool WHOLE>
+template <typename TR, typename TX, int VEC, int EL, bool OWN_GATE, bool WHOLE>
 __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
+    next_kernel_may_start();
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(16) float red[2][16 * 8];
     __shared__ __align__(16) float peer_sums[2][8];
@@ -271,7 +274,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
         TR *sh = stage_r(s, 0), *sdh = stage_r(s, 1);
         TX *sx = stage_x(s, 0), *sdy = stage_x(s, 1);
 #pragma unroll
-        for (int i = 0; i < kNormElems / VEC; ++i) {
+        for (int i = 0; i < EL / VEC; ++i) {
             const int col = c + i * stride;
             if (!WHOLE && col >= d) break;
             copy_vec<TR, VEC>(sh + col, h + col);
@@ -280,7 +283,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
             if (has_dy) copy_vec<TX, VEC>(sdy + col, dy + col);
         }
     };
-    constexpr int Q = kNormElems / 8;
+    constexpr int Q = EL / 8;
     float2 pre[Q][4], post[Q][4], sum_b[Q][4], sum_pre[Q][4];
     // factors of the thread's columns: v = 1, then v *= each array
     auto factors = [&](float2 (&v)[Q][4], float start) {
@@ -469,8 +472,12 @@ struct NormColumns {
     float* post_rows;
 };
 
-__global__ void __launch_bounds__(kThreads) norm_columns_kernel(NormArgs a, NormColumns k) {
+// Two such jobs in one launch, blockIdx.z apart.
+__global__ void __launch_bounds__(kThreads) norm_columns_kernel(NormArgs a, NormColumns first, NormColumns second) {
     __shared__ float sh[kWarps][32];
+    const NormColumns& k = blockIdx.z == 0 ? first : second;
+    next_kernel_may_start();
+    previous_kernel_done();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane, d = a.width, pitch = align_up(d, 8);
     for (int64_t g = blockIdx.y; g < k.groups; g += gridDim.y) {
@@ -510,9 +517,9 @@ struct NormGradPlan {
     int64_t workers, units, units_per_gate;  // workers: blocks or clusters
     int64_t off_b, off_pre, off_post, bytes;
 };
-static NormGradPlan norm_grad_plan(int64_t n, int64_t width, int64_t gate_rows) {
+static NormGradPlan norm_grad_plan(int64_t n, int64_t width, int64_t gate_rows, int elems) {
     NormGradPlan p{};
-    p.shape = norm_shape(width);
+    p.shape = norm_shape(width, elems);
     const int64_t want = 148 * std::max(1, 512 / p.shape.threads) / p.shape.cluster;
     const bool own = gate_rows == n && n > 1;
     const int64_t groups = own || gate_rows < 1 ? 1 : gate_rows;
@@ -574,7 +581,7 @@ int cresso_block_norm(const void* residual, const void* x, const void* post_weig
     NvtxRange range("block_norm n=%lld", (long long)n);
     const NormArgs a{post_weight, pre_weight, gate, n, width, gate != nullptr ? n / gate_rows : n,
                      (int)weight_dtype, (int)gate_dtype, (float)scale, (float)eps};
-    const NormShape p = norm_shape(width);
+    const NormShape p = norm_shape(width, n < kNormFewRows ? 8 : 16);
     const int64_t rb = dtype_bytes(res_dtype), xb = dtype_bytes(act_dtype), wb = dtype_bytes(weight_dtype),
                   gb = dtype_bytes(gate_dtype);
     // the widest accesses that the width and the addresses allow
@@ -603,9 +610,13 @@ int cresso_block_norm(const void* residual, const void* x, const void* post_weig
             CRESSO_LAUNCHED("norm_kernel");
             return (int)CRESSO_OK;
         };
-        if (fits(8)) return launch(norm_kernel<TR, TX, 8>);
-        if (fits(2)) return launch(norm_kernel<TR, TX, 2>);
-        return launch(norm_kernel<TR, TX, 1>);
+        if (p.elems == 8)
+            return fits(8)   ? launch(norm_kernel<TR, TX, 8, 8>)
+                   : fits(2) ? launch(norm_kernel<TR, TX, 2, 8>)
+                             : launch(norm_kernel<TR, TX, 1, 8>);
+        return fits(8)   ? launch(norm_kernel<TR, TX, 8, 16>)
+               : fits(2) ? launch(norm_kernel<TR, TX, 2, 16>)
+                         : launch(norm_kernel<TR, TX, 1, 16>);
     });
 }
 
@@ -613,7 +624,9 @@ int cresso_block_norm_grad_scratch_bytes(int64_t n, int64_t width, int64_t gate_
     CRESSO_REQUIRE(bytes != nullptr, CRESSO_EINVAL, "block_norm_grad_scratch_bytes: NULL result");
     CRESSO_REQUIRE(n >= 0 && width >= 0 && gate_rows >= 0, CRESSO_EINVAL, "block_norm_grad: negative size");
     CRESSO_REQUIRE(width <= kNormMaxWidth, CRESSO_EUNSUPPORTED, "block_norm_grad: width above %d", kNormMaxWidth);
-    *bytes = n == 0 || width == 0 ? 0 : norm_grad_plan(n, width, gate_rows).bytes;
+    *bytes = n == 0 || width == 0 ? 0
+                                   : std::max(norm_grad_plan(n, width, gate_rows, 8).bytes,
+                                              norm_grad_plan(n, width, gate_rows, 16).bytes);
     return CRESSO_OK;
 }
 
@@ -647,13 +660,26 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
     CRESSO_REQUIRE((x != nullptr) == (d_x != nullptr) && (post_weight != nullptr) == (d_post_weight != nullptr) &&
                        (d_y != nullptr) == (d_pre_weight != nullptr) && (gate != nullptr) == (d_gate != nullptr),
                    CRESSO_EINVAL, "block_norm_grad: an input without its gradient, or a gradient without its input");
-    const NormGradPlan p = norm_grad_plan(n, width, gate != nullptr ? gate_rows : 0);
+    const bool own = gate != nullptr && gate_rows == n && n > 1;
+    const int64_t rb = dtype_bytes(res_dtype), xb = dtype_bytes(act_dtype), gb = dtype_bytes(gate_dtype);
+    // the widest accesses that the width and the addresses allow
+    auto fits = [&](int vec) {
+        if (width % vec != 0) return false;
+        const int64_t ar = std::min<int64_t>(32, vec * rb), ax = std::min<int64_t>(32, vec * xb);
+        const int64_t ag = std::min<int64_t>(32, vec * gb), aw = std::min<int64_t>(32, vec * dtype_bytes(weight_dtype));
+        return aligned_to(h, ar) && aligned_to(d_h, ar) && aligned_to(d_residual, ar) && aligned_to(x, ax) &&
+               aligned_to(d_y, ax) && aligned_to(d_x, ax) && aligned_to(gate, ag) && (!own || aligned_to(d_gate, ag)) &&
+               aligned_to(post_weight, aw) && aligned_to(pre_weight, aw);
+    };
+    const int vec = fits(8) ? 8 : fits(2) ? 2 : 1;
+    // narrow accesses cost instructions and registers: 8 columns a thread (1023 rows of 2050
+    // float16: 34 us instead of 51)
+    const NormGradPlan p = norm_grad_plan(n, width, gate != nullptr ? gate_rows : 0, vec < 8 || n < kNormFewRows ? 8 : 16);
     CRESSO_REQUIRE(scratch != nullptr && scratch_bytes >= p.bytes, CRESSO_ESCRATCH,
                    "block_norm_grad: scratch has %lld bytes, %lld are needed", (long long)scratch_bytes,
                    (long long)p.bytes);
     CRESSO_REQUIRE(aligned_to(scratch, 32), CRESSO_EINVAL, "block_norm_grad: scratch is not 32-byte aligned");
     NvtxRange range("block_norm_grad n=%lld", (long long)n);
-    const bool own = gate != nullptr && gate_rows == n && n > 1;
     const int64_t groups = gate == nullptr || own ? 1 : gate_rows;
     NormGrad k{};
     k.a = NormArgs{post_weight, pre_weight, gate, n, width, n / groups, (int)weight_dtype, (int)gate_dtype,
@@ -672,23 +698,12 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
     k.units_per_gate = p.units_per_gate;
     k.cluster = p.shape.cluster;
     k.block_width = p.shape.block_width;
-    const int64_t rb = dtype_bytes(res_dtype), xb = dtype_bytes(act_dtype), gb = dtype_bytes(gate_dtype);
     const int stage = (int)(align_up(p.shape.block_width, 8) * 2 * (rb + xb));
     // as many blocks an SM as the registers admit where each of them has two stages, else
     // as many stages as fit for one block
     const int share = 220 * 1024 / std::max(1, 512 / p.shape.threads) - 2048;
     k.stages = 2 * stage <= share ? std::min(4, share / stage) : std::min(4, 220 * 1024 / stage);
     const int smem = k.stages * stage;
-    // the widest accesses that the width and the addresses allow
-    auto fits = [&](int vec) {
-        if (width % vec != 0) return false;
-        const int64_t ar = std::min<int64_t>(32, vec * rb), ax = std::min<int64_t>(32, vec * xb);
-        const int64_t ag = std::min<int64_t>(32, vec * gb), aw = std::min<int64_t>(32, vec * dtype_bytes(weight_dtype));
-        return aligned_to(h, ar) && aligned_to(d_h, ar) && aligned_to(d_residual, ar) && aligned_to(x, ax) &&
-               aligned_to(d_y, ax) && aligned_to(d_x, ax) &&
-               aligned_to(gate, ag) && (!own || aligned_to(d_gate, ag)) && aligned_to(post_weight, aw) &&
-               aligned_to(pre_weight, aw);
-    };
     const int rc = with_norm_types(res_dtype, act_dtype, [&](auto tr, auto tx) {
         using TR = decltype(tr);
         using TX = decltype(tx);
@@ -709,35 +724,40 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
             CRESSO_LAUNCHED("norm_grad_kernel");
             return (int)CRESSO_OK;
         };
-        if (fits(8)) {
+        if (vec == 8 && p.shape.elems == 16) {
             const bool whole = x != nullptr && d_h != nullptr && d_y != nullptr && post_weight != nullptr &&
-                               p.shape.cluster == 1 && width == (int64_t)p.shape.threads * kNormElems;
-            if (whole && !own) return launch(norm_grad_kernel<TR, TX, 8, false, true>);
-            return own ? launch(norm_grad_kernel<TR, TX, 8, true, false>) : launch(norm_grad_kernel<TR, TX, 8, false, false>);
+                               p.shape.cluster == 1 && width == (int64_t)p.shape.threads * 16;
+            if (whole && !own) return launch(norm_grad_kernel<TR, TX, 8, 16, false, true>);
+            return own ? launch(norm_grad_kernel<TR, TX, 8, 16, true, false>)
+                       : launch(norm_grad_kernel<TR, TX, 8, 16, false, false>);
         }
-        if (fits(2))
-            return own ? launch(norm_grad_kernel<TR, TX, 2, true, false>) : launch(norm_grad_kernel<TR, TX, 2, false, false>);
-        return own ? launch(norm_grad_kernel<TR, TX, 1, true, false>) : launch(norm_grad_kernel<TR, TX, 1, false, false>);
+        if (vec == 8)
+            return own ? launch(norm_grad_kernel<TR, TX, 8, 8, true, false>) : launch(norm_grad_kernel<TR, TX, 8, 8, false, false>);
+        if (p.shape.elems == 16)  // a row wider than 4096
+            return own ? launch(norm_grad_kernel<TR, TX, 1, 16, true, false>)
+                       : launch(norm_grad_kernel<TR, TX, 1, 16, false, false>);
+        if (vec == 2)
+            return own ? launch(norm_grad_kernel<TR, TX, 2, 8, true, false>) : launch(norm_grad_kernel<TR, TX, 2, 8, false, false>);
+        return own ? launch(norm_grad_kernel<TR, TX, 1, 8, true, false>) : launch(norm_grad_kernel<TR, TX, 1, 8, false, false>);
     });
     if (rc != CRESSO_OK) return rc;
-    auto columns = [&](const float* part, int64_t count, int64_t grp, int which, void* out, void* dgate) {
-        NormColumns c{part, count, grp, which, out, dgate, reinterpret_cast<float*>(base + p.off_post)};
-        NormArgs args = k.a;
-        if (own) args.gate = nullptr;
-        const dim3 grid((unsigned)ceil_div(width, 32), (unsigned)std::min<int64_t>(65535, grp));
-        norm_columns_kernel<<<grid, kThreads, 0, s>>>(args, c);
+    float* post_rows = reinterpret_cast<float*>(base + p.off_post);
+    NormArgs args = k.a;
+    if (own) args.gate = nullptr;
+    const bool sum_b = post_weight != nullptr || (gate != nullptr && !own), sum_pre = d_y != nullptr;
+    const NormColumns job_b{k.part_b, p.units_per_gate, groups, 0, d_post_weight, own ? nullptr : d_gate, post_rows};
+    const NormColumns job_pre{k.part_pre, p.workers, 1, 1, d_pre_weight, nullptr, nullptr};
+    const unsigned blocks = (unsigned)ceil_div(width, 32);
+    if (sum_b || sum_pre) {
+        const dim3 grid(blocks, sum_b ? (unsigned)std::min<int64_t>(65535, groups) : 1, sum_b && sum_pre ? 2 : 1);
+        CRESSO_CUDA(launch_overlapped(norm_columns_kernel, grid, kThreads, 0, s, args, sum_b ? job_b : job_pre, job_pre));
         CRESSO_LAUNCHED("norm_columns_kernel");
-        return (int)CRESSO_OK;
-    };
-    if (post_weight != nullptr || (gate != nullptr && !own)) {
-        const int r1 = columns(k.part_b, p.units_per_gate, groups, 0, d_post_weight, own ? nullptr : d_gate);
-        if (r1 != CRESSO_OK) return r1;
-        if (post_weight != nullptr && groups > 1) {
-            const int r2 = columns(reinterpret_cast<float*>(base + p.off_post), groups, 1, 2, d_post_weight, nullptr);
-            if (r2 != CRESSO_OK) return r2;
-        }
     }
-    if (d_y != nullptr) return columns(k.part_pre, p.workers, 1, 1, d_pre_weight, nullptr);
+    if (post_weight != nullptr && groups > 1) {  // the groups' rows to one
+        const NormColumns job{post_rows, groups, 1, 2, d_post_weight, nullptr, nullptr};
+        CRESSO_CUDA(launch_overlapped(norm_columns_kernel, dim3(blocks), kThreads, 0, s, args, job, job));
+        CRESSO_LAUNCHED("norm_columns_kernel");
+    }
     return CRESSO_OK;
 }
 
