@@ -11,6 +11,7 @@ tensors, allocate their outputs with torch, and run on the current stream.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Sequence, Tuple
 
@@ -132,10 +133,18 @@ _TRAIN_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ID_BYTES = {torch.int32: 4, torch.int64: 8}
 
 
-def _train_dtype(dtype, what: str) -> int:
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the stream's address without the object around it: 2 us less a call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+def _train_dtype(dtype, what: str, name: str) -> int:
     code = _TRAIN_DTYPES.get(dtype)
     if code is None:
-        raise RuntimeError(f"{what} must be float32, float16 or bfloat16 (got {dtype})")
+        raise RuntimeError(f"{what}: {name} must be float32, float16 or bfloat16 (got {dtype})")
     return code
 
 
@@ -161,9 +170,9 @@ def _train_inputs(what: str, **tensors) -> torch.device:
     return device
 
 
-def _number(value, what: str) -> float:
+def _number(value, what: str, name: str) -> float:
     if isinstance(value, Tensor):
-        raise TypeError(f"{what} must be a number, not a tensor")
+        raise TypeError(f"{what}: {name} must be a number, not a tensor")
     return float(value)
 
 
@@ -184,17 +193,25 @@ def _address(t: Optional[Tensor]) -> int:
 
 
 def _train_call(what: str, fn, device: torch.device, *args) -> None:
+    """One C entry point on the current stream of the tensors' device."""
     if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+        status = fn(*args, _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+            status = fn(*args, _raw_stream(device.index))
+    if status != 0:
+        _lib.check(status, what)
 
 
-def _train_scratch(what: str, fn, device: torch.device, *sizes) -> Tensor:
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(entry: str, *sizes: int) -> int:
     nbytes = ctypes.c_int64()
-    _lib.check(fn(*sizes, ctypes.byref(nbytes)), what)
-    return torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+    _lib.check(getattr(_lib.lib(), entry)(*sizes, ctypes.byref(nbytes)), entry)
+    return nbytes.value
+
+
+def _train_scratch(entry: str, like: Tensor, *sizes: int) -> Tensor:
+    return like.new_empty(_scratch_bytes(entry, *sizes), dtype=torch.uint8)
 
 
 def embedding_gather(weight: Tensor, tokens: Tensor, scale: float = 1.0, *, row0: int = 0,
@@ -209,15 +226,15 @@ def embedding_gather(weight: Tensor, tokens: Tensor, scale: float = 1.0, *, row0
     if weight.dim() != 2:
         raise RuntimeError(f"embedding_gather: weight must be (rows, width) (got {tuple(weight.shape)})")
     dtype = weight.dtype if dtype is None else dtype
-    wd, od = _train_dtype(weight.dtype, "embedding_gather: weight"), _train_dtype(dtype, "embedding_gather: dtype")
+    wd, od = _train_dtype(weight.dtype, "embedding_gather", "weight"), _train_dtype(dtype, "embedding_gather", "dtype")
     if tokens.dtype not in _ID_BYTES:
         raise RuntimeError(f"embedding_gather: tokens must be int32 or int64 (got {tokens.dtype})")
-    scale = _number(scale, "embedding_gather: scale")
+    scale = _number(scale, "embedding_gather", "scale")
     device = _train_inputs("embedding_gather", weight=weight, tokens=tokens)
     rows, width = weight.shape
     weight, _, stride = _row_view(weight)
     tokens = tokens.contiguous()
-    out = torch.empty((*tokens.shape, width), dtype=dtype, device=device)
+    out = weight.new_empty((*tokens.shape, width), dtype=dtype)
     _train_call("embedding_gather", _lib.lib().cresso_embedding_gather, device, weight.data_ptr(), wd, rows, width,
                 stride, tokens.data_ptr(), _ID_BYTES[tokens.dtype], tokens.numel(), int(row0), scale, out.data_ptr(),
                 od)
@@ -251,15 +268,15 @@ def embedding_grad(grad: Tensor, tokens: Tensor, rows: int, scale: float = 1.0, 
             raise RuntimeError(f"embedding_grad: into must be contiguous ({rows}, {width}) (got {tuple(into.shape)})")
         dtype = into.dtype
     dtype = grad.dtype if dtype is None else dtype
-    gd, od = _train_dtype(grad.dtype, "embedding_grad: grad"), _train_dtype(dtype, "embedding_grad: dtype")
-    scale = _number(scale, "embedding_grad: scale")
+    gd, od = _train_dtype(grad.dtype, "embedding_grad", "grad"), _train_dtype(dtype, "embedding_grad", "dtype")
+    scale = _number(scale, "embedding_grad", "scale")
     device = _train_inputs("embedding_grad", grad=grad, tokens=tokens, into=into)
     grad, _, stride = _row_view(grad)
     tokens = tokens.contiguous()
     n = tokens.numel()
-    out = torch.empty((rows, width), dtype=dtype, device=device) if into is None else into
+    out = grad.new_empty((rows, width), dtype=dtype) if into is None else into
     L = _lib.lib()
-    scratch = _train_scratch("embedding_grad", L.cresso_embedding_grad_scratch_bytes, device, n, rows, width)
+    scratch = _train_scratch("cresso_embedding_grad_scratch_bytes", grad, n, rows, width)
     _train_call("embedding_grad", L.cresso_embedding_grad, device, grad.data_ptr(), gd, n, width, stride,
                 tokens.data_ptr(), _ID_BYTES[tokens.dtype], rows, int(row0), int(padding is not None),
                 0 if padding is None else int(padding), scale, out.data_ptr(), od, int(into is not None),
@@ -272,7 +289,7 @@ def _norm_arguments(what: str, residual: Tensor, x: Optional[Tensor], act_dtype,
     if residual.dim() < 1:
         raise RuntimeError(f"{what}: the residual must be (..., width)")
     width = residual.shape[-1]
-    rd, ad = _train_dtype(residual.dtype, f"{what}: residual"), _train_dtype(act_dtype, f"{what}: x")
+    rd, ad = _train_dtype(residual.dtype, what, "residual"), _train_dtype(act_dtype, what, "x")
     if rd != ad and rd != 0:
         raise RuntimeError(f"{what}: x must have the residual's type, or 16 bits beside a float32 residual "
                            f"(got {act_dtype} beside {residual.dtype})")
@@ -284,14 +301,16 @@ def _norm_arguments(what: str, residual: Tensor, x: Optional[Tensor], act_dtype,
     for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
         if w is None:
             continue
-        if tuple(w.shape) != (width,):
+        if w.dim() != 1 or w.shape[0] != width:
             raise RuntimeError(f"{what}: {name} must be ({width},) (got {tuple(w.shape)})")
-        wd = _train_dtype(w.dtype, f"{what}: {name}")
+        wd = _train_dtype(w.dtype, what, name)
     if post_weight is not None and pre_weight is not None and post_weight.dtype is not pre_weight.dtype:
         raise RuntimeError(f"{what}: the two weights must have one type")
     gate_rows, gd = 0, 0
     if gate is not None:
-        gd = _train_dtype(gate.dtype, f"{what}: gate")
+        gd = _train_dtype(gate.dtype, what, "gate")
+        if gate.dim() == 1 and gate.shape[0] == width:
+            return residual.numel() // width if width else 0, width, 1, (rd, ad, wd, gd)
         lead = tuple(residual.shape[:-1])
         g = (1,) * (residual.dim() - gate.dim()) + tuple(gate.shape[:-1])
         shared = len(g)
@@ -324,14 +343,14 @@ def block_norm(residual: Tensor, x: Optional[Tensor] = None, post_weight: Option
         raise RuntimeError(f"block_norm: y has x's type ({x.dtype}), not {dtype}")
     n, width, gate_rows, (rd, ad, wd, gd) = _norm_arguments("block_norm", residual, x, act, post_weight, pre_weight,
                                                             gate)
-    scale, eps = _number(scale, "block_norm: scale"), _number(eps, "block_norm: eps")
+    scale, eps = _number(scale, "block_norm", "scale"), _number(eps, "block_norm", "eps")
     device = _train_inputs("block_norm", residual=residual, x=x, post_weight=post_weight, pre_weight=pre_weight,
                            gate=gate)
     given = residual
-    residual, x, post_weight, pre_weight, gate = (
-        None if t is None else t.contiguous() for t in (residual, x, post_weight, pre_weight, gate))
+    residual, x, post_weight, pre_weight, gate = [
+        None if t is None else t.contiguous() for t in (residual, x, post_weight, pre_weight, gate)]
     h = given if x is None else torch.empty_like(residual)
-    y = None if pre_weight is None else torch.empty_like(residual, dtype=act)
+    y = None if pre_weight is None else torch.empty_like(residual, dtype=act) if x is None else torch.empty_like(x)
     if x is not None or y is not None:
         _train_call("block_norm", _lib.lib().cresso_block_norm, device, residual.data_ptr(), _address(x),
                     _address(post_weight), _address(pre_weight), _address(gate), n, width, gate_rows, rd, ad, wd, gd,
@@ -358,16 +377,16 @@ def block_norm_grad(h: Tensor, x: Optional[Tensor], d_h: Optional[Tensor], d_y: 
         if t is not None and (t.shape != h.shape or t.dtype is not like):
             raise RuntimeError(f"block_norm_grad: {name} must be {like} {tuple(h.shape)} (got {t.dtype} "
                                f"{tuple(t.shape)})")
-    scale, eps = _number(scale, "block_norm_grad: scale"), _number(eps, "block_norm_grad: eps")
+    scale, eps = _number(scale, "block_norm_grad", "scale"), _number(eps, "block_norm_grad", "eps")
     device = _train_inputs("block_norm_grad", h=h, x=x, d_h=d_h, d_y=d_y, post_weight=post_weight,
                            pre_weight=pre_weight, gate=gate)
-    h, x, d_h, d_y, post_weight, pre_weight, gate = (
-        None if t is None else t.contiguous() for t in (h, x, d_h, d_y, post_weight, pre_weight, gate))
+    h, x, d_h, d_y, post_weight, pre_weight, gate = [
+        None if t is None else t.contiguous() for t in (h, x, d_h, d_y, post_weight, pre_weight, gate)]
     d_residual = torch.empty_like(h)
-    d_x, d_post, d_gate = (None if t is None else torch.empty_like(t) for t in (x, post_weight, gate))
+    d_x, d_post, d_gate = [None if t is None else torch.empty_like(t) for t in (x, post_weight, gate)]
     d_pre = None if d_y is None else torch.empty_like(pre_weight)
     L = _lib.lib()
-    scratch = _train_scratch("block_norm_grad", L.cresso_block_norm_grad_scratch_bytes, device, n, width, gate_rows)
+    scratch = _train_scratch("cresso_block_norm_grad_scratch_bytes", h, n, width, gate_rows)
     _train_call("block_norm_grad", L.cresso_block_norm_grad, device, h.data_ptr(), _address(x), _address(d_h),
                 _address(d_y), _address(post_weight), _address(pre_weight), _address(gate), n, width, gate_rows, rd,
                 ad, wd, gd, scale, eps, d_residual.data_ptr(), _address(d_x), _address(d_post), _address(d_pre),
@@ -377,7 +396,7 @@ def block_norm_grad(h: Tensor, x: Optional[Tensor], d_h: Optional[Tensor], d_y: 
 
 def _distill(what: str, logits: Tensor, ids: Tensor, teacher: Tensor, weight: Optional[Tensor], temperature: float,
              backward: bool, inplace: bool):
-    ld, td = _train_dtype(logits.dtype, f"{what}: logits"), _train_dtype(teacher.dtype, f"{what}: teacher")
+    ld, td = _train_dtype(logits.dtype, what, "logits"), _train_dtype(teacher.dtype, what, "teacher")
     if ids.dtype not in _ID_BYTES:
         raise RuntimeError(f"{what}: ids must be int32 or int64 (got {ids.dtype})")
     if logits.dim() < 1 or ids.dim() < 1 or ids.shape[:-1] != logits.shape[:-1] or teacher.shape != ids.shape:
@@ -388,7 +407,7 @@ def _distill(what: str, logits: Tensor, ids: Tensor, teacher: Tensor, weight: Op
                            f"{tuple(weight.shape)})")
     if ids.shape[-1] > _lib.TRAIN_MAX_TOP:
         raise RuntimeError(f"{what}: at most {_lib.TRAIN_MAX_TOP} teacher entries in a row (got {ids.shape[-1]})")
-    temperature = _number(temperature, f"{what}: temperature")
+    temperature = _number(temperature, what, "temperature")
     if inplace and not logits.is_contiguous():
         raise RuntimeError(f"{what}: inplace needs contiguous logits")
     device = _train_inputs(what, logits=logits, ids=ids, teacher=teacher, weight=weight)
@@ -397,9 +416,8 @@ def _distill(what: str, logits: Tensor, ids: Tensor, teacher: Tensor, weight: Op
     n = math.prod(lead)
     rows, _, stride = _row_view(logits)
     ids, teacher, weight = ids.contiguous(), teacher.contiguous(), None if weight is None else weight.contiguous()
-    loss = torch.empty(lead, dtype=torch.float32, device=device)
-    grad = None if not backward else logits if inplace else torch.empty(logits.shape, dtype=logits.dtype,
-                                                                       device=device)
+    loss = logits.new_empty(lead, dtype=torch.float32)
+    grad = None if not backward else logits if inplace else logits.new_empty(logits.shape)
     _train_call(what, _lib.lib().cresso_distill, device, rows.data_ptr(), ld, n, vocab, stride, ids.data_ptr(),
                 _ID_BYTES[ids.dtype], teacher.data_ptr(), td, k, _address(weight), temperature, loss.data_ptr(),
                 _address(grad))
