@@ -708,7 +708,8 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
         using TR = decltype(tr);
         using TX = decltype(tx);
         auto launch = [&](auto kernel) {
-            CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            if (smem > 48 * 1024)
+                CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3((unsigned)(p.workers * p.shape.cluster));
             cfg.blockDim = dim3((unsigned)p.shape.threads);
