@@ -708,7 +708,7 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
         using TR = decltype(tr);
         using TX = decltype(tx);
         auto launch = [&](auto kernel) {
-            if (smem > 48 * 1024)
+            if (smem > 40 * 1024)  // with the static part, 48 KB need no leave
                 CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3((unsigned)(p.workers * p.shape.cluster));

@@ -10,10 +10,11 @@
 // operation, whose error is that of its result, because the same rounded B stands in the sum,
 // in the gradient and in the loss.  B needs no maximum over the row, only a reference near it:
 // every warp takes the largest of the first logits it reads, sums relative to that, and the
-// parts are joined relative to the largest reference.  A row whose sum leaves [1e-18, 1e18]
-// (a later logit about 40 tau above its warp's reference, a row far from zero or without
-// finite logits) is computed again from its maximum.  Sums are float32.  A NaN or +inf logit
-// makes its row NaN through the sum; a row of -inf alone has q = 0.  Repeated ids: every entry
+// parts are joined relative to the largest reference.  The sum is then at least 1; a row whose
+// sum leaves (0.5, 1e18) (a later logit about 40 tau above its warp's reference, a row far from
+// zero, or a warp without finite logits at first) is computed again from its maximum.  Sums are
+// float32; an exponential below 2^-126 counts as zero.  A NaN or +inf logit makes its row NaN
+// through the sum; a row of -inf alone has q = 0.  Repeated ids: every entry
 // holds the whole P of its id, so that all of them write the same value.
 #include "train_common.cuh"
 
@@ -159,13 +160,16 @@ __device__ __forceinline__ void join_warp(float& m, float& s, float c2) {
 constexpr float kFar = 16777216.0f;
 constexpr float kLargeSum = 1e18f;  // its reciprocal, times a small weight, stays a normal number
 
-// Loss of the row from its base = -B and sum by one warp, and the gradients of the entries' ids in
+// Loss of the row from its reference m and sum by one warp, and the gradients of the entries' ids in
 // [v0, v1) by `threads` threads.
-__device__ __forceinline__ float row_loss(const DistillArgs& a, const TopList& top, float w, float c2, float base, float s) {
-    const float log_s = s == 0.0f ? 0.0f : logf(s);
+__device__ __forceinline__ float row_loss(const DistillArgs& a, const TopList& top, float w, float c2, float m, float s) {
+    // log q = (z - m) / tau - log of the sum relative to m, which is s but for the rounding of B; in
+    // natural units, where a masked logit of the type's lowest value is still finite
+    const float inv_tau = 1.0f / a.tau;
+    const float log_s = (s == 0.0f ? 0.0f : logf(s)) - fmaf(m, c2, -__fmul_rn(m, c2)) * kLn2;
     float cross = 0.0f;
     for (int k = threadIdx.x & 31; k < a.k; k += 32)
-        if (top.p[k] != 0.0f) cross += top.p[k] * (fmaf(top.z[k], c2, base) * kLn2 - log_s);
+        if (top.p[k] != 0.0f) cross += top.p[k] * ((top.z[k] - m) * inv_tau - log_s);
     return w * a.tau * a.tau * (*top.entropy - warp_sum(cross));
 }
 template <typename T>
@@ -342,7 +346,7 @@ __global__ void __launch_bounds__(THREADS + 32)
             join_warp<8>(m, s, c2);
         }
         any = *top.any;
-        if (any && !(s < kLargeSum && s > 1.0f / kLargeSum)) {
+        if (any && !(s < kLargeSum && s > 0.5f)) {
             // no usable reference: from the row's maximum
             const T* part = reinterpret_cast<const T*>(words);
             m = -INFINITY;
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(THREADS + 32)
     const float base = -__fmul_rn(m, c2);
     if (is_teacher) {
         if (rank == 0) {
-            const float v = any ? row_loss(a, top, w, c2, base, s) : 0.0f;
+            const float v = any ? row_loss(a, top, w, c2, m, s) : 0.0f;
             if (lane == 0) loss[t] = v;
         }
     } else if (out != nullptr) {

@@ -176,6 +176,13 @@ def _number(value, what: str, name: str) -> float:
     return float(value)
 
 
+def _int64(value, what: str, name: str) -> int:
+    value = int(value)
+    if not -2**63 <= value < 2**63:
+        raise RuntimeError(f"{what}: {name} does not fit 64 bits (got {value})")
+    return value
+
+
 def _row_view(t: Tensor) -> Tuple[Tensor, int, int]:
     """(tensor, number of rows, row stride) of (..., width) with the elements of a row
     adjacent and the rows equally far apart; a copy where the strides do not allow that."""
@@ -236,8 +243,8 @@ def embedding_gather(weight: Tensor, tokens: Tensor, scale: float = 1.0, *, row0
     tokens = tokens.contiguous()
     out = weight.new_empty((*tokens.shape, width), dtype=dtype)
     _train_call("embedding_gather", _lib.lib().cresso_embedding_gather, device, weight.data_ptr(), wd, rows, width,
-                stride, tokens.data_ptr(), _ID_BYTES[tokens.dtype], tokens.numel(), int(row0), scale, out.data_ptr(),
-                od)
+                stride, tokens.data_ptr(), _ID_BYTES[tokens.dtype], tokens.numel(), _int64(row0, "embedding_gather", "row0"), scale,
+                out.data_ptr(), od)
     return out
 
 
@@ -269,7 +276,8 @@ def embedding_grad(grad: Tensor, tokens: Tensor, rows: int, scale: float = 1.0, 
         dtype = into.dtype
     dtype = grad.dtype if dtype is None else dtype
     gd, od = _train_dtype(grad.dtype, "embedding_grad", "grad"), _train_dtype(dtype, "embedding_grad", "dtype")
-    scale = _number(scale, "embedding_grad", "scale")
+    scale, row0 = _number(scale, "embedding_grad", "scale"), _int64(row0, "embedding_grad", "row0")
+    padding = None if padding is None else _int64(padding, "embedding_grad", "padding")
     device = _train_inputs("embedding_grad", grad=grad, tokens=tokens, into=into)
     grad, _, stride = _row_view(grad)
     tokens = tokens.contiguous()
@@ -278,8 +286,8 @@ def embedding_grad(grad: Tensor, tokens: Tensor, rows: int, scale: float = 1.0, 
     L = _lib.lib()
     scratch = _train_scratch("cresso_embedding_grad_scratch_bytes", grad, n, rows, width)
     _train_call("embedding_grad", L.cresso_embedding_grad, device, grad.data_ptr(), gd, n, width, stride,
-                tokens.data_ptr(), _ID_BYTES[tokens.dtype], rows, int(row0), int(padding is not None),
-                0 if padding is None else int(padding), scale, out.data_ptr(), od, int(into is not None),
+                tokens.data_ptr(), _ID_BYTES[tokens.dtype], rows, row0, int(padding is not None),
+                0 if padding is None else padding, scale, out.data_ptr(), od, int(into is not None),
                 scratch.data_ptr(), scratch.numel())
     return out
 

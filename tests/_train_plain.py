@@ -166,4 +166,7 @@ def distill(logits, ids, teacher, weight, tau):
     wide = torch.where(torch.isfinite(w), w.abs(), 0.0)
     loss_bound = wide * tau ** 2 * (size * (2 * dp + (k + 8) * U32) + dq + dp)
     grad_bound = (wide * tau)[:, None] * (torch.nan_to_num(q) * dq[:, None] + torch.nan_to_num(target) * dp[:, None])
-    return (loss, loss_bound), (grad, 2 * grad_bound)
+    # an exponential below the normal range, 2^-126, may count as zero: relative to a sum of at least
+    # 0.5 its q is off by at most 2^-125
+    flushed = (wide * tau)[:, None] * 2.0 ** -125
+    return (loss, loss_bound), (grad, 2 * grad_bound + flushed)

@@ -134,6 +134,8 @@ IDS = torch.zeros(4, dtype=torch.int64)
     (lambda: ops.embedding_grad(_f(4, 4), IDS, 9, into=_f(8, 4)), "into must be"),
     (lambda: ops.embedding_grad(_f(4, 4), IDS, 9, into=_f(4, 9).t()), "into must be"),
     (lambda: ops.embedding_grad(_f(4, 4), IDS, 9, into=_f(9, 4), dtype=torch.float16), "not the type of into"),
+    (lambda: ops.embedding_grad(_f(4, 4), IDS, 9, row0=2**63), "64 bits"),
+    (lambda: ops.embedding_grad(_f(4, 4), IDS, 9, padding=-2**63 - 1), "64 bits"),
     (lambda: ops.embedding_grad(_f(4, 4), IDS, 9), "CUDA tensor"),
     (lambda: ops.block_norm(_f(2, 4), _f(2, 5)), "x is"),
     (lambda: ops.block_norm(_f(2, 4, dtype=torch.float16), _f(2, 4)), "residual's type"),

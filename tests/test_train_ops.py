@@ -86,7 +86,7 @@ def test_embedding_grad(ops, n, rows, width, gd, od):
 
 
 @pytest.mark.parametrize("rows,width,n", [(32000, 64, 16384), (1000, 512, 20000), (3, 1024, 9000), (100000, 16, 70000),
-                                          (250001, 8, 5000)])
+                                          (250001, 8, 5000), (174720, 8, 2000), (47000, 8, 16384)])
 def test_embedding_grad_uneven_rows(ops, rows, width, n):
     """Most positions fall on a few rows (a frequent word, padding), some on no row at all."""
     gen = torch.Generator(device="cuda").manual_seed(9)
@@ -153,7 +153,8 @@ def test_embedding_infinities_stay_in_their_rows(ops):
 # ---------------------------------------------------------------------------- block norm
 
 NORM_SIZES = [(1, 1, 1), (1, 1, 4096), (2, 3, 7), (3, 5, 64), (2, 33, 250), (3, 341, 130), (1, 9, 2050), (5, 1, 1024),
-              (1, 7, 8200), (2, 2, 20001), (4, 64, 512), (1, 2, 40000), (2, 700, 32)]
+              (1, 7, 8200), (2, 2, 20001), (4, 64, 512), (1, 2, 40000), (2, 700, 32), (2, 600, 4096), (3, 400, 2560),
+              (1, 1201, 1030), (2, 600, 5001), (1, 1190, 520)]
 PAIRS = [(F32, F32), (F32, BF16), (BF16, BF16), (F16, F16), (F32, F16)]
 
 
@@ -371,6 +372,53 @@ def test_distill_far_logits(ops):
     teacher[3] += 500
     _check_distill(ops, logits, ids, teacher, weight, 1.0)
     _check_distill(ops, logits, ids, teacher, weight, 30.0)
+
+
+@pytest.mark.parametrize("vocab", [3001, 32000, 128259])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_distill_uneven_rows(ops, vocab, dtype):
+    """A logit far above all others, or all of them far below, at the end of a row; beginnings
+    that are masked; every one of them in every part of the row."""
+    inf = float("inf")
+    logits, ids, teacher, weight = _distill_inputs(9, vocab, 6, dtype)
+    weight[:] = 1
+    logits[0, -1] = 300
+    logits[1, vocab // 2] = 88
+    logits[2, :vocab - 5] = -inf
+    ids[2] = torch.arange(6, device="cuda") + vocab - 6
+    logits[3, :vocab - 5] = torch.finfo(dtype).min
+    logits[4, :vocab // 2] = -inf
+    logits[4, vocab // 2:] -= 100
+    logits[5, vocab // 3:] = -200
+    logits[6, vocab // 2:] += 200
+    logits[7] = -1e4
+    logits[8] = 0
+    _check_distill(ops, logits, ids, teacher, weight, 1.0)
+
+
+def test_distill_long_lists_of_one_id(ops):
+    logits, ids, teacher, weight = _distill_inputs(3, 5000, 1024, F32)
+    ids[0] = 4999
+    ids[1] = torch.arange(1024, device="cuda") % 3
+    ids[2, ::2] = -1
+    _check_distill(ops, logits, ids, teacher, weight, 2.0)
+
+
+def test_calls_at_once_on_two_streams(ops):
+    """Calls that overlap on the GPU share nothing."""
+    t = [_chain_inputs(s) for s in (110, 130)]
+    want = [_chain(ops, x) for x in t]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(5):
+        for x, s in zip(t, streams):
+            with torch.cuda.stream(s):
+                outs.append(_chain(ops, x))
+    torch.cuda.synchronize()
+    for i, (loss, grads) in enumerate(outs):
+        assert torch.equal(loss, want[i % 2][0])
+        assert all(torch.equal(grads[k], want[i % 2][1][k]) for k in grads)
 
 
 def test_distill_rows_beyond_32_bit_offsets(ops):
