@@ -1,5 +1,5 @@
 // Distillation from a teacher's top logits: the loss of each row and the gradient
-// of the student's logits, from one reading of the row.
+// of the student's logits, from one reading of the row from DRAM.
 //
 // A row has V student logits z, K teacher entries (id, u), a weight w and the
 // temperature tau:
@@ -189,6 +189,10 @@ __device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopLis
 // the gradient, while it is still in L2 (the rows at work at a time are a third of it).  No
 // storage on the SM means many blocks an SM, in different phases: their loads overlap the others'
 // exponentials, barriers and teacher lists.  One further warp prepares the teacher's list.
+// Bound by the concurrency of loads and stores: 4096 rows of 32000 bfloat16 with their gradient take
+// 94 us, 495 MB at 5.3 TB/s.  Rows in registers (125 us) or in shared memory with the next row on
+// its way (100 us) leave fewer blocks; without any exponential the latter still took 93 us.  Six
+// blocks an SM instead of five let rows fall out of L2 (105 us).
 constexpr int kDistillThreads = 256;         // without the teacher's warp
 // Bytes of a row that a block is given at least.  With the gradient, more of them are in L2 for
 // longer and fewer blocks are better: 64 KB.  The loss alone is bound by what a block does before
