@@ -190,9 +190,9 @@ __device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopLis
 // storage on the SM means many blocks an SM, in different phases: their loads overlap the others'
 // exponentials, barriers and teacher lists.  One further warp prepares the teacher's list.
 // Bound by the concurrency of loads and stores: 4096 rows of 32000 bfloat16 with their gradient take
-// 94 us, 495 MB at 5.3 TB/s.  Rows in registers (125 us) or in shared memory with the next row on
+// 88 us, 495 MB at 5.6 TB/s.  Rows in registers (125 us) or in shared memory with the next row on
 // its way (100 us) leave fewer blocks; without any exponential the latter still took 93 us.  Six
-// blocks an SM instead of five let rows fall out of L2 (105 us).
+// blocks an SM instead of five let rows fall out of L2 (105 us, 94 with five).
 constexpr int kDistillThreads = 256;         // without the teacher's warp
 // Bytes of a row that a block is given at least.  With the gradient, more of them are in L2 for
 // longer and fewer blocks are better: 64 KB.  The loss alone is bound by what a block does before
@@ -314,6 +314,12 @@ __global__ void __launch_bounds__(THREADS + 32)
     bool any = false;
     float m = 0.0f, s = 0.0f, far = 0.0f;
     if (w != 0.0f) {
+        // with the gradient, the rest of the block's part is sent for at once (94 -> 89 us); the loss
+        // alone has more of its part in flight anyway and loses by it
+        if (out != nullptr && tid == 0 && r.count > U * THREADS)
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(words + U * THREADS),
+                         "r"((r.count - U * THREADS) * 16)
+                         : "memory");
         if (is_teacher) {
             load_teacher<T>(a, t, row, top, seen);
         } else {

@@ -486,6 +486,61 @@ def test_chain_gradients_against_autograd_in_float64(ops):
         assert rel < 16 * 2.0 ** -8, (name, rel)
 
 
+def test_inside_autograd_functions(ops):
+    """As the forward and backward of torch.autograd.Function: gradients against autograd's of the
+    formulas in float64."""
+    class Embedding(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, weight, tokens, scale):
+            ctx.save_for_backward(tokens)
+            ctx.rows, ctx.scale, ctx.dtype = weight.shape[0], scale, weight.dtype
+            return ops.embedding_gather(weight, tokens, scale)
+
+        @staticmethod
+        def backward(ctx, grad):
+            return ops.embedding_grad(grad, ctx.saved_tensors[0], ctx.rows, ctx.scale, dtype=ctx.dtype), None, None
+
+    class Norm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, residual, x, post, pre):
+            h, y = ops.block_norm(residual, x, post, pre, None, 0.5)
+            ctx.save_for_backward(h, x, post, pre)
+            return h, y
+
+        @staticmethod
+        def backward(ctx, d_h, d_y):
+            h, x, post, pre = ctx.saved_tensors
+            d_residual, d_x, d_post, d_pre, _ = ops.block_norm_grad(h, x, d_h, d_y, post, pre, None, 0.5)
+            return d_residual, d_x, d_post, d_pre
+
+    class Distill(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, logits, ids, teacher):
+            loss, grad = ops.distill_grad(logits, ids, teacher)
+            ctx.save_for_backward(grad)
+            return loss
+
+        @staticmethod
+        def backward(ctx, d_loss):
+            return ctx.saved_tensors[0] * d_loss[:, None], None, None
+
+    v, d, n = 301, 64, 23
+    table, other = _randn(150, v, d, scale=0.3), _randn(151, n, d)
+    post, pre = 1 + _randn(152, d, scale=0.2), 1 + _randn(153, d, scale=0.2)
+    tok, ids, teacher = _tokens(154, n, v), _tokens(155, (n, 4), v), _randn(156, n, 4)
+    leaves = [t.clone().requires_grad_() for t in (table, other, post, pre)]
+    e = Embedding.apply(leaves[0], tok, 2.0)
+    h, y = Norm.apply(leaves[1], e, leaves[2], leaves[3])
+    z = (h + y) @ table.t()
+    Distill.apply(z, ids, teacher).sum().backward()
+    wide = [t.double().requires_grad_() for t in (table, other, post, pre)]
+    (h, _), (y, _) = P.block_norm(wide[1], wide[0][tok] * 2.0, wide[2], wide[3], None, 0.5, 1e-6)
+    P.distill((h + y) @ table.double().t(), ids, teacher, None, 1.0)[0][0].sum().backward()
+    # float32 throughout: a few hundred roundings of 2^-24 on the way to a gradient
+    for got, want in zip(leaves, wide):
+        assert float((got.grad.double() - want.grad).norm() / want.grad.norm()) < 1000 * 2.0 ** -24
+
+
 def test_chain_feeds_the_optimizer(ops):
     """The gradients go to CRESSO5.step() as they are."""
     import cresso_b200
