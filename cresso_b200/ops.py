@@ -148,12 +148,21 @@ def _train_dtype(dtype, what: str, name: str) -> int:
     return code
 
 
-def _train_inputs(what: str, **tensors) -> torch.device:
-    """The one CUDA device of the given tensors (None is skipped); nothing that autograd
-    would have to record."""
-    device = None
-    grad = torch.is_grad_enabled()
-    for name, t in tensors.items():
+def _train_inputs(what: str, **tensors) -> int:
+    """Index of the one CUDA device of the given tensors (None is skipped); nothing among
+    them that autograd would have to record."""
+    index, grad = -1, torch.is_grad_enabled()
+    for t in tensors.values():
+        if t is None:
+            continue
+        at = t.get_device() if isinstance(t, Tensor) else -2  # -1 on the CPU
+        if index == -1:
+            index = at
+        if at != index or at < 0 or (grad and t.requires_grad):
+            break
+    else:
+        return index
+    for name, t in tensors.items():  # which one, and why
         if t is None:
             continue
         if not isinstance(t, Tensor):
@@ -163,11 +172,9 @@ def _train_inputs(what: str, **tensors) -> torch.device:
                                f"torch.no_grad() or inside a torch.autograd.Function")
         if not t.is_cuda:
             raise RuntimeError(f"{what}: {name} must be a CUDA tensor")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, not on {device}")
-    return device
+        if t.get_device() != index:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, not on cuda:{index}")
+    raise RuntimeError(f"{what}: tensors of one CUDA device are needed")
 
 
 def _number(value, what: str, name: str) -> float:
@@ -199,13 +206,13 @@ def _address(t: Optional[Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _train_call(what: str, fn, device: torch.device, *args) -> None:
+def _train_call(what: str, fn, device: int, *args) -> None:
     """One C entry point on the current stream of the tensors' device."""
-    if device.index == torch.cuda.current_device():
-        status = fn(*args, _raw_stream(device.index))
+    if device == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, _raw_stream(device.index))
+            status = fn(*args, _raw_stream(device))
     if status != 0:
         _lib.check(status, what)
 
