@@ -57,29 +57,6 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-// Sum over the block, the same in every thread and in a fixed order; `sh` holds
-// one float per warp.  Ends with a barrier, so that `sh` can be used again.
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-    const int warps = blockDim.x >> 5;
-    v = warp_sum(v);
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float s = (threadIdx.x & 31) < warps ? sh[threadIdx.x & 31] : 0.0f;
-    s = warp_sum(s);
-    __syncthreads();
-    return s;
-}
-__device__ __forceinline__ float block_max(float v, float* sh) {
-    const int warps = blockDim.x >> 5;
-    v = warp_max(v);
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float s = (threadIdx.x & 31) < warps ? sh[threadIdx.x & 31] : -INFINITY;
-    s = warp_max(s);
-    __syncthreads();
-    return s;
-}
-
 // Two packed 16-bit elements and their float values: one instruction an element to read,
 // one for both to write.
 template <typename T>

@@ -6,12 +6,14 @@
  * scale, and the distillation loss from a teacher's top logits.  They have no
  * counterpart in the reference, whose package holds the optimizer only.
  *
- * The conventions are those of cresso_b200.h: raw device pointers, an int status
- * (the message is read with cresso_last_error), caller-owned scratch (32-byte
- * aligned) whose size is queried first, work ordered on the given stream of the current device,
- * no allocation and no synchronisation.  Element types are CRESSO_DTYPE_F32,
- * _F16 and _BF16; sums, statistics and norms are float32 and every output is
- * rounded once.  The same inputs give the same bits in every run.
+ * The conventions are those of cresso_b200.h: raw device pointers aligned to
+ * their elements, an int status (the message is read with cresso_last_error),
+ * caller-owned scratch (32-byte aligned, not shared by calls that may overlap)
+ * whose size is queried first, work ordered on the given stream of the current
+ * device, no allocation and no synchronisation.  Outputs overlap inputs only
+ * where that is said.  Element types are CRESSO_DTYPE_F32, _F16 and _BF16; sums,
+ * statistics and norms are float32 and every output is rounded once.  The same
+ * inputs give the same bits in every run.
  */
 #ifndef CRESSO_B200_TRAIN_H
 #define CRESSO_B200_TRAIN_H
@@ -25,8 +27,8 @@ extern "C" {
 /* Bounds of the operators below; larger calls get CRESSO_EUNSUPPORTED. */
 enum { CRESSO_TRAIN_MAX_TOP = 1024 };          /* teacher entries of a row            */
 enum { CRESSO_TRAIN_MAX_ROWS = 2147483392 };   /* rows of a table, tokens, logit rows */
-enum { CRESSO_TRAIN_MAX_EMBEDDING_WIDTH = 4194240 }; /* columns of a table row     */
-enum { CRESSO_TRAIN_MAX_NORM_WIDTH = 65536 };  /* columns of a block norm             */
+enum { CRESSO_TRAIN_MAX_EMBEDDING_WIDTH = 4194240 }; /* columns of an embedding gradient */
+enum { CRESSO_TRAIN_MAX_NORM_WIDTH = 65536 };  /* columns of a block norm, of at most 2^28 - 32 rows */
 
 /* ------------------------------------------------------------ embedding --- */
 
@@ -89,9 +91,9 @@ CRESSO_API int cresso_block_norm_grad(const void* h, const void* x, const void* 
  *   loss_t = weight_t * temperature^2 * sum_k p_k (log p_k - log q[id_k]),
  *   grad_t[v] = weight_t * temperature * (q[v] - sum of p_k with id_k = v).
  * An entry is valid when 0 <= id < vocab and u is not -inf; an id may occur more
- * than once; temperature is in [1e-6, 1e6].  A row with weight 0 or no valid entry has loss 0 and gradient 0
- * whatever its logits hold.  A student that gives a teacher entry probability 0
- * has loss +inf.  ids and teacher are contiguous (n, k), ids int32 or int64,
+ * than once; temperature is in [1e-6, 1e6].  A row with weight 0 or no valid entry
+ * has loss 0 and gradient 0 whatever its logits hold.  A student that gives a
+ * teacher entry probability 0 (a logit of -inf) has loss +inf.  ids and teacher are contiguous (n, k), ids int32 or int64,
  * weight float32 (n) or NULL (1); loss is float32 (n); grad has the logits'
  * type, contiguous (n, vocab), and may be the logits themselves when their rows
  * are contiguous; grad NULL computes the loss only. */

@@ -74,7 +74,8 @@ def _norm(**kw):
     (dict(rd=2, ad=0), 2), (dict(rd=2, ad=1), 2), (dict(rd=3, ad=3), 2), (dict(wd=3), 2), (dict(gd=3), 2),
     (dict(n=-1), 1), (dict(width=-1), 1), (dict(gate_rows=4), 1), (dict(gate_rows=0), 1), (dict(eps=-1.0), 1),
     (dict(eps=float("nan")), 1), (dict(x=0), 1), (dict(residual=0), 1), (dict(h=0), 1), (dict(y=0), 1),
-    (dict(pre=0), 1), (dict(x=0, post=0, gate=0, pre=0, y=0), 1), (dict(n=2**31, gate=0), 2), (dict(n=0), 0),
+    (dict(pre=0), 1), (dict(x=0, post=0, gate=0, pre=0, y=0), 1), (dict(n=2**31, gate=0), 2), (dict(n=2**28, gate=0), 2),
+    (dict(width=65537), 2), (dict(n=0), 0),
     (dict(width=0), 0)])
 def test_block_norm_status(kw, status):
     assert _norm(**kw) == status, _lib.last_error()
