@@ -172,3 +172,33 @@ def test_numbers_are_not_read_from_tensors():
         ops.embedding_gather(_f(3, 4), IDS, torch.ones(()))
     with pytest.raises(TypeError, match="must be a number"):
         ops.distill_loss(_f(4, 9), IDS[:, None], _f(4, 1), temperature=torch.ones(()))
+
+
+def test_calls_run_on_the_tensors_device(monkeypatch):
+    """With another device current, an entry point is called with the tensors' device current and
+    on that device's current stream."""
+    current, seen = [0], []
+
+    class Guard:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 100 + index)
+
+    def entry(*args):
+        seen.append((current[0], args))
+        return 0
+
+    ops._train_call("x", entry, 0, 7)
+    ops._train_call("x", entry, 3, 7, 8)
+    assert seen == [(0, (7, 100)), (3, (7, 8, 103))] and current == [0]
+    with pytest.raises(RuntimeError, match="invalid argument"):
+        ops._train_call("x", lambda *a: 1, 0)

@@ -257,6 +257,27 @@ def test_block_norm_empty_and_extreme(ops):
     assert torch.isnan(y[1, 1]).all()
 
 
+def test_block_norm_beyond_32_bit_offsets(ops):
+    n, d, last = 530001, 4104, 3  # 2.17e9 elements
+    make = lambda seed: _randn(seed, last, d, dtype=BF16)  # noqa: E731
+    res, x = torch.zeros(n, d, dtype=BF16, device="cuda"), torch.zeros(n, d, dtype=BF16, device="cuda")
+    res[-last:], x[-last:] = make(120), make(121)
+    post, pre, gate = 1 + _randn(122, d, scale=0.3), 1 + _randn(123, d, scale=0.3), _randn(124, d)
+    h, y = ops.block_norm(res, x, post, pre, gate, 0.5)
+    want_h, want_y = P.block_norm(make(120), make(121), post, pre, gate, 0.5, 1e-6)
+    P.check(h[-last:], *want_h, BF16, "h")
+    P.check(y[-last:], *want_y, BF16, "y")
+    assert not h[:-last].any() and not y[:-last].any()
+    del h, y
+    dh, dy = torch.zeros(n, d, dtype=BF16, device="cuda"), torch.zeros(n, d, dtype=BF16, device="cuda")
+    dh[-last:], dy[-last:] = make(125), make(126)
+    got = ops.block_norm_grad(res, x, dh, dy, post, pre, gate, 0.5)
+    want = P.block_norm_grad(make(120), make(121), make(125), make(126), post, pre, gate, 0.5, 1e-6)
+    for i, like in enumerate((BF16, BF16, F32, F32, F32)):  # rows of zeros add nothing to the sums
+        P.check(got[i][-last:] if i < 2 else got[i], *want[i], like, str(i))
+    assert not got[0][:-last].any() and not got[1][:-last].any()
+
+
 # -------------------------------------------------------------------------- distillation
 
 def _distill_inputs(n, vocab, k, dtype, seed=30, td=F32, ids_dtype=torch.int64):
