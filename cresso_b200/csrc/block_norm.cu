@@ -40,8 +40,8 @@ static NormShape norm_shape(int64_t width, int elems) {
     p.threads = (int)align_up(ceil_div(p.block_width, p.elems), 32);
     return p;
 }
-// Few rows are a matter of latency, for which 8 columns a thread are better: one row of 4096
-// takes 4.2 us instead of 6.2, and 16384 rows 142 us instead of 139.
+// Few rows are a matter of latency, for which 8 columns a thread are better in the forward pass:
+// one row of 4096 takes 4.2 us instead of 6.2, and 16384 rows 142 us instead of 139.
 constexpr int64_t kNormFewRows = 8 * 148;
 
 // ----------------------------------------------------------------- forward ---
@@ -163,8 +163,11 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __re
 // gradients follow from B, since the gate is constant over the rows of a unit:
 //   d_gate = scale w_post B,  d_post = scale gate B
 // (a gate with a row of its own for each row: d_gate per row, B over e q gate).
-// Rows come through `stages` stages of shared memory that cp.async fills ahead; each
-// thread copies and reads the same columns.
+// Rows come through `stages` stages of shared memory that cp.async fills ahead.  A thread copies
+// and reads the same columns, 2 or 8 at an access; rows of odd width or address (VEC 1) come as the
+// 16-byte pieces that hold them, each shifted by its own offset.  Absent arrays and columns behind
+// the row are zeros there, so that nothing but the stores is guarded: 12000 float16 rows of 2051
+// take 195 us instead of 541, of 1030 69 us instead of 106.
 // Bound by memory, then by instructions: 16384 bfloat16 rows of 4096 take 132 us and 140 us with the
 // column sums, 805 MB at 5.8 TB/s; scalar float32 arithmetic and bounds checks on every access took
 // 182 us.
@@ -247,6 +250,31 @@ __device__ __forceinline__ void put8(int chunk, int c, int stride, int d, const 
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+// Begins to copy the 16-byte pieces that hold src[0, count) to `dst`, which is 16-byte aligned:
+// src[i] comes to lie at dst[ahead(src) + i].  Nothing before `array`, where src's array starts,
+// is read, and nothing behind src[count - 1]: zeros follow it, eight at least.  The block's threads
+// share the pieces.
+template <typename T>
+__device__ __forceinline__ int ahead(const T* src) {
+    return (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
+}
+template <typename T>
+__device__ __forceinline__ void copy_span(T* dst, const T* array, const T* src, int count) {
+    const uintptr_t start = reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15;
+    const int bytes = (ahead(src) + count) * (int)sizeof(T);
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
+    for (int i = 16 * threadIdx.x; i < bytes + 16; i += 16 * blockDim.x) {
+        if (start + i >= reinterpret_cast<uintptr_t>(array)) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i), "l"(start + i),
+                         "r"(max(0, min(16, bytes - i)))
+                         : "memory");
+        } else {  // the first piece of an array that starts inside it
+            const int from = ahead(src);
+            for (int j = from; j < 16 / (int)sizeof(T); ++j) dst[j] = j < from + count ? src[j - from] : T(0.0f);
+        }
+    }
+}
+
 // WHOLE: x, d_h, d_y and post_weight are there, and the threads' columns are the row's.
 template <typename TR, typename TX, int VEC, int EL, bool OWN_GATE, bool WHOLE>
 __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
@@ -261,7 +289,8 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
     const int rank = k.cluster > 1 ? (int)(blockIdx.x % k.cluster) : 0;
     const int64_t col0 = (int64_t)rank * k.block_width, worker = blockIdx.x / k.cluster, workers = gridDim.x / k.cluster;
     const int d = (int)min((int64_t)k.block_width, width - col0);  // columns of this block, counted from col0
-    const int slots = (d + 7) / 8 * 8, c = tid * VEC, stride = T * VEC;
+    constexpr bool kSpans = VEC == 1;
+    const int slots = T * EL + (kSpans ? 16 : 0), c = tid * VEC, stride = T * VEC;
     const float inv_d = 1.0f / (float)width;
     const bool has_x = WHOLE || k.x != nullptr, has_dh = WHOLE || k.dh != nullptr, has_dy = WHOLE || k.dy != nullptr;
     const bool has_post = WHOLE || a.post_w != nullptr;
@@ -278,6 +307,13 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
         const TX *x = static_cast<const TX*>(k.x) + at, *dy = static_cast<const TX*>(k.dy) + at;
         TR *sh = stage_r(s, 0), *sdh = stage_r(s, 1);
         TX *sx = stage_x(s, 0), *sdy = stage_x(s, 1);
+        if constexpr (kSpans) {
+            copy_span(sh, static_cast<const TR*>(k.h), h, d);
+            if (has_x) copy_span(sx, static_cast<const TX*>(k.x), x, d);
+            if (has_dh) copy_span(sdh, static_cast<const TR*>(k.dh), dh, d);
+            if (has_dy) copy_span(sdy, static_cast<const TX*>(k.dy), dy, d);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < EL / VEC; ++i) {
             const int col = c + i * stride;
@@ -287,6 +323,12 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
             if (has_dh) copy_vec<TR, VEC>(sdh + col, dh + col);
             if (has_dy) copy_vec<TX, VEC>(sdy + col, dy + col);
         }
+    };
+    auto block_sync = [&] {
+        if (warps > 1)
+            __syncthreads();
+        else
+            __syncwarp();
     };
     constexpr int Q = EL / 8;
     float2 pre[Q][4], post[Q][4], sum_b[Q][4], sum_pre[Q][4];
@@ -311,6 +353,15 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
                 for (int j = 0; j < 4; ++j) v[q][j] = __fmul2_rn(v[q][j], f[q][j]);
         });
     };
+    if (!WHOLE) {  // absent arrays and the columns behind the row read as zero: no bounds checks then
+        for (int st = 0; st < k.stages; ++st) {
+            for (int i = tid + (has_dh ? d : 0); i < slots; i += T) stage_r(st, 1)[i] = TR(0.0f);
+            for (int i = tid + (has_x ? d : 0); i < slots; i += T) stage_x(st, 0)[i] = TX(0.0f);
+            for (int i = tid + (has_dy ? d : 0); i < slots; i += T) stage_x(st, 1)[i] = TX(0.0f);
+            for (int i = tid + d; i < slots; i += T) stage_r(st, 0)[i] = TR(0.0f);
+        }
+        block_sync();
+    }
     factors(pre, has_dy ? 1.0f : 0.0f);
     if (has_dy) multiply(pre, a.pre_w, a.w_dtype, col0);
     factors(sum_pre, 0.0f);
@@ -330,6 +381,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
         int s = 0;
         for (int64_t r = r0; r < r1; ++r) {
             if (k.stages == 1) {
+                if (kSpans) block_sync();
                 fetch(0, r);
                 copy_commit();
             }
@@ -342,24 +394,37 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
             const int64_t at = r * width + col0;
             const TR *sh = stage_r(s, 0), *sdh = stage_r(s, 1);
             const TX *sx = stage_x(s, 0), *sdy = stage_x(s, 1);
-            auto load_r = [&](int q, const TR* p, bool has, float2 (&f)[4]) {
-                get8<VEC, WHOLE>(q, c, stride, has ? d : 0, f, [&](int col, float (&v)[VEC]) { load_vec<TR, VEC>(p + col, v); });
+            if constexpr (kSpans) {
+                block_sync();  // the other threads' pieces
+                sh += ahead(static_cast<const TR*>(k.h) + at);
+                sdh += ahead(static_cast<const TR*>(k.dh) + at);
+                sx += ahead(static_cast<const TX*>(k.x) + at);
+                sdy += ahead(static_cast<const TX*>(k.dy) + at);
+            }
+            auto load_r = [&](int q, const TR* p, float2 (&f)[4]) {
+                get8<VEC, true>(q, c, stride, d, f, [&](int col, float (&v)[VEC]) { load_vec<TR, VEC>(p + col, v); });
             };
-            auto load_x = [&](int q, const TX* p, bool has, float2 (&f)[4]) {
-                get8<VEC, WHOLE>(q, c, stride, has ? d : 0, f, [&](int col, float (&v)[VEC]) { load_vec<TX, VEC>(p + col, v); });
+            auto load_x = [&](int q, const TX* p, float2 (&f)[4]) {
+                get8<VEC, true>(q, c, stride, d, f, [&](int col, float (&v)[VEC]) { load_vec<TX, VEC>(p + col, v); });
             };
             auto load_gate = [&](int q, float2 (&f)[4]) {
-                get8<VEC, WHOLE>(q, c, stride, d, f,
-                          [&](int col, float (&v)[VEC]) { load_any_vec<VEC>(a.gate, a.gate_dtype, at + col, v); });
+                with_any(a.gate, a.gate_dtype, [&](auto* w) {
+                    using T0 = std::remove_cv_t<std::remove_pointer_t<decltype(w)>>;
+                    get8<VEC, true>(q, c, stride, d, f, [&](int col, float (&v)[VEC]) {
+                        load_global<T0, VEC>(w + at + (WHOLE ? col : min(col, d - VEC)), v);
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) v[j] = WHOLE || col < d ? v[j] : 0.0f;
+                    });
+                });
             };
             float2 t2[6] = {};
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
                 float2 h[4], x[4], dh[4], dy[4], gate[4];
-                load_r(q, sh, true, h);
-                load_x(q, sx, has_x, x);
-                load_r(q, sdh, has_dh, dh);
-                load_x(q, sdy, has_dy, dy);
+                load_r(q, sh, h);
+                load_x(q, sx, x);
+                load_r(q, sdh, dh);
+                load_x(q, sdy, dy);
                 if (OWN_GATE) load_gate(q, gate);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -410,10 +475,10 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
                 float2 h[4], x[4], e[4], dy[4], gate[4];
-                load_r(q, sh, true, h);
-                load_x(q, sx, has_x, x);
-                load_r(q, sdh, has_dh, e);
-                load_x(q, sdy, has_dy, dy);
+                load_r(q, sh, h);
+                load_x(q, sx, x);
+                load_r(q, sdh, e);
+                load_x(q, sdy, dy);
                 if (OWN_GATE) load_gate(q, gate);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -447,7 +512,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
             s = s == k.stages - 1 ? 0 : s + 1;
         }
         copy_wait<0>();
-        if (warps > 1) __syncthreads();  // the next unit fills the stages again
+        block_sync();  // the next unit fills the stages again
         if (has_x)
 #pragma unroll
             for (int q = 0; q < Q; ++q)
@@ -677,9 +742,10 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
                aligned_to(post_weight, aw) && aligned_to(pre_weight, aw);
     };
     const int vec = fits(8) ? 8 : fits(2) ? 2 : 1;
-    // narrow accesses cost instructions and registers: 8 columns a thread (1023 rows of 2050
-    // float16: 34 us instead of 51)
-    const NormGradPlan p = norm_grad_plan(n, width, gate != nullptr ? gate_rows : 0, vec < 8 || n < kNormFewRows ? 8 : 16);
+    // narrow accesses cost instructions: 8 columns a thread (1023 rows of 2050 float16: 24 us
+    // instead of 31); wide ones leave fewer warps to the reduction with 16 (1100 rows of 4096
+    // bfloat16: 24.5 us instead of 29.8; 100 rows: 10.3 instead of 11.5)
+    const NormGradPlan p = norm_grad_plan(n, width, gate != nullptr ? gate_rows : 0, vec < 8 ? 8 : 16);
     CRESSO_REQUIRE(scratch != nullptr && scratch_bytes >= p.bytes, CRESSO_ESCRATCH,
                    "block_norm_grad: scratch has %lld bytes, %lld are needed", (long long)scratch_bytes,
                    (long long)p.bytes);
@@ -703,7 +769,7 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
     k.units_per_gate = p.units_per_gate;
     k.cluster = p.shape.cluster;
     k.block_width = p.shape.block_width;
-    const int stage = (int)(align_up(p.shape.block_width, 8) * 2 * (rb + xb));
+    const int stage = (int)((p.shape.threads * p.shape.elems + (vec == 1 ? 16 : 0)) * 2 * (rb + xb));
     // as many blocks an SM as the registers admit where each of them has two stages, else
     // as many stages as fit for one block
     const int share = 220 * 1024 / std::max(1, 512 / p.shape.threads) - 2048;
@@ -730,18 +796,17 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
             CRESSO_LAUNCHED("norm_grad_kernel");
             return (int)CRESSO_OK;
         };
-        if (vec == 8 && p.shape.elems == 16) {
-            const bool whole = x != nullptr && d_h != nullptr && d_y != nullptr && post_weight != nullptr &&
-                               p.shape.cluster == 1 && width == (int64_t)p.shape.threads * 16;
-            if (whole && !own) return launch(norm_grad_kernel<TR, TX, 8, 16, false, true>);
-            return own ? launch(norm_grad_kernel<TR, TX, 8, 16, true, false>)
-                       : launch(norm_grad_kernel<TR, TX, 8, 16, false, false>);
-        }
+        const bool whole = x != nullptr && d_h != nullptr && d_y != nullptr && post_weight != nullptr &&
+                           p.shape.cluster == 1 && width == (int64_t)p.shape.threads * 16;
         if (vec == 8)
-            return own ? launch(norm_grad_kernel<TR, TX, 8, 8, true, false>) : launch(norm_grad_kernel<TR, TX, 8, 8, false, false>);
+            return own     ? launch(norm_grad_kernel<TR, TX, 8, 16, true, false>)
+                   : whole ? launch(norm_grad_kernel<TR, TX, 8, 16, false, true>)
+                           : launch(norm_grad_kernel<TR, TX, 8, 16, false, false>);
         if (p.shape.elems == 16)  // a row wider than 4096
-            return own ? launch(norm_grad_kernel<TR, TX, 1, 16, true, false>)
-                       : launch(norm_grad_kernel<TR, TX, 1, 16, false, false>);
+            return vec == 2 ? (own ? launch(norm_grad_kernel<TR, TX, 2, 16, true, false>)
+                                   : launch(norm_grad_kernel<TR, TX, 2, 16, false, false>))
+                            : (own ? launch(norm_grad_kernel<TR, TX, 1, 16, true, false>)
+                                   : launch(norm_grad_kernel<TR, TX, 1, 16, false, false>));
         if (vec == 2)
             return own ? launch(norm_grad_kernel<TR, TX, 2, 8, true, false>) : launch(norm_grad_kernel<TR, TX, 2, 8, false, false>);
         return own ? launch(norm_grad_kernel<TR, TX, 1, 8, true, false>) : launch(norm_grad_kernel<TR, TX, 1, 8, false, false>);

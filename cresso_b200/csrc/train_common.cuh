@@ -202,16 +202,6 @@ __device__ __forceinline__ void with_any(const void* p, int dtype, F f) {
 
 // VEC elements of an array whose type is only known at run time; the branch is uniform.
 template <int VEC>
-__device__ __forceinline__ void load_any_vec(const void* p, int dtype, int64_t i, float (&f)[VEC]) {
-    if (dtype == CRESSO_DTYPE_F32)
-        load_global<float, VEC>(static_cast<const float*>(p) + i, f);
-    else if (dtype == CRESSO_DTYPE_F16)
-        load_global<__half, VEC>(static_cast<const __half*>(p) + i, f);
-    else
-        load_global<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(p) + i, f);
-}
-
-template <int VEC>
 __device__ __forceinline__ void store_any_vec(void* p, int dtype, int64_t i, const float (&f)[VEC]) {
     if (dtype == CRESSO_DTYPE_F32)
         store_global<float, VEC>(static_cast<float*>(p) + i, f);

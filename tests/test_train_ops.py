@@ -233,6 +233,40 @@ def test_block_norm_strides(ops):
     _check_norm_grad(ops, res, x, w[1:65], w[::2][:64], gate[:])
 
 
+@pytest.mark.parametrize("n,width", [(1, 1), (5, 3), (700, 1), (901, 33), (1300, 259), (700, 2051), (450, 4099), (3, 20003)])
+@pytest.mark.parametrize("rd,ad", PAIRS)
+def test_block_norm_odd_addresses(ops, n, width, rd, ad):
+    """Contiguous arrays at addresses that only their type aligns, each another one, between NaN:
+    nothing around an array, and nothing of another row, gets into a row."""
+    def at(offset, t):
+        flat = torch.full((t.numel() + 32,), float("nan"), dtype=t.dtype, device="cuda")
+        flat[offset:offset + t.numel()] = t.reshape(-1)
+        return flat[offset:offset + t.numel()].view(t.shape)
+
+    res, x, post, pre, gate = _norm_inputs((1, n, width), rd, ad, "channel")
+    dh, dy = _randn(25, 1, n, width, scale=0.5, dtype=rd), _randn(26, 1, n, width, scale=0.5, dtype=ad)
+    res, x, dh, dy, post, pre, gate = (at(i, t) for i, t in zip((1, 3, 5, 7, 1, 2, 5), (res, x, dh, dy, post, pre, gate)))
+    h, y = ops.block_norm(res, x, post, pre, gate, 0.35)
+    want_h, want_y = P.block_norm(res, x, post, pre, gate, 0.35, 1e-6)
+    P.check(h, *want_h, rd, "h")
+    P.check(y, *want_y, ad, "y")
+    for a in ((res, x, dh, dy, post, pre, gate), (res, x, dh, None, post, pre, gate), (res, None, None, dy, None, pre, None)):
+        want = P.block_norm_grad(*a, 0.35, 1e-6)
+        like = (rd, rd if a[1] is None else ad, F32, F32, gate.dtype)
+        if a[1] is None and ad != rd:
+            continue
+        for i, g in enumerate(ops.block_norm_grad(*a, 0.35)):
+            if g is not None:
+                P.check(g, *want[i], like[i], str(i))
+    if n > 600:
+        dh[0, n // 2, -1], dy[0, n // 3, width // 2:] = float("inf"), float("nan")
+        got = ops.block_norm_grad(res, x, dh, dy, post, pre, gate, 0.35)
+        bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+        bad[n // 2] = bad[n // 3] = True
+        for g in got[:2]:
+            assert torch.isfinite(g[0, ~bad]).all() and not torch.isfinite(g[0, bad]).all(1).any()
+
+
 def test_block_norm_empty_and_extreme(ops):
     res, x, post, pre, gate = _norm_inputs((3, 0, 16), BF16, BF16, "sample")
     h, y = ops.block_norm(res, x, post, pre, gate)
