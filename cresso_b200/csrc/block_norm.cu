@@ -44,6 +44,19 @@ static NormShape norm_shape(int64_t width, int elems) {
 // one row of 4096 takes 4.2 us instead of 6.2, and 16384 rows 142 us instead of 139.
 constexpr int64_t kNormFewRows = 8 * 148;
 
+// A thread's columns of p[0, d), VEC at an access and the accesses of a row blockDim.x VEC apart.
+// Behind the row zeros, by a choice and not by a branch, so that all the loads are in flight together.
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void load_columns(const T* p, int d, float (&v)[NV][VEC]) {
+    const int c = threadIdx.x * VEC, stride = blockDim.x * VEC;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load_global<T, VEC>(p + min(c + i * stride, d - VEC), v[i]);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] = c + i * stride < d ? v[i][j] : 0.0f;
+}
+
 // ----------------------------------------------------------------- forward ---
 //
 // A row lies in the registers of a block (of a warp up to 512 columns, four rows a block): x and residual are read once, h and y written once, two reductions between.
@@ -84,28 +97,17 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __re
     };
     float hv[NV][VEC], xv[NV][VEC];
     const int64_t at = t * width + col0;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        const int c = (v * T + tid) * VEC;
-        if (c >= d) break;
-        if (x != nullptr) load_global<TX, VEC>(x + at + c, xv[v]);
-        load_global<TR, VEC>(res + at + c, hv[v]);
-    }
-    // v *= an array's values at the thread's columns; all its loads are in flight together
+    if (x != nullptr) load_columns(x + at, d, xv);
+    load_columns(res + at, d, hv);
+    // v *= an array's values at the thread's columns
     auto multiply = [&](float (&v)[NV][VEC], const void* p, int dtype, int64_t from) {
         with_any(p, dtype, [&](auto* w) {
-            using T0 = std::remove_cv_t<std::remove_pointer_t<decltype(w)>>;
             float f[NV][VEC];
+            load_columns(w + from, d, f);
 #pragma unroll
-            for (int v0 = 0; v0 < NV; ++v0) {
-                const int c = (v0 * T + tid) * VEC;
-                if (c < d) load_global<T0, VEC>(w + from + c, f[v0]);
-            }
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int v0 = 0; v0 < NV; ++v0)
-                if ((v0 * T + tid) * VEC < d)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[v0][j] *= f[v0][j];
+                for (int j = 0; j < VEC; ++j) v[i][j] *= f[i][j];
         });
     };
     if (x != nullptr) {
@@ -113,11 +115,9 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __re
         if (a.post_w != nullptr) {
             float s = 0.0f;
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                if ((v * T + tid) * VEC >= d) break;
+            for (int v = 0; v < NV; ++v)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) s += xv[v][j] * xv[v][j];
-            }
             multiply(xv, a.post_w, a.w_dtype, col0);  // on the way while the sum is formed
             rx *= rsqrtf(row_sum(s, 0) * inv_d + a.eps);
         }
@@ -134,11 +134,9 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __re
     if (y != nullptr) {
         float s = 0.0f;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            if ((v * T + tid) * VEC >= d) break;
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) s += hv[v][j] * hv[v][j];
-        }
         multiply(hv, a.pre_w, a.w_dtype, col0);
         const float rh = rsqrtf(row_sum(s, 1) * inv_d + a.eps);
 #pragma unroll
@@ -167,7 +165,7 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __re
 // and reads the same columns, 2 or 8 at an access; rows of odd width or address (VEC 1) come as the
 // 16-byte pieces that hold them, each shifted by its own offset.  Absent arrays and columns behind
 // the row are zeros there, so that nothing but the stores is guarded: 12000 float16 rows of 2051
-// take 195 us instead of 541, of 1030 69 us instead of 106.
+// take 195 us instead of 541, 16384 bfloat16 rows of 1030 88 us instead of 107.
 // Bound by memory, then by instructions: 16384 bfloat16 rows of 4096 take 132 us and 140 us with the
 // column sums, 805 MB at 5.8 TB/s; scalar float32 arithmetic and bounds checks on every access took
 // 182 us.
