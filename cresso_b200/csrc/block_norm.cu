@@ -40,30 +40,34 @@ static NormShape norm_shape(int64_t width, int elems) {
     p.threads = (int)align_up(ceil_div(p.block_width, p.elems), 32);
     return p;
 }
-// Few rows are a matter of latency, for which 8 columns a thread are better in the forward pass:
-// one row of 4096 takes 4.2 us instead of 6.2, and 16384 rows 142 us instead of 139.
-constexpr int64_t kNormFewRows = 8 * 148;
+// Few rows, no more than there are SMs, are a matter of latency, for which 8 columns a thread are
+// better in the forward pass: one row of 4096 takes 4.2 us instead of 6.2, and 300 rows 8.2 us
+// instead of 6.2.
+constexpr int64_t kNormFewRows = 149;
 
-// A thread's columns of p[0, d), VEC at an access and the accesses of a row blockDim.x VEC apart.
-// Behind the row zeros, by a choice and not by a branch, so that all the loads are in flight together.
-template <typename T, int VEC, int NV>
-__device__ __forceinline__ void load_columns(const T* p, int d, float (&v)[NV][VEC]) {
-    const int c = threadIdx.x * VEC, stride = blockDim.x * VEC;
+// Accesses first, first + 1, .. of a thread to p[0, d): VEC columns each, the accesses of a row
+// blockDim.x VEC apart; zeros behind the row.  No access waits for another one.
+template <typename T, int VEC, int N>
+__device__ __forceinline__ void load_columns(const T* p, int d, int first, float (&v)[N][VEC]) {
+    const int stride = blockDim.x * VEC, c = threadIdx.x * VEC + first * stride;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load_global<T, VEC>(p + min(c + i * stride, d - VEC), v[i]);
+    for (int i = 0; i < N; ++i) {
+        Raw<T, VEC> u;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = c + i * stride < d ? v[i][j] : 0.0f;
+        for (int j = 0; j < (int)(sizeof(u.w) / 4); ++j) u.w[j] = 0;
+        if (c + i * stride < d) u.load_global(p + c + i * stride);
+        u.to(v[i]);
+    }
 }
 
 // ----------------------------------------------------------------- forward ---
 //
-// A row lies in the registers of a block (of a warp up to 512 columns, four rows a block): x and residual are read once, h and y written once, two reductions between.
-// Weights and gate come from L1 for every row.  Many small blocks an SM, each at another point
-// of its row, keep the memory busy without any staging.  Bound by memory: 16384 rows of 4096,
-// float32 beside bfloat16, take 139 us, 805 MB at 5.8 TB/s; three blocks of 512 threads an SM
-// instead of two spill (218 us).
+// A row lies in the registers of a block (of a warp up to 512 columns, four rows a block): x and
+// residual are read once, h and y written once, two reductions between.  Weights and gate come from
+// L1 for every row.  Many small blocks an SM, each at another point of its row, keep the memory busy
+// without any staging; a loop that leaves at the row's end held up the loads behind it.  Bound by
+// memory: 16384 rows of 4096, float32 beside bfloat16, take 125 us, 805 MB at 6.4 TB/s (139 us with
+// such loops); three blocks of 512 threads an SM instead of two spill (218 us).
 template <typename TR, typename TX, int VEC, int EL>
 __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __restrict__ res,
                                                       const TX* __restrict__ x, TR* __restrict__ h,
@@ -97,17 +101,21 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __re
     };
     float hv[NV][VEC], xv[NV][VEC];
     const int64_t at = t * width + col0;
-    if (x != nullptr) load_columns(x + at, d, xv);
-    load_columns(res + at, d, hv);
+    if (x != nullptr) load_columns(x + at, d, 0, xv);
+    load_columns(res + at, d, 0, hv);
     // v *= an array's values at the thread's columns
     auto multiply = [&](float (&v)[NV][VEC], const void* p, int dtype, int64_t from) {
         with_any(p, dtype, [&](auto* w) {
-            float f[NV][VEC];
-            load_columns(w + from, d, f);
+            constexpr int N = VEC == 1 ? 4 : NV;  // all single columns at once would spill
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+            for (int first = 0; first < NV; first += N) {
+                float f[N][VEC];
+                load_columns(w + from, d, first, f);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[i][j] *= f[i][j];
+                for (int i = 0; i < N; ++i)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[first + i][j] *= f[i][j];
+            }
         });
     };
     if (x != nullptr) {
@@ -649,7 +657,6 @@ int cresso_block_norm(const void* residual, const void* x, const void* post_weig
     NvtxRange range("block_norm n=%lld", (long long)n);
     const NormArgs a{post_weight, pre_weight, gate, n, width, gate != nullptr ? n / gate_rows : n,
                      (int)weight_dtype, (int)gate_dtype, (float)scale, (float)eps};
-    const NormShape p = norm_shape(width, n < kNormFewRows ? 8 : 16);
     const int64_t rb = dtype_bytes(res_dtype), xb = dtype_bytes(act_dtype), wb = dtype_bytes(weight_dtype),
                   gb = dtype_bytes(gate_dtype);
     // the widest accesses that the width and the addresses allow
@@ -658,6 +665,10 @@ int cresso_block_norm(const void* residual, const void* x, const void* post_weig
         return width % vec == 0 && ok(residual, rb) && ok(h, rb) && ok(x, xb) && ok(y, xb) && ok(post_weight, wb) &&
                ok(pre_weight, wb) && ok(gate, gb);
     };
+    const int vec = fits(8) ? 8 : fits(2) ? 2 : 1;
+    // single columns: 12000 bfloat16 rows of 1031 take 67 us with 8 a thread and 78 with 16, of 2051
+    // 125 and 97
+    const NormShape p = norm_shape(width, n < kNormFewRows || (vec == 1 && width <= 2048) ? 8 : 16);
     return with_norm_types(res_dtype, act_dtype, [&](auto tr, auto tx) {
         using TR = decltype(tr);
         using TX = decltype(tx);
@@ -679,12 +690,12 @@ int cresso_block_norm(const void* residual, const void* x, const void* post_weig
             return (int)CRESSO_OK;
         };
         if (p.elems == 8)
-            return fits(8)   ? launch(norm_kernel<TR, TX, 8, 8>)
-                   : fits(2) ? launch(norm_kernel<TR, TX, 2, 8>)
-                             : launch(norm_kernel<TR, TX, 1, 8>);
-        return fits(8)   ? launch(norm_kernel<TR, TX, 8, 16>)
-               : fits(2) ? launch(norm_kernel<TR, TX, 2, 16>)
-                         : launch(norm_kernel<TR, TX, 1, 16>);
+            return vec == 8   ? launch(norm_kernel<TR, TX, 8, 8>)
+                   : vec == 2 ? launch(norm_kernel<TR, TX, 2, 8>)
+                              : launch(norm_kernel<TR, TX, 1, 8>);
+        return vec == 8   ? launch(norm_kernel<TR, TX, 8, 16>)
+               : vec == 2 ? launch(norm_kernel<TR, TX, 2, 16>)
+                          : launch(norm_kernel<TR, TX, 1, 16>);
     });
 }
 
