@@ -268,6 +268,17 @@ __device__ __forceinline__ void write_row(TO* __restrict__ out, int64_t width, i
     }
 }
 
+// p[0, n) = 0 by `threads` threads, of which this is number t: 16 bytes a store but for the ends
+template <typename T>
+__device__ __forceinline__ void clear_span(T* p, int n, int t, int threads) {
+    constexpr int kPiece = 16 / (int)sizeof(T);
+    const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) % 16 / sizeof(T)));
+    const int pieces = (n - head) / kPiece;
+    for (int i = t; i < head; i += threads) p[i] = T(0.0f);
+    for (int i = t; i < pieces; i += threads) reinterpret_cast<uint4*>(p + head)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = head + pieces * kPiece + t; i < n; i += threads) p[i] = T(0.0f);
+}
+
 struct GradSums {
     const int2* range;  // (begin, end) of each row in the order
     const int2* order;  // (position, row | kLastOfRow)
@@ -284,8 +295,10 @@ template <typename TG, typename TO, int VEC>
 __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG* __restrict__ g,
                                                            TO* __restrict__ out) {
     constexpr int U = kSumCols / VEC;
-    constexpr int kDepth = 16 / sizeof(TG);  // positions in 32 KB of shared memory
-    __shared__ __align__(16) TG ring[kDepth * kThreads * kSumCols];
+    // single 16-bit columns come as the aligned words that hold them, which cp.async can copy
+    constexpr bool kWords = VEC * sizeof(TG) == 2;
+    constexpr int kDepth = kWords ? 4 : 16 / sizeof(TG);  // positions in 32 KB of shared memory
+    __shared__ __align__(16) TG ring[kDepth * kThreads * kSumCols * (kWords ? 2 : 1)];
     const int tpr = k.tpr;
     const int64_t item = (int64_t)blockIdx.x * (kThreads / tpr) + threadIdx.x / tpr;
     const int64_t c0 = (int64_t)blockIdx.y * tpr * kSumCols + (int64_t)(threadIdx.x & (tpr - 1)) * VEC;
@@ -303,7 +316,15 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
         }
 #pragma unroll
         for (int i = 0; i < kEmptyRows; ++i)
-            if (empty[i]) write_row<TO, VEC, U>(out + (r0 + i) * k.width, k.width, c0, tpr, 1.0f, 0, acc);
+            if (empty[i]) {
+                if constexpr (VEC == kSumCols) {
+                    write_row<TO, VEC, U>(out + (r0 + i) * k.width, k.width, c0, tpr, 1.0f, 0, acc);
+                } else {
+                    const int64_t c = (int64_t)blockIdx.y * tpr * kSumCols;
+                    clear_span(out + (r0 + i) * k.width + c, (int)min(k.width - c, (int64_t)tpr * kSumCols),
+                               threadIdx.x & (tpr - 1), tpr);
+                }
+            }
         return;
     }
     const int total = *k.total;
@@ -317,13 +338,28 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
     const int to = last_long ? b : lr.x >= a ? lr.y : from;
     if (from >= to) return;
     // each thread fetches its columns of the next kDepth - 1 positions ahead
-    TG* mine = ring + threadIdx.x * VEC;
+    TG* mine = ring + threadIdx.x * (kWords ? 2 : VEC);
+    constexpr int kNext = kThreads * (kWords ? 2 : VEC);
     auto fetch = [&](int j, int slot) {
         const TG* src = g + (int64_t)k.order[j].x * k.stride + c0;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (c0 + (int64_t)u * tpr * VEC < k.width)
-                copy_vec<TG, VEC>(mine + (slot * U + u) * kThreads * VEC, src + u * tpr * VEC);
+            if (c0 + (int64_t)u * tpr * VEC < k.width) {
+                TG* dst = mine + (slot * U + u) * kNext;
+                if constexpr (kWords) {
+                    const uintptr_t at = reinterpret_cast<uintptr_t>(src + u * tpr), word = at & ~(uintptr_t)3;
+                    const bool both = (at & 2) != 0 || c0 + u * tpr + 1 < k.width;  // the row's end is not passed
+                    if (word >= reinterpret_cast<uintptr_t>(g))
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                                         (uint32_t)__cvta_generic_to_shared(dst)),
+                                     "l"(word), "r"(both ? 4 : 2)
+                                     : "memory");
+                    else  // the gradient starts inside the word
+                        dst[1] = src[u * tpr];
+                } else {
+                    copy_vec<TG, VEC>(dst, src + u * tpr * VEC);
+                }
+            }
     };
 #pragma unroll
     for (int p = 0; p < kDepth - 1; ++p) {
@@ -332,16 +368,19 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
     }
     int slot = 0;
     for (int j = from; j < to; ++j) {
-        const int mark = k.order[j].y;
+        const int2 entry = k.order[j];
+        const int mark = entry.y;
+        // the half of its word that the thread's first column is in
+        const int half = kWords ? (int)(reinterpret_cast<uintptr_t>(g + (int64_t)entry.x * k.stride + c0) >> 1) : 0;
         copy_wait<kDepth - 2>();
+        // columns behind the row as well, whose sums are not written
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (c0 + (int64_t)u * tpr * VEC < k.width) {
-                float f[VEC];
-                load_vec<TG, VEC>(mine + (slot * U + u) * kThreads * VEC, f);
+        for (int u = 0; u < U; ++u) {
+            float f[VEC];
+            load_vec<TG, VEC>(mine + (slot * U + u) * kNext + (kWords ? (half + u * tpr) & 1 : 0), f);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[u][i] += f[i];
-            }
+            for (int i = 0; i < VEC; ++i) acc[u][i] += f[i];
+        }
         if (j + kDepth - 1 < to) fetch(j + kDepth - 1, slot == 0 ? kDepth - 1 : slot - 1);
         copy_commit();
         slot = slot == kDepth - 1 ? 0 : slot + 1;

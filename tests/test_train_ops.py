@@ -120,6 +120,31 @@ def test_embedding_grad_strides_and_ids(ops):
     assert ops.embedding_grad(g, far, 0).shape == (0, 8)
 
 
+@pytest.mark.parametrize("width", [1, 2, 7, 8, 9, 33, 130, 515, 2050, 2051, 4095])
+@pytest.mark.parametrize("gd,od", [(BF16, BF16), (F16, F32), (F32, BF16), (F32, F32)])
+def test_embedding_odd_addresses(ops, width, gd, od):
+    """Gradients and tables that only their type aligns, with gaps between the rows: what lies
+    around them is NaN, and the bytes around the result stay."""
+    n, rows, first = 700, 90, 3
+    flat = torch.full((n * (width + 1) + 16,), float("nan"), dtype=gd, device="cuda")
+    tok = _tokens(18, n, 60)
+    for offset, stride in ((1, width), (5, width + 1), (0, width)):
+        flat.fill_(float("nan"))
+        g = flat[offset:offset + n * stride].view(n, stride)[:, :width]
+        g.copy_(_randn(19, n, width, dtype=gd))
+        value, bound = P.embedding_grad(g, tok, rows, 0.5)
+        P.check(ops.embedding_grad(g, tok, rows, 0.5, dtype=od), value, bound, od)
+        value, bound = P.gather(g, tok, 0.5, 0, od)
+        P.check(ops.embedding_gather(g, tok, 0.5, dtype=od), value, bound, od)
+        around = torch.full((rows * width + 16,), 7.0, dtype=od, device="cuda")
+        into = around[first:first + rows * width].view(rows, width)
+        into.copy_(_randn(20, rows, width, dtype=od))
+        value, bound = P.embedding_grad(g, tok, rows, 0.5, into=into)
+        ops.embedding_grad(g, tok, rows, 0.5, into=into)
+        P.check(into, value, bound, od)
+        assert (around[:first] == 7).all() and (around[first + rows * width:] == 7).all()
+
+
 def test_embedding_rows_beyond_32_bit_offsets(ops):
     rows, width = 530001, 4104  # 2.17e9 elements
     w = torch.zeros(rows, width, dtype=BF16, device="cuda")
