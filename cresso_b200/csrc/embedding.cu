@@ -340,8 +340,8 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
     // each thread fetches its columns of the next kDepth - 1 positions ahead
     TG* mine = ring + threadIdx.x * (kWords ? 2 : VEC);
     constexpr int kNext = kThreads * (kWords ? 2 : VEC);
-    auto fetch = [&](int j, int slot) {
-        const TG* src = g + (int64_t)k.order[j].x * k.stride + c0;
+    auto fetch = [&](int position, int slot) {
+        const TG* src = g + (int64_t)position * k.stride + c0;
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (c0 + (int64_t)u * tpr * VEC < k.width) {
@@ -361,14 +361,19 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
                 }
             }
     };
+    int early[kDepth - 1];
+#pragma unroll
+    for (int p = 0; p < kDepth - 1; ++p) early[p] = k.order[min(from + p, to - 1)].x;
 #pragma unroll
     for (int p = 0; p < kDepth - 1; ++p) {
-        if (from + p < to) fetch(from + p, p);
+        if (from + p < to) fetch(early[p], p);
         copy_commit();
     }
+    // entries of the order are read an iteration before they are used
+    int2 entry = k.order[from];
+    int next = k.order[min(from + kDepth - 1, to - 1)].x;
     int slot = 0;
     for (int j = from; j < to; ++j) {
-        const int2 entry = k.order[j];
         const int mark = entry.y;
         // the half of its word that the thread's first column is in
         const int half = kWords ? (int)(reinterpret_cast<uintptr_t>(g + (int64_t)entry.x * k.stride + c0) >> 1) : 0;
@@ -381,8 +386,10 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
 #pragma unroll
             for (int i = 0; i < VEC; ++i) acc[u][i] += f[i];
         }
-        if (j + kDepth - 1 < to) fetch(j + kDepth - 1, slot == 0 ? kDepth - 1 : slot - 1);
+        if (j + kDepth - 1 < to) fetch(next, slot == 0 ? kDepth - 1 : slot - 1);
         copy_commit();
+        next = k.order[min(j + kDepth, to - 1)].x;
+        entry = k.order[min(j + 1, to - 1)];
         slot = slot == kDepth - 1 ? 0 : slot + 1;
         if (mark >= 0 && j + 1 < to) continue;
         // the row ends here, or the item does: a long row leaves a partial row
