@@ -254,17 +254,17 @@ constexpr int kJoinCols = 128;
 
 // out row = scale * acc (+ out row)
 template <typename TO, int VEC, int U>
-__device__ __forceinline__ void write_row(TO* __restrict__ out, int64_t width, int64_t c0, int tpr, float scale,
-                                          int accumulate, float (&acc)[U][VEC]) {
+__device__ __forceinline__ void write_row(TO* __restrict__ out, int64_t c0, int left, int tpr, float scale, int accumulate,
+                                          float (&acc)[U][VEC]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int64_t c = c0 + (int64_t)u * tpr * VEC;
-        if (c >= width) continue;
+        const int c = u * tpr * VEC;
+        if (c >= left) continue;
         float old[VEC] = {};
-        if (accumulate) load_vec<TO, VEC>(out + c, old);
+        if (accumulate) load_vec<TO, VEC>(out + c0 + c, old);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[u][i] = acc[u][i] * scale + old[i];
-        store_global<TO, VEC>(out + c, acc[u]);
+        store_global<TO, VEC>(out + c0 + c, acc[u]);
     }
 }
 
@@ -277,6 +277,13 @@ __device__ __forceinline__ void clear_span(T* p, int n, int t, int threads) {
     for (int i = t; i < head; i += threads) p[i] = T(0.0f);
     for (int i = t; i < pieces; i += threads) reinterpret_cast<uint4*>(p + head)[i] = make_uint4(0, 0, 0, 0);
     for (int i = head + pieces * kPiece + t; i < n; i += threads) p[i] = T(0.0f);
+}
+
+// Begins to copy the first `bytes` (2 or 4) of an aligned word to shared memory.
+__device__ __forceinline__ void copy_word(void* dst, const char* word, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(word),
+                 "r"(bytes)
+                 : "memory");
 }
 
 struct GradSums {
@@ -302,6 +309,7 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
     const int tpr = k.tpr;
     const int64_t item = (int64_t)blockIdx.x * (kThreads / tpr) + threadIdx.x / tpr;
     const int64_t c0 = (int64_t)blockIdx.y * tpr * kSumCols + (int64_t)(threadIdx.x & (tpr - 1)) * VEC;
+    const int left = (int)min(k.width - c0, (int64_t)tpr * kSumCols);  // columns from the thread's first one on
     float acc[U][VEC] = {};
     next_kernel_may_start();
     previous_kernel_done();
@@ -318,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
         for (int i = 0; i < kEmptyRows; ++i)
             if (empty[i]) {
                 if constexpr (VEC == kSumCols) {
-                    write_row<TO, VEC, U>(out + (r0 + i) * k.width, k.width, c0, tpr, 1.0f, 0, acc);
+                    write_row<TO, VEC, U>(out + (r0 + i) * k.width, c0, left, tpr, 1.0f, 0, acc);
                 } else {
                     const int64_t c = (int64_t)blockIdx.y * tpr * kSumCols;
                     clear_span(out + (r0 + i) * k.width + c, (int)min(k.width - c, (int64_t)tpr * kSumCols),
@@ -338,29 +346,29 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
     const int to = last_long ? b : lr.x >= a ? lr.y : from;
     if (from >= to) return;
     // each thread fetches its columns of the next kDepth - 1 positions ahead
-    TG* mine = ring + threadIdx.x * (kWords ? 2 : VEC);
     constexpr int kNext = kThreads * (kWords ? 2 : VEC);
+    TG* mine = ring + threadIdx.x * (kWords ? 2 : VEC);
     auto fetch = [&](int position, int slot) {
         const TG* src = g + (int64_t)position * k.stride + c0;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (c0 + (int64_t)u * tpr * VEC < k.width) {
-                TG* dst = mine + (slot * U + u) * kNext;
-                if constexpr (kWords) {
-                    const uintptr_t at = reinterpret_cast<uintptr_t>(src + u * tpr), word = at & ~(uintptr_t)3;
-                    const bool both = (at & 2) != 0 || c0 + u * tpr + 1 < k.width;  // the row's end is not passed
-                    if (word >= reinterpret_cast<uintptr_t>(g))
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
-                                         (uint32_t)__cvta_generic_to_shared(dst)),
-                                     "l"(word), "r"(both ? 4 : 2)
-                                     : "memory");
-                    else  // the gradient starts inside the word
-                        dst[1] = src[u * tpr];
-                } else {
-                    copy_vec<TG, VEC>(dst, src + u * tpr * VEC);
-                }
+        TG* dst = mine + slot * U * kNext;
+        if constexpr (kWords) {  // tpr is even: the same half of each word
+            const bool upper = (reinterpret_cast<uintptr_t>(src) & 2) != 0;
+            const char* word = reinterpret_cast<const char*>(src) - (upper ? 2 : 0);
+            if (upper && position == 0 && c0 == 0) {  // the gradient starts inside the word
+                dst[1] = src[0];
+            } else if (left > 0) {
+                copy_word(dst, word, upper || left > 1 ? 4 : 2);
             }
+#pragma unroll
+            for (int u = 1; u < U; ++u)
+                if (u * tpr < left) copy_word(dst + u * kNext, word + 2 * u * tpr, upper || u * tpr + 1 < left ? 4 : 2);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (u * tpr * VEC < left) copy_vec<TG, VEC>(dst + u * kNext, src + u * tpr * VEC);
+        }
     };
+#pragma unroll
     int early[kDepth - 1];
 #pragma unroll
     for (int p = 0; p < kDepth - 1; ++p) early[p] = k.order[min(from + p, to - 1)].x;
@@ -375,14 +383,14 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
     int slot = 0;
     for (int j = from; j < to; ++j) {
         const int mark = entry.y;
-        // the half of its word that the thread's first column is in
-        const int half = kWords ? (int)(reinterpret_cast<uintptr_t>(g + (int64_t)entry.x * k.stride + c0) >> 1) : 0;
+        // the half of a word that the thread's columns are in
+        const int half = kWords ? (int)(reinterpret_cast<uintptr_t>(g + (int64_t)entry.x * k.stride + c0) >> 1 & 1) : 0;
         copy_wait<kDepth - 2>();
         // columns behind the row as well, whose sums are not written
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float f[VEC];
-            load_vec<TG, VEC>(mine + (slot * U + u) * kNext + (kWords ? (half + u * tpr) & 1 : 0), f);
+            load_vec<TG, VEC>(mine + (slot * U + u) * kNext + half, f);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) acc[u][i] += f[i];
         }
@@ -396,9 +404,9 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
         const int row = mark & (int)~kLastOfRow;
         if ((row == first && first_long) || (row == last && last_long))
             write_row<float, VEC, U>(k.partial + (2 * item + ((row == first ? fr.x : lr.x) > a ? 1 : 0)) * k.pitch,
-                                     k.width, c0, tpr, 1.0f, 0, acc);
+                                     c0, left, tpr, 1.0f, 0, acc);
         else
-            write_row<TO, VEC, U>(out + (int64_t)row * k.width, k.width, c0, tpr, k.scale, k.accumulate, acc);
+            write_row<TO, VEC, U>(out + (int64_t)row * k.width, c0, left, tpr, k.scale, k.accumulate, acc);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -588,7 +596,7 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
             using TO = decltype(to);
             const int rc = with_vec(width, grad_stride, grad, sizeof(TG), out, sizeof(TO), [&](auto vec) {
                 constexpr int VEC = decltype(vec)::value;
-                k.tpr = threads_per_row(width, kSumCols);
+                k.tpr = std::max(2, threads_per_row(width, kSumCols));
                 const dim3 grid((unsigned)ceil_div(items, kThreads / k.tpr),
                                 (unsigned)ceil_div(width, k.tpr * kSumCols));
                 CRESSO_CUDA(launch_overlapped(grad_kernel<TG, TO, VEC>, grid, kThreads, 0, s, k,
