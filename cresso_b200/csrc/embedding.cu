@@ -368,7 +368,6 @@ __global__ void __launch_bounds__(kThreads, 5) grad_kernel(GradSums k, const TG*
                 if (u * tpr * VEC < left) copy_vec<TG, VEC>(dst + u * kNext, src + u * tpr * VEC);
         }
     };
-#pragma unroll
     int early[kDepth - 1];
 #pragma unroll
     for (int p = 0; p < kDepth - 1; ++p) early[p] = k.order[min(from + p, to - 1)].x;
@@ -475,9 +474,14 @@ __global__ void __launch_bounds__(kThreads) grad_join_kernel(GradSums k, TO* __r
     }
 }
 
-// Positions of a tile: few where there are few tokens, so that their latencies overlap (2047 tokens:
-// 11 us with 8, 20 us with 32), many where there are many (16384 tokens: 50 us with 32, 58 us with 8).
-static int grad_tile(int64_t n) { return n <= 4096 ? 8 : n <= 32768 ? 32 : 128; }
+// Positions of a tile: 8 where few elements leave SMs idle, so that more latencies overlap (2047
+// tokens of 1024: 11 us with 8, 20 us with 32; 16384 of 512: 31 us and 47 us), 32 where there are
+// many, since a tile costs partial rows (16384 of 4096: 126 us with 32, 133 us with 8).  Few tiles
+// at last, for a frequent row's partial rows are one chain (2000000 tokens of 64: 1015 us with 128,
+// 1013 us with 32, 1143 us with 8).
+static int grad_tile(int64_t n, int64_t width) {
+    return n <= 4096 || (n <= 131072 && n * width <= ((int64_t)1 << 24)) ? 8 : n <= 1048576 ? 32 : 128;
+}
 
 }  // namespace cresso
 
@@ -522,7 +526,7 @@ struct GradScratch {
 };
 static GradScratch grad_scratch(int64_t n, int64_t rows, int64_t width) {
     GradScratch p{};
-    p.tile = grad_tile(n);
+    p.tile = grad_tile(n, width);
     p.tiles = ceil_div(n, p.tile);
     p.order = align_up(8 * rows, 256);
     p.total = p.order + align_up(8 * n, 256);

@@ -104,6 +104,16 @@ def test_embedding_grad_uneven_rows(ops, rows, width, n):
     P.check(ops.embedding_grad(g, tok, rows // 3, row0=rows // 3, dtype=F32), value, bound, F32)
 
 
+@pytest.mark.parametrize("rows,width,n", [(400, 128, 131072), (400, 129, 131072), (3000, 9, 200001), (60, 3, 1048577)])
+def test_embedding_grad_many_tokens(ops, rows, width, n):
+    """Rows that span many tiles, at the bounds of the tiles' sizes."""
+    gen = torch.Generator(device="cuda").manual_seed(19)
+    tok = (torch.rand(n, generator=gen, device="cuda", dtype=torch.float64) ** 3 * rows).long()
+    g = _randn(21, n, width, dtype=F16)
+    value, bound = P.embedding_grad(g, tok, rows, 1.0)
+    P.check(ops.embedding_grad(g, tok, rows, dtype=F32), value, bound, F32)
+
+
 def test_embedding_grad_strides_and_ids(ops):
     tok = _tokens(11, (5, 13), 60, torch.int32, low=-5)
     base = _randn(12, 65, 80, dtype=F16)
