@@ -243,9 +243,10 @@ __global__ void __launch_bounds__(kSortMaxWarps * 32) sort_kernel(TokenWindow wi
 // rows, one that reaches it from the left (partial 2 tile) and one that begins inside and
 // leaves it to the right (partial 2 tile + 1).  Further items write the rows without a
 // token, kEmptyRows rows each.
-// Bound by memory: 16384 bfloat16 rows of 4096 into (32000, 4096) float32 take 120 us, of which the
-// empty rows are 70 us (a plain fill of the whole gradient takes 72) and the tiles 50 us (230 MB at
-// 4.6 TB/s).  One row an item took 1264 us (a frequent row is one long chain), rows in order with
+// Bound by memory: 16384 bfloat16 rows of 4096 into (32000, 4096) float32 take 116 us, of which the
+// empty rows are 70 us (a plain fill of the whole gradient takes 72) and the tiles 46 us (230 MB at
+// 5 TB/s); entries of the order read when they were needed cost 3 us.  Single columns cost
+// instructions: 16384 bfloat16 rows of 2051 into 50000 take 160 us with the sort, of 2048 62 us.  One row an item took 1264 us (a frequent row is one long chain), rows in order with
 // their own tiles 188 us.  Rows in flight in registers spilled (163 us); in shared memory, fetched
 // by the thread that adds them, they need neither registers nor a barrier.
 constexpr int kEmptyRows = 8;
