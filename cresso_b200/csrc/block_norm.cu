@@ -25,6 +25,7 @@ struct NormArgs {
 };
 
 constexpr int kNormMaxWidth = CRESSO_TRAIN_MAX_NORM_WIDTH;
+constexpr int kNormStageBytes = 220 * 1024;  // shared memory of a backward block's stages at most
 
 // Columns of a thread (EL, 16 or 8), threads and blocks of a row: a row of more than 512 EL
 // columns is cut over a cluster of 2 to 8 blocks, which add their sums through distributed
@@ -781,15 +782,17 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
     const int stage = (int)((p.shape.threads * p.shape.elems + (vec == 1 ? 16 : 0)) * 2 * (rb + xb));
     // as many blocks an SM as the registers admit where each of them has two stages, else
     // as many stages as fit for one block
-    const int share = 220 * 1024 / std::max(1, 512 / p.shape.threads) - 2048;
-    k.stages = 2 * stage <= share ? std::min(4, share / stage) : std::min(4, 220 * 1024 / stage);
+    const int share = kNormStageBytes / std::max(1, 512 / p.shape.threads) - 2048;
+    k.stages = 2 * stage <= share ? std::min(4, share / stage) : std::min(4, kNormStageBytes / stage);
     const int smem = k.stages * stage;
     const int rc = with_norm_types(res_dtype, act_dtype, [&](auto tr, auto tx) {
         using TR = decltype(tr);
         using TX = decltype(tx);
         auto launch = [&](auto kernel) {
-            if (smem > 40 * 1024)  // with the static part, 48 KB need no leave
-                CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            // with the static part, 48 KB need no leave; one bound for all calls, since a kernel's bound
+            // is shared by the host's threads and another one's smaller stages must not lower it
+            if (smem > 40 * 1024)
+                CRESSO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormStageBytes));
             cudaLaunchConfig_t cfg{};
             cfg.gridDim = dim3((unsigned)(p.workers * p.shape.cluster));
             cfg.blockDim = dim3((unsigned)p.shape.threads);
