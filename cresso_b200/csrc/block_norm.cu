@@ -282,14 +282,20 @@ __device__ __forceinline__ void copy_span(T* dst, const T* array, const T* src, 
     }
 }
 
-// WHOLE: x, d_h, d_y and post_weight are there, and the threads' columns are the row's.
-template <typename TR, typename TX, int VEC, int EL, bool OWN_GATE, bool WHOLE>
+// What a call has.  kAllWhole: x, d_h, d_y and post_weight, and the threads' columns are the row's.
+// kParts: d_y, and post_weight or no x.  kFewParts: no d_y, or x without post_weight; then e = d_h
+// whatever h holds, or d_x = dq whatever x holds, so that their arithmetic is left out instead of
+// multiplied by zero, which infinities, NaN and rows of zeros (eps 0) would turn into NaN.  A form of
+// its own, since these branches cost the others 2 to 10% (12000 float16 rows of 2050: 148 us to 161).
+enum NormForm { kAllWhole, kParts, kFewParts };
+template <typename TR, typename TX, int VEC, int EL, bool OWN_GATE, NormForm FORM>
 __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
     next_kernel_may_start();
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ __align__(16) float red[2][16 * 8];
     __shared__ __align__(16) float peer_sums[2][8];
     namespace cg = cooperative_groups;
+    constexpr bool WHOLE = FORM == kAllWhole;
     const NormArgs& a = k.a;
     const int tid = threadIdx.x, T = blockDim.x, warps = T >> 5;
     const int64_t width = a.width;
@@ -301,6 +307,8 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
     const float inv_d = 1.0f / (float)width;
     const bool has_x = WHOLE || k.x != nullptr, has_dh = WHOLE || k.dh != nullptr, has_dy = WHOLE || k.dy != nullptr;
     const bool has_post = WHOLE || a.post_w != nullptr;
+    // whether h and d_y, and the second mean's sums, take part
+    const bool use_h = FORM != kFewParts || has_dy, use_mean = FORM != kFewParts || has_post;
     const int64_t pitch = align_up(width, 8);
     // a stage: h, dh, x, dy
     const int stage_bytes = slots * 2 * (int)(sizeof(TR) + sizeof(TX));
@@ -315,7 +323,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
         TR *sh = stage_r(s, 0), *sdh = stage_r(s, 1);
         TX *sx = stage_x(s, 0), *sdy = stage_x(s, 1);
         if constexpr (kSpans) {
-            copy_span(sh, static_cast<const TR*>(k.h), h, d);
+            if (use_h) copy_span(sh, static_cast<const TR*>(k.h), h, d);
             if (has_x) copy_span(sx, static_cast<const TX*>(k.x), x, d);
             if (has_dh) copy_span(sdh, static_cast<const TR*>(k.dh), dh, d);
             if (has_dy) copy_span(sdy, static_cast<const TX*>(k.dy), dy, d);
@@ -325,7 +333,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
         for (int i = 0; i < EL / VEC; ++i) {
             const int col = c + i * stride;
             if (!WHOLE && col >= d) break;
-            copy_vec<TR, VEC>(sh + col, h + col);
+            if (use_h) copy_vec<TR, VEC>(sh + col, h + col);
             if (has_x) copy_vec<TX, VEC>(sx + col, x + col);
             if (has_dh) copy_vec<TR, VEC>(sdh + col, dh + col);
             if (has_dy) copy_vec<TX, VEC>(sdy + col, dy + col);
@@ -365,7 +373,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
             for (int i = tid + (has_dh ? d : 0); i < slots; i += T) stage_r(st, 1)[i] = TR(0.0f);
             for (int i = tid + (has_x ? d : 0); i < slots; i += T) stage_x(st, 0)[i] = TX(0.0f);
             for (int i = tid + (has_dy ? d : 0); i < slots; i += T) stage_x(st, 1)[i] = TX(0.0f);
-            for (int i = tid + d; i < slots; i += T) stage_r(st, 0)[i] = TR(0.0f);
+            for (int i = tid + (use_h ? d : 0); i < slots; i += T) stage_r(st, 0)[i] = TR(0.0f);
         }
         block_sync();
     }
@@ -428,6 +436,30 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
                 float2 h[4], x[4], dh[4], dy[4], gate[4];
+                if constexpr (FORM == kFewParts) {
+                    if (use_h) {
+                        load_r(q, sh, h);
+                        load_x(q, sdy, dy);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            t2[0] = __ffma2_rn(h[j], h[j], t2[0]);
+                            t2[2] = __ffma2_rn(__fmul2_rn(dy[j], pre[q][j]), h[j], t2[2]);
+                        }
+                    }
+                    if (use_mean) {  // and no d_y
+                        load_x(q, sx, x);
+                        load_r(q, sdh, dh);
+                        if (OWN_GATE) load_gate(q, gate);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float2 ax = __fmul2_rn(post[q][j], x[j]);
+                            if (OWN_GATE) ax = __fmul2_rn(ax, gate[j]);
+                            t2[1] = __ffma2_rn(x[j], x[j], t2[1]);
+                            t2[3] = __ffma2_rn(ax, dh[j], t2[3]);
+                        }
+                    }
+                    continue;
+                }
                 load_r(q, sh, h);
                 load_x(q, sx, x);
                 load_r(q, sdh, dh);
@@ -471,7 +503,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
                 if (r + k.stages - 1 < r1) fetch(free_stage, r + k.stages - 1);
                 copy_commit();
             }
-            const float rh = rsqrtf(t[0] * inv_d + a.eps);
+            const float rh = use_h ? rsqrtf(t[0] * inv_d + a.eps) : 0.0f;
             const float m1 = t[2] * rh * inv_d;
             float rx = 1.0f, m2 = 0.0f;
             if (has_post) {
@@ -490,7 +522,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float2 n = __fmul2_rn(h[j], rh2), p = __fmul2_rn(x[j], rx2);
-                    e[j] = __ffma2_rn(rh2, __ffma2_rn(n, minus_m1, __fmul2_rn(dy[j], pre[q][j])), e[j]);
+                    if (use_h) e[j] = __ffma2_rn(rh2, __ffma2_rn(n, minus_m1, __fmul2_rn(dy[j], pre[q][j])), e[j]);
                     float2 dq = __fmul2_rn(post[q][j], e[j]);
                     if (OWN_GATE) {
                         dy[j] = __fmul2_rn(dy[j], n);
@@ -502,7 +534,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(NormGrad k) {
                         sum_pre[q][j] = __ffma2_rn(dy[j], n, sum_pre[q][j]);
                         sum_b[q][j] = __ffma2_rn(e[j], p, sum_b[q][j]);
                     }
-                    x[j] = __fmul2_rn(rx2, __ffma2_rn(p, minus_m2, dq));  // d_x
+                    x[j] = use_mean ? __fmul2_rn(rx2, __ffma2_rn(p, minus_m2, dq)) : dq;  // d_x
                 }
                 put8<VEC, WHOLE>(q, c, stride, d, e, [&](int col, const float (&v)[VEC]) {
                     store_global<TR, VEC>(static_cast<TR*>(k.dres) + at + col, v);
@@ -810,18 +842,23 @@ int cresso_block_norm_grad(const void* h, const void* x, const void* d_h, const 
         };
         const bool whole = x != nullptr && d_h != nullptr && d_y != nullptr && post_weight != nullptr &&
                            p.shape.cluster == 1 && width == (int64_t)p.shape.threads * 16;
-        if (vec == 8)
-            return own     ? launch(norm_grad_kernel<TR, TX, 8, 16, true, false>)
-                   : whole ? launch(norm_grad_kernel<TR, TX, 8, 16, false, true>)
-                           : launch(norm_grad_kernel<TR, TX, 8, 16, false, false>);
-        if (p.shape.elems == 16)  // a row wider than 4096
-            return vec == 2 ? (own ? launch(norm_grad_kernel<TR, TX, 2, 16, true, false>)
-                                   : launch(norm_grad_kernel<TR, TX, 2, 16, false, false>))
-                            : (own ? launch(norm_grad_kernel<TR, TX, 1, 16, true, false>)
-                                   : launch(norm_grad_kernel<TR, TX, 1, 16, false, false>));
-        if (vec == 2)
-            return own ? launch(norm_grad_kernel<TR, TX, 2, 8, true, false>) : launch(norm_grad_kernel<TR, TX, 2, 8, false, false>);
-        return own ? launch(norm_grad_kernel<TR, TX, 1, 8, true, false>) : launch(norm_grad_kernel<TR, TX, 1, 8, false, false>);
+        auto with_form = [&](auto form) {
+            constexpr NormForm F = decltype(form)::value;
+            if (vec == 8)
+                return own ? launch(norm_grad_kernel<TR, TX, 8, 16, true, F>) : launch(norm_grad_kernel<TR, TX, 8, 16, false, F>);
+            if (p.shape.elems == 16)  // a row wider than 4096
+                return vec == 2 ? (own ? launch(norm_grad_kernel<TR, TX, 2, 16, true, F>)
+                                       : launch(norm_grad_kernel<TR, TX, 2, 16, false, F>))
+                                : (own ? launch(norm_grad_kernel<TR, TX, 1, 16, true, F>)
+                                       : launch(norm_grad_kernel<TR, TX, 1, 16, false, F>));
+            if (vec == 2)
+                return own ? launch(norm_grad_kernel<TR, TX, 2, 8, true, F>) : launch(norm_grad_kernel<TR, TX, 2, 8, false, F>);
+            return own ? launch(norm_grad_kernel<TR, TX, 1, 8, true, F>) : launch(norm_grad_kernel<TR, TX, 1, 8, false, F>);
+        };
+        if (vec == 8 && !own && whole) return launch(norm_grad_kernel<TR, TX, 8, 16, false, kAllWhole>);
+        if (d_y == nullptr || (x != nullptr && post_weight == nullptr))
+            return with_form(std::integral_constant<NormForm, kFewParts>());
+        return with_form(std::integral_constant<NormForm, kParts>());
     });
     if (rc != CRESSO_OK) return rc;
     float* post_rows = reinterpret_cast<float*>(base + p.off_post);

@@ -5,6 +5,8 @@ import threading
 import pytest
 import torch
 
+import _train_plain as P
+
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 gpu = pytest.mark.gpu
 
@@ -60,3 +62,34 @@ def test_backward_norms_of_host_threads(ops):
     assert not errors, errors
     for _, out, want, _ in calls:
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@gpu
+@pytest.mark.parametrize("width", [7, 130, 520, 2051, 4096, 4104, 8200, 20001])
+@pytest.mark.parametrize("gate_shape", [None, "channel", "full"])
+@pytest.mark.parametrize("rd,ad", [(F32, BF16), (F16, F16)])
+def test_backward_norm_does_not_read_what_it_does_not_need(ops, width, gate_shape, rd, ad):
+    """Without d_y the gradient of the residual is d_h, and d_x has nothing of h; without post_weight d_x
+    has nothing of x: infinities, NaN and rows of zeros in them (with eps 0) do not get there."""
+    n, inf, nan = 6, float("inf"), float("nan")
+    h, x = _randn(1, n, width, dtype=rd), _randn(2, n, width, dtype=ad)
+    dh, dy = _randn(3, n, width, dtype=rd), _randn(4, n, width, dtype=ad)
+    post, pre = 1 + _randn(5, width, scale=0.2), 1 + _randn(6, width, scale=0.2)
+    gate = None if gate_shape is None else _randn(7, *((width,) if gate_shape == "channel" else (n, width)), dtype=ad)
+    odd_h, odd_x = h.clone(), x.clone()
+    for t in (odd_h, odd_x):
+        t[1, width // 2], t[2, 0], t[3], t[5] = inf, nan, 0, -inf
+    for args in ((odd_h, x, dh, None, post, pre, gate), (odd_h, x, dh, None, None, None, gate),
+                 (odd_h, None, dh, None, None, None, None), (odd_h, odd_x, dh, None, None, pre, gate),
+                 (h, odd_x, dh, dy, None, pre, gate), (h, odd_x, None, dy, None, pre, gate)):
+        if args[1] is None and rd != ad:
+            continue
+        want = P.block_norm_grad(*args, 0.35, 0.0)
+        got = ops.block_norm_grad(*args, 0.35, 0.0)
+        types = (rd, ad, post.dtype, pre.dtype, ad)
+        for i, name in enumerate(("d_residual", "d_x", "d_post", "d_pre", "d_gate")):
+            present = (True, args[1] is not None, args[4] is not None, args[3] is not None, args[6] is not None)[i]
+            assert (got[i] is not None) == present, name
+            if present:
+                P.check(got[i], *want[i], types[i], name)
+        assert torch.isfinite(got[0]).all() and (args[1] is None or torch.isfinite(got[1]).all())
