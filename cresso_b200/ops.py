@@ -18,6 +18,7 @@ from typing import Optional, Sequence, Tuple
 import numpy as np
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._host import multiscale_frequencies
@@ -264,8 +265,8 @@ def embedding_grad(grad: Tensor, tokens: Tensor, rows: int, scale: float = 1.0, 
     [row0, row0 + rows) and the token ``padding`` take no part.
 
     The result has grad's type unless ``dtype`` names another.  With ``into`` (contiguous,
-    (rows, width), usually ``param.grad``) the sums are added to it in place, rows without a
-    token are not touched, and ``into`` is returned.  Positions of a row are summed in their
+    (rows, width), usually ``param.grad``) the sums are added to it in place, which autograd
+    sees as such, rows without a token are not touched, and ``into`` is returned.  Positions of a row are summed in their
     order, in float32."""
     if tokens.dtype not in _ID_BYTES:
         raise RuntimeError(f"embedding_grad: tokens must be int32 or int64 (got {tokens.dtype})")
@@ -296,6 +297,8 @@ def embedding_grad(grad: Tensor, tokens: Tensor, rows: int, scale: float = 1.0, 
                 tokens.data_ptr(), _ID_BYTES[tokens.dtype], rows, row0, int(padding is not None),
                 0 if padding is None else padding, scale, out.data_ptr(), od, int(into is not None),
                 scratch.data_ptr(), scratch.numel())
+    if into is not None:
+        increment_version(into)  # a backward pass that kept it has to see the write
     return out
 
 
@@ -436,6 +439,8 @@ def _distill(what: str, logits: Tensor, ids: Tensor, teacher: Tensor, weight: Op
     _train_call(what, _lib.lib().cresso_distill, device, rows.data_ptr(), ld, n, vocab, stride, ids.data_ptr(),
                 _ID_BYTES[ids.dtype], teacher.data_ptr(), td, k, _address(weight), temperature, loss.data_ptr(),
                 _address(grad))
+    if inplace:
+        increment_version(logits)  # a backward pass that kept them has to see the write
     return loss, grad
 
 
@@ -462,5 +467,6 @@ def distill_grad(logits: Tensor, ids: Tensor, teacher: Tensor, weight: Optional[
         grad_v = weight * temperature * (softmax(logits / temperature)_v - sum of p_k with id_k = v)
 
     An id may occur more than once.  ``weight`` carries the mean over the batch and a loss
-    scale.  With ``inplace`` the gradient takes the place of the (contiguous) logits."""
+    scale.  With ``inplace`` the gradient takes the place of the (contiguous) logits, which
+    autograd sees as a write to them."""
     return _distill("distill_grad", logits, ids, teacher, weight, temperature, True, inplace)

@@ -93,3 +93,44 @@ def test_backward_norm_does_not_read_what_it_does_not_need(ops, width, gate_shap
             if present:
                 P.check(got[i], *want[i], types[i], name)
         assert torch.isfinite(got[0]).all() and (args[1] is None or torch.isfinite(got[1]).all())
+
+
+def test_writes_in_place_raise_the_version(ops, monkeypatch):
+    """What a call writes counts as changed for autograd, and nothing else does (no GPU: the
+    launches are left out)."""
+    monkeypatch.setattr(ops, "_train_inputs", lambda what, **tensors: 0)
+    monkeypatch.setattr(ops, "_train_call", lambda *args: None)
+    logits, ids, teacher = torch.zeros(4, 9), torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2)
+    ops.distill_grad(logits, ids, teacher)
+    ops.distill_loss(logits, ids, teacher)
+    assert logits._version == 0
+    ops.distill_grad(logits, ids, teacher, inplace=True)
+    assert logits._version == 1 and ids._version == teacher._version == 0
+    grad, tokens, into = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64), torch.zeros(6, 8)
+    ops.embedding_grad(grad, tokens, 6)
+    ops.embedding_grad(grad, tokens, 6, into=into)
+    assert into._version == 1 and grad._version == tokens._version == 0
+    with torch.inference_mode():  # tensors without a version
+        logits, into = torch.zeros(4, 9), torch.zeros(6, 8)
+        ops.distill_grad(logits, ids, teacher, inplace=True)
+        ops.embedding_grad(grad, tokens, 6, into=into)
+
+
+@gpu
+def test_writes_in_place_are_seen_by_autograd(ops):
+    """A term that kept the logits, or the tensor that a gradient is added to, for its own backward pass
+    gets an error instead of another tensor's values."""
+    leaf = _randn(1, 5, 33).requires_grad_()
+    logits = leaf * 2
+    term = torch.logsumexp(logits, -1).sum()
+    with torch.no_grad():
+        ops.distill_grad(logits, torch.zeros(5, 2, dtype=torch.int64, device="cuda"), _randn(2, 5, 2), inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        term.backward()
+    leaf = _randn(3, 7, 16).requires_grad_()
+    into = leaf * 2
+    term = into.square().sum()
+    with torch.no_grad():
+        ops.embedding_grad(_randn(4, 3, 16), torch.tensor([1, 1, 6], device="cuda"), 7, into=into)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        term.backward()
