@@ -31,6 +31,10 @@ int with_vec(int64_t width, int64_t stride, const void* p, int64_t p_bytes, cons
     return f(std::integral_constant<int, 1>());
 }
 
+// token - row0 in 64 bits is the row for every token if the window's last row has a 64-bit number; the
+// difference would wrap into a longer window from the other end.
+static bool window_ok(int64_t row0, int64_t rows) { return rows == 0 || row0 <= INT64_MAX - (rows - 1); }
+
 // ------------------------------------------------------------------ lookup ---
 //
 // Bound by memory: the distinct rows are read, every row is written.  16384 of 32000 x 4096
@@ -500,6 +504,7 @@ int cresso_embedding_gather(const void* weight, int64_t weight_dtype, int64_t ro
                    "embedding_gather: negative size, or row stride below the width");
     CRESSO_REQUIRE(n <= CRESSO_TRAIN_MAX_ROWS && rows <= CRESSO_TRAIN_MAX_ROWS, CRESSO_EUNSUPPORTED,
                    "embedding_gather: more than 2^31 - 256 tokens or rows");
+    CRESSO_REQUIRE(window_ok(row0, rows), CRESSO_EINVAL, "embedding_gather: the last row's number exceeds 64 bits");
     if (n == 0 || width == 0) return CRESSO_OK;
     CRESSO_REQUIRE((weight != nullptr || rows == 0) && tokens != nullptr && out != nullptr, CRESSO_EINVAL,
                    "embedding_gather: NULL pointer");
@@ -558,6 +563,7 @@ int cresso_embedding_grad(const void* grad, int64_t grad_dtype, int64_t n, int64
     int64_t need = 0;
     const int st = cresso_embedding_grad_scratch_bytes(n, rows, width, &need);
     if (st != CRESSO_OK) return st;
+    CRESSO_REQUIRE(window_ok(row0, rows), CRESSO_EINVAL, "embedding_grad: the last row's number exceeds 64 bits");
     if (rows == 0 || width == 0 || (n == 0 && accumulate)) return CRESSO_OK;
     CRESSO_REQUIRE(out != nullptr, CRESSO_EINVAL, "embedding_grad: NULL output");
     const cudaStream_t s = (cudaStream_t)stream;

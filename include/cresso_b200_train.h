@@ -36,7 +36,7 @@ enum { CRESSO_TRAIN_MAX_NORM_WIDTH = 65536 };  /* columns of a block norm, of at
  * is outside [0, rows).  `weight` holds the rows [row0, row0 + rows) of the
  * table (a whole table, or the local block of a row-sharded one), `weight_stride`
  * elements apart; tokens are int32 or int64 (token_bytes 4 or 8); out is
- * contiguous (n, width). */
+ * contiguous (n, width).  row0 + rows - 1 fits 64 bits. */
 CRESSO_API int cresso_embedding_gather(const void* weight, int64_t weight_dtype, int64_t rows, int64_t width,
                                        int64_t weight_stride, const void* tokens, int64_t token_bytes, int64_t n,
                                        int64_t row0, double scale, void* out, int64_t out_dtype,

@@ -134,3 +134,32 @@ def test_writes_in_place_are_seen_by_autograd(ops):
         ops.embedding_grad(_randn(4, 3, 16), torch.tensor([1, 1, 6], device="cuda"), 7, into=into)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         term.backward()
+
+
+@pytest.mark.parametrize("row0,rows,status", [(2**63 - 1, 2, 1), (2**63 - 5, 10, 1), (2**63 - 1, 2**31 - 256, 1),
+                                              (2**63 - 10, 10, 0), (2**63 - 1, 0, 0), (-2**63, 10, 0)])
+def test_windows_end_within_64_bits(row0, rows, status):
+    """A window whose last row has no 64-bit number would take tokens from the other end of the range."""
+    from cresso_b200 import _lib
+    lib, p = _lib.lib(), 4096
+    # no tokens and nothing to clear: the arguments are checked and nothing is launched
+    assert lib.cresso_embedding_gather(p, 0, rows, 8, 8, p, 8, 0, row0, 1.0, p, 0, None) == status
+    assert lib.cresso_embedding_grad(p, 0, 0, 8, 8, p, 8, rows, row0, 0, 0, 1.0, p, 0, 1, p, 1 << 20, None) == status
+
+
+@gpu
+def test_last_windows_of_64_bits(ops):
+    w = _randn(1, 4, 8)
+    tok = torch.tensor([2**63 - 1, -2**63, -2**63 + 1, 2**63 - 4, 2**63 - 5, 0], device="cuda")
+    for row0, at in ((2**63 - 4, (3, None, None, 0, None, None)), (-2**63, (None, 0, 1, None, None, None))):
+        got = ops.embedding_gather(w, tok, row0=row0)
+        grad = ops.embedding_grad(got, tok, 4, row0=row0)
+        for i, r in enumerate(at):
+            assert torch.equal(got[i], w[r] if r is not None else torch.zeros_like(w[0]))
+        for r in range(4):
+            assert torch.equal(grad[r], w[r] if r in at else torch.zeros_like(w[0]))
+    for row0 in (2**63 - 3, 2**63 - 1):
+        with pytest.raises(RuntimeError, match="64 bits"):
+            ops.embedding_gather(w, tok, row0=row0)
+        with pytest.raises(RuntimeError, match="64 bits"):
+            ops.embedding_grad(torch.zeros(6, 8, device="cuda"), tok, 4, row0=row0)
