@@ -12,7 +12,8 @@
 // every warp takes the largest of the first logits it reads, sums relative to that, and the
 // parts are joined relative to the largest reference.  The sum is then at least 1; a row whose
 // sum leaves (0.5, 1e18) (a later logit about 40 tau above its warp's reference, a row far from
-// zero, or a warp without finite logits at first) is computed again from its maximum.  Sums are
+// zero, or a warp without finite logits at first), or whose weight is tiny, is computed again from its
+// maximum.  Sums are
 // float32; an exponential below 2^-126 counts as zero.  A NaN or +inf logit makes its row NaN
 // through the sum; a row of -inf alone has q = 0.  Repeated ids: every entry
 // holds the whole P of its id, so that all of them write the same value.
@@ -158,7 +159,10 @@ __device__ __forceinline__ void join_warp(float& m, float& s, float c2) {
 // B's rounding shifts all exponents of a row by up to 2^-24 |B|, which cancels as long as it
 // is small.
 constexpr float kFar = 16777216.0f;
-constexpr float kLargeSum = 1e18f;  // its reciprocal, times a small weight, stays a normal number
+constexpr float kLargeSum = 1e18f;
+// The gradient's factor c / sum is a normal number for |c| from here on; a smaller one would lose
+// digits that the large exponentials it meets bring back.
+constexpr float kSmallFactor = 1.2e-20f;  // kLargeSum 2^-126
 
 // Loss of the row from its reference m and sum by one warp, and the gradients of the entries' ids in
 // [v0, v1) by `threads` threads.
@@ -356,8 +360,9 @@ __global__ void __launch_bounds__(THREADS + 32)
             join_warp<8>(m, s, c2);
         }
         any = *top.any;
-        if (any && !(s < kLargeSum && s > 0.5f)) {
-            // no usable reference: from the row's maximum
+        if (any && !(s < kLargeSum && s > 0.5f && (out == nullptr || fabsf(w * a.tau) >= kSmallFactor))) {
+            // no usable reference, or a factor that needs the largest exponential to be 1: from the row's
+            // maximum
             const T* part = reinterpret_cast<const T*>(words);
             m = -INFINITY;
             s = 0.0f;

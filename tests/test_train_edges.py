@@ -163,3 +163,22 @@ def test_last_windows_of_64_bits(ops):
             ops.embedding_gather(w, tok, row0=row0)
         with pytest.raises(RuntimeError, match="64 bits"):
             ops.embedding_grad(torch.zeros(6, 8, device="cuda"), tok, 4, row0=row0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_distill_weights_near_the_end_of_the_range(ops, dtype):
+    """A logit far above the ones a row begins with, times a weight that is small: the gradient is the
+    weight's size, and keeps its digits."""
+    n, vocab = 300, 32000
+    logits = torch.zeros(n, vocab, dtype=dtype, device="cuda")
+    logits[:, 15000] = 39
+    logits[1::2, 31999] = 40
+    ids, teacher = torch.arange(n, device="cuda")[:, None] + torch.tensor([5, 20000], device="cuda"), _randn(1, n, 2)
+    for size in (3e-28, 1e-27, 1e-21, 1e-19, 1e-36):
+        weight = torch.full((n,), size, device="cuda")
+        weight[::3] *= -1
+        (loss, lb), (grad, gb) = P.distill(logits, ids, teacher, weight, 1.5)
+        got_loss, got = ops.distill_grad(logits, ids, teacher, weight, 1.5)
+        P.check(got_loss, loss, lb, F32, "loss")
+        P.check(got, grad, gb, dtype, f"gradient for {size}")
