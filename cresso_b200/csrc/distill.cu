@@ -167,14 +167,16 @@ constexpr float kSmallFactor = 1.2e-20f;  // kLargeSum 2^-126
 // Loss of the row from its reference m and sum by one warp, and the gradients of the entries' ids in
 // [v0, v1) by `threads` threads.
 __device__ __forceinline__ float row_loss(const DistillArgs& a, const TopList& top, float w, float c2, float m, float s) {
-    // log q = (z - m) / tau - log of the sum relative to m, which is s but for the rounding of B; in
-    // natural units, where a masked logit of the type's lowest value is still finite
-    const float inv_tau = 1.0f / a.tau;
+    // tau log q = z - m - tau log of the sum relative to m, which is s but for the rounding of B; in the
+    // logits' units, halved, where a masked logit of the type's lowest value is finite at every
+    // temperature, and times w tau, the gradient's factor, which loses nothing beside them
     const float log_s = (s == 0.0f ? 0.0f : logf(s)) - fmaf(m, c2, -__fmul_rn(m, c2)) * kLn2;
+    const float half_m = 0.5f * m, half_tau = 0.5f * a.tau;
     float cross = 0.0f;
+#pragma unroll 1  // 40 registers for the kernel; unrolled, the float32 form took 56
     for (int k = threadIdx.x & 31; k < a.k; k += 32)
-        if (top.p[k] != 0.0f) cross += top.p[k] * ((top.z[k] - m) * inv_tau - log_s);
-    return w * a.tau * a.tau * (*top.entropy - warp_sum(cross));
+        if (top.p[k] != 0.0f) cross += top.p[k] * (0.5f * top.z[k] - half_m - half_tau * log_s);
+    return 2.0f * w * a.tau * (half_tau * *top.entropy - warp_sum(cross));
 }
 template <typename T>
 __device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopList& top, T* out, int threads, int v0, int v1,
@@ -196,7 +198,10 @@ __device__ __forceinline__ void top_gradients(const DistillArgs& a, const TopLis
 // Bound by the concurrency of loads and stores: 4096 rows of 32000 bfloat16 with their gradient take
 // 88 us, 495 MB at 5.6 TB/s.  Rows in registers (125 us) or in shared memory with the next row on
 // its way (100 us) leave fewer blocks; without any exponential the latter still took 93 us.  Six
-// blocks an SM instead of five let rows fall out of L2 (105 us, 94 with five).
+// blocks an SM instead of five let rows fall out of L2 (105 us, 94 with five), and four take 76 us
+// instead of 71 for 301 rows of 128259 float32.  Five follow from 40 registers a thread, which the
+// compiler chooses by itself (-Xptxas -v shows them): asked for by a launch bound of five blocks it
+// spilled (73 us), and the form of 64 threads got 72.
 constexpr int kDistillThreads = 256;         // without the teacher's warp
 // Bytes of a row that a block is given at least.  With the gradient, more of them are in L2 for
 // longer and fewer blocks are better: 64 KB.  The loss alone is bound by what a block does before

@@ -182,3 +182,25 @@ def test_distill_weights_near_the_end_of_the_range(ops, dtype):
         got_loss, got = ops.distill_grad(logits, ids, teacher, weight, 1.5)
         P.check(got_loss, loss, lb, F32, "loss")
         P.check(got, grad, gb, dtype, f"gradient for {size}")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tau", [0.25, 0.5, 1.0, 4.0])
+def test_distill_loss_of_masked_logits(ops, dtype, tau):
+    """The teacher's entries on logits of the type's lowest value, one of them or all: probability 0, but a
+    finite logit, so the loss is its multiple and not infinite, at temperatures below 1 too."""
+    logits, ids, teacher = _randn(1, 6, 1003, dtype=dtype), torch.arange(6 * 4, device="cuda").view(6, 4), _randn(2, 6, 4)
+    logits[0, ids[0, 1]] = torch.finfo(dtype).min
+    logits[1, ids[1]] = torch.finfo(dtype).min
+    logits[2, 30:] = torch.finfo(dtype).min
+    logits[3, :30] = torch.finfo(dtype).min
+    logits[4, :1000] = torch.finfo(dtype).min
+    # the largest loss is weight x temperature x 3.4e38, which has to be a float32 number
+    weight = torch.tensor([1.0, 0.25, 1.0, 0.125, -0.25, 1e-30], device="cuda") / max(1.0, tau)
+    (loss, lb), (grad, gb) = P.distill(logits, ids, teacher, weight, tau)
+    assert torch.isfinite(loss).all() and float(loss.abs().max()) < 3e38
+    P.check(ops.distill_loss(logits, ids, teacher, weight, tau), loss, lb, F32, "loss")
+    got_loss, got = ops.distill_grad(logits, ids, teacher, weight, tau)
+    P.check(got_loss, loss, lb, F32, "loss with gradient")
+    P.check(got, grad, gb, dtype, "gradient")
