@@ -107,7 +107,8 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __re
     // v *= an array's values at the thread's columns
     auto multiply = [&](float (&v)[NV][VEC], const void* p, int dtype, int64_t from) {
         with_any(p, dtype, [&](auto* w) {
-            constexpr int N = VEC == 1 ? 4 : NV;  // all single columns at once would spill
+            // all 16 single columns at once would spill more than the 16 to 48 bytes of this form
+            constexpr int N = VEC == 1 ? 4 : NV;
 #pragma unroll
             for (int first = 0; first < NV; first += N) {
                 float f[N][VEC];
@@ -174,7 +175,8 @@ __global__ void __launch_bounds__(512, 2) norm_kernel(NormArgs a, const TR* __re
 // and reads the same columns, 2 or 8 at an access; rows of odd width or address (VEC 1) come as the
 // 16-byte pieces that hold them, each shifted by its own offset.  Absent arrays and columns behind
 // the row are zeros there, so that nothing but the stores is guarded: 12000 float16 rows of 2051
-// take 195 us instead of 541, 16384 bfloat16 rows of 1030 88 us instead of 107.
+// take 191 us instead of 541, 16384 bfloat16 rows of 1030 80 us instead of 107.  The widest forms with a
+// gate row for each row (VEC 1 or 2, EL 16) spill up to 392 bytes.
 // Bound by memory, then by instructions: 16384 bfloat16 rows of 4096 take 132 us and 140 us with the
 // column sums, 805 MB at 5.8 TB/s; scalar float32 arithmetic and bounds checks on every access took
 // 182 us.
@@ -259,8 +261,9 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // Begins to copy the 16-byte pieces that hold src[0, count) to `dst`, which is 16-byte aligned:
 // src[i] comes to lie at dst[ahead(src) + i].  Nothing before `array`, where src's array starts,
-// is read, and nothing behind src[count - 1]: zeros follow it, eight at least.  The block's threads
-// share the pieces.
+// is read, and nothing behind src[count - 1]: at least 16 bytes of zeros follow it, more than ahead()
+// can put one row before another, so that an earlier row's end does not show behind it.  The block's
+// threads share the pieces.
 template <typename T>
 __device__ __forceinline__ int ahead(const T* src) {
     return (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
@@ -699,8 +702,8 @@ int cresso_block_norm(const void* residual, const void* x, const void* post_weig
                ok(pre_weight, wb) && ok(gate, gb);
     };
     const int vec = fits(8) ? 8 : fits(2) ? 2 : 1;
-    // single columns: 12000 bfloat16 rows of 1031 take 67 us with 8 a thread and 78 with 16, of 2051
-    // 125 and 97
+    // single columns: 12000 bfloat16 rows of 1031 take 60 us with 8 a thread and 66 with 16; of 2051 they
+    // take 133 and 138, float32 ones 110 and 85
     const NormShape p = norm_shape(width, n < kNormFewRows || (vec == 1 && width <= 2048) ? 8 : 16);
     return with_norm_types(res_dtype, act_dtype, [&](auto tr, auto tx) {
         using TR = decltype(tr);

@@ -3,8 +3,8 @@
 // Lookup: out[t] = scale * W[token_t - row0].  Gradient: dW[r] = scale * sum of
 // g[t] over the positions t whose token is row r.  The positions are brought into
 // row order by a stable counting sort (positions ascending inside a row), so every
-// row is summed in float32 in the order of its tokens: no atomics on values, the
-// same bits every run, one rounding at the end.
+// row is summed in float32 in a fixed order, that of its tokens or, for long rows, of
+// tiles of them: no atomics on values, the same bits every run, one rounding at the end.
 #include "train_common.cuh"
 
 #include <algorithm>
@@ -243,15 +243,15 @@ __global__ void __launch_bounds__(kSortMaxWarps * 32) sort_kernel(TokenWindow wi
 // even however the tokens fall.  A tile fetches its positions ahead whatever rows they
 // belong to, and writes a row's sum where the row ends.  A row of up to `tile`
 // positions belongs to the tile it begins in.  A longer one is summed tile by tile into
-// partial rows, which a second kernel adds in their order; a tile meets at most two such
+// partial rows, which a second kernel adds in a fixed order; a tile meets at most two such
 // rows, one that reaches it from the left (partial 2 tile) and one that begins inside and
 // leaves it to the right (partial 2 tile + 1).  Further items write the rows without a
 // token, kEmptyRows rows each.
 // Bound by memory: 16384 bfloat16 rows of 4096 into (32000, 4096) float32 take 116 us, of which the
 // empty rows are 70 us (a plain fill of the whole gradient takes 72) and the tiles 46 us (230 MB at
 // 5 TB/s); entries of the order read when they were needed cost 3 us.  Single columns cost
-// instructions: 16384 bfloat16 rows of 2051 into 50000 take 160 us with the sort, of 2048 62 us.  One row an item took 1264 us (a frequent row is one long chain), rows in order with
-// their own tiles 188 us.  Rows in flight in registers spilled (163 us); in shared memory, fetched
+// instructions: 16384 bfloat16 rows of 2051 into 50000 take 160 us with the sort, of 2048 62 us.  One
+// row an item took 1264 us (a frequent row is one long chain), rows in order with their own tiles 188 us.  Rows in flight in registers spilled (163 us); in shared memory, fetched
 // by the thread that adds them, they need neither registers nor a barrier.
 constexpr int kEmptyRows = 8;
 constexpr int kSumCols = 8;    // columns of a thread

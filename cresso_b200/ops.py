@@ -193,7 +193,8 @@ def _int64(value, what: str, name: str) -> int:
 
 def _row_view(t: Tensor) -> Tuple[Tensor, int, int]:
     """(tensor, number of rows, row stride) of (..., width) with the elements of a row
-    adjacent and the rows equally far apart; a copy where the strides do not allow that."""
+    adjacent and the rows equally far apart: the tensor itself if it is contiguous or has two
+    axes with such strides, else a copy."""
     width = t.shape[-1]
     n = t.numel() // width if width else 0
     if t.is_contiguous():
@@ -266,8 +267,8 @@ def embedding_grad(grad: Tensor, tokens: Tensor, rows: int, scale: float = 1.0, 
 
     The result has grad's type unless ``dtype`` names another.  With ``into`` (contiguous,
     (rows, width), usually ``param.grad``) the sums are added to it in place, which autograd
-    sees as such, rows without a token are not touched, and ``into`` is returned.  Positions of a row are summed in their
-    order, in float32."""
+    sees as such, rows without a token are not touched, and ``into`` is returned.  A row is
+    summed in float32 in a fixed order."""
     if tokens.dtype not in _ID_BYTES:
         raise RuntimeError(f"embedding_grad: tokens must be int32 or int64 (got {tokens.dtype})")
     if grad.dim() < 1 or tuple(grad.shape[:-1]) != tuple(tokens.shape):
@@ -454,7 +455,7 @@ def distill_loss(logits: Tensor, ids: Tensor, teacher: Tensor, weight: Optional[
 
     An entry is valid when 0 <= id < vocab and its logit is not -inf (pad short lists with
     id -1).  A row with weight 0, or without a valid entry, has loss 0 whatever its logits
-    hold.  A row whose student gives a teacher's entry probability 0 has loss +inf.  weight:
+    hold.  A row whose student has a logit of -inf at a teacher's entry has loss +inf.  weight:
     float32 of the leading shape, 1 when omitted; the loss is float32."""
     return _distill("distill_loss", logits, ids, teacher, weight, temperature, False, False)[0]
 

@@ -92,9 +92,9 @@ CRESSO_API int cresso_block_norm_grad(const void* h, const void* x, const void* 
  *   grad_t[v] = weight_t * temperature * (q[v] - sum of p_k with id_k = v).
  * An entry is valid when 0 <= id < vocab and u is not -inf; an id may occur more
  * than once; temperature is in [1e-6, 1e6].  A row with weight 0 or no valid entry
- * has loss 0 and gradient 0 whatever its logits hold.  A student that gives a
- * teacher entry probability 0 (a logit of -inf) has loss +inf.  ids and teacher are contiguous (n, k), ids int32 or int64,
- * weight float32 (n) or NULL (1); loss is float32 (n); grad has the logits'
+ * has loss 0 and gradient 0 whatever its logits hold.  A student with a logit of
+ * -inf at a teacher entry has loss +inf.  ids and teacher are contiguous (n, k), ids
+ * int32 or int64, weight float32 (n) or NULL (1); loss is float32 (n); grad has the logits'
  * type, contiguous (n, vocab), and may be the logits themselves when their rows
  * are contiguous; grad NULL computes the loss only. */
 CRESSO_API int cresso_distill(const void* logits, int64_t dtype, int64_t n, int64_t vocab, int64_t logits_stride,
