@@ -10,7 +10,8 @@
  * their elements, an int status (the message is read with cresso_last_error),
  * caller-owned scratch (32-byte aligned, not shared by calls that may overlap)
  * whose size is queried first, work ordered on the given stream of the current
- * device, no allocation and no synchronisation.  Outputs overlap inputs only
+ * device, no allocation and no synchronisation.  Several host threads may call
+ * them at once, each with a stream of its own.  Outputs overlap inputs only
  * where that is said.  Element types are CRESSO_DTYPE_F32, _F16 and _BF16; sums,
  * statistics and norms are float32 and every output is rounded once.  The same
  * inputs give the same bits in every run.
